@@ -56,6 +56,11 @@ extern "C" {
 #define MMB_SEG_JET 1       /* (B,K_s) one row per jet, broadcast over its N particles    */
 #define MMB_SEG_JET_MASK 2  /* (B,K_s) per jet, multiplied by maskf of the particle       */
 
+/* element types of the operators that take more than float (cross attention, head norm, 8-bit checkpoints) */
+#define MMB_DT_F32 0
+#define MMB_DT_BF16 1
+#define MMB_DT_F16 2
+
 const char* mmb_last_error(void);
 int mmb_version(void);
 
@@ -426,6 +431,30 @@ int mmb_attention_dropout_bwd(int B, int N, int H, int nheads, const float* qkv,
  * keys n, 0 at the others -- for tests that rebuild the dropped attention with another implementation. */
 int mmb_attention_dropout_mask(int B, int N, int nheads, const float* maskf, int valid_is_zero, float drop_p,
                                uint64_t seed, uint64_t offset, float* out, void* stream);
+/* Cross attention: the slots of one cloud (queries) attend to the slots of another (keys, values), another length.
+ *   s_ij = scale q_i . k_j over the kept keys j;  out_i = sum_j softmax_j(s_ij) v_j;  lse_i = log sum_j exp s_ij
+ * q, out: B*Nq rows of nheads*D; k, v: B*Nk rows of nheads_kv*D (column slices of wider rows are fine: *_ld in elements).
+ * nheads_kv divides nheads: query heads h*g .. h*g+g-1 share key head h (g = nheads / nheads_kv).  1 <= D <= 128, any
+ * lengths; dtype MMB_DT_*: q, k, v, out (sums, softmax and lse in 32 bits; with 16-bit types the probabilities are rounded
+ * to the type for the product with v).  maskf_q (B,Nq), maskf_k (B,Nk) | NULL: slots with 0 take no part -- their rows are
+ * not read (whatever they hold), a masked query gets a zero row and lse -inf, as does a query without a kept key.
+ * lse (B,nheads,Nq) | NULL.  scale > 0.  workspace: device memory of the size mmb_cross_attention_workspace gives for the
+ * same arguments (0: none), owned by this call until it has run: two calls that may overlap (streams, captured graphs)
+ * need one each. */
+int mmb_cross_attention_fwd(int B, int Nq, int Nk, int nheads, int nheads_kv, int D, int dtype, const void* q, int64_t q_ld,
+                            const void* k, int64_t k_ld, const void* v, int64_t v_ld, const float* maskf_q,
+                            const float* maskf_k, float scale, void* out, int64_t out_ld, float* lse, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+/* its reverse: dq, dk, dv (rows and types as q, k, v) are OVERWRITTEN; masked slots get zero rows.  out, lse: what the
+ * forward returned for the same inputs; dout = d loss / d out.  Sums run in a fixed order: equal inputs, equal bits. */
+int mmb_cross_attention_bwd(int B, int Nq, int Nk, int nheads, int nheads_kv, int D, int dtype, const void* q, int64_t q_ld,
+                            const void* k, int64_t k_ld, const void* v, int64_t v_ld, const float* maskf_q,
+                            const float* maskf_k, float scale, const void* out, int64_t out_ld, const void* dout,
+                            int64_t dout_ld, const float* lse, void* dq, int64_t dq_ld, void* dk, int64_t dk_ld, void* dv,
+                            int64_t dv_ld, void* workspace, int64_t workspace_bytes, void* stream);
+/* *bytes_host (HOST) = workspace of the forward (backward = 0) or the reverse (backward = 1) for these sizes */
+int mmb_cross_attention_workspace(int B, int Nq, int Nk, int nheads, int nheads_kv, int D, int dtype, int backward,
+                                  int64_t* bytes_host);
 /* The per-particle tail of one encoder layer in one launch, inference arithmetic (no dropout):
  *   h1 = LayerNorm1(h + out_proj(a));  out = LayerNorm2(h1 + linear2(relu(linear1(h1))));  qkv = in_proj_next(out)
  * (nn.TransformerEncoderLayer.forward as built at particle_transformer.py:29-35, post-LN, ReLU), replacing two
@@ -450,6 +479,41 @@ int mmb_layernorm_fwd(int64_t M, int D, const float* x, int64_t x_ld, const floa
 int mmb_layernorm_bwd(int64_t M, int D, const float* x, int64_t x_ld, const float* gamma, const float* stats,
                       const float* dy, int64_t dy_ld, float* dx, int64_t dx_ld, int accumulate, float* dgamma,
                       float* dbeta, void* stream);
+/* Norm of every query and key head together with the rotation by the rows' positions, in one pass.
+ * x, y: M rows of (nheads + nheads2) heads of D features (leading dimensions in elements; y may be x).  Per head
+ *   u = x / sqrt(mean x^2 + eps) * w      w = weight (D) for the first nheads heads, weight2 (D) for the others, NULL: ones
+ *   pair p < n_pairs of u's first 2 n_pairs features is turned by the angle pos[row][p / (n_pairs / n_axes)] * freq[p]:
+ *   (a, b) -> (a cos - b sin, a sin + b cos); pairs (p, p + n_pairs) when interleaved = 0, (2p, 2p + 1) when 1.
+ * The other features pass through.  n_pairs = 0: norm only (pos, freq unused).  pos (M, n_axes) with row stride pos_ld: any
+ * finite values -- places in a list or coordinates, one per axis --, freq (n_pairs): per-pair speeds, scaled as the caller
+ * likes.  D <= 256; dtype MMB_DT_* for x, y; weights, pos, freq and all arithmetic in 32 bits, the angle in 64. */
+int mmb_head_norm_rotate_fwd(int64_t M, int nheads, int nheads2, int D, int dtype, const void* x, int64_t x_ld,
+                             const float* weight, const float* weight2, float eps, const float* pos, int64_t pos_ld, int n_axes,
+                             const float* freq, int n_pairs, int interleaved, void* y, int64_t y_ld, void* stream);
+#define MMB_HEAD_NORM_MAX_BLOCKS 1024
+/* its reverse from the SAME x (before the norm) and dy: dx (type and rows as x; may be dy), dweight, dweight2 (D) | NULL,
+ * both OVERWRITTEN.  partials: workspace of 2 * D * MMB_HEAD_NORM_MAX_BLOCKS floats.  No gradient reaches pos and freq.
+ * Sums run in a fixed order. */
+int mmb_head_norm_rotate_bwd(int64_t M, int nheads, int nheads2, int D, int dtype, const void* x, int64_t x_ld, const void* dy,
+                             int64_t dy_ld, const float* weight, const float* weight2, float eps, const float* pos,
+                             int64_t pos_ld, int n_axes, const float* freq, int n_pairs, int interleaved, void* dx,
+                             int64_t dx_ld, float* dweight, float* dweight2, float* partials, void* stream);
+
+/* Activations kept for the reverse pass in 8 bits.  32 consecutive features of a row share a step 2^e, e the smallest
+ * exponent >= -127 with 127 * 2^e >= max |x|; codes (M, 32*ceil(K/32)) int8 = round(x / 2^e), ties to even, features past K
+ * zero; steps (M, ceil(K/32)) uint8 = e + 127, 255 for a block that holds an infinity or NaN (it is restored as NaN).
+ * |restored - x| <= 2^(e-1).  x: M rows of K, dtype MMB_DT_*.  codes 16-byte aligned. */
+int mmb_checkpoint_rows(int64_t M, int K, int dtype, const void* x, int64_t x_ld, void* codes, void* steps, void* stream);
+/* y (M, K) = code * 2^e, rounded to dtype (exact in float and bf16) */
+int mmb_restore_rows(int64_t M, int K, int dtype, const void* codes, const void* steps, void* y, int64_t y_ld, void* stream);
+/* Weight gradient of a Linear straight from its input's checkpoint: dW (N, K) = dZ^T Xhat, db (N) | NULL = column sums of
+ * dZ (M, N) (dtype MMB_DT_*); accumulate != 0: added to what dW, db hold.  Products are exact (a code times a power of two
+ * is one bf16 value, dZ is split into bf16 planes without loss), sums in 32 bits in a fixed order.  Infinite or NaN
+ * gradients give non-finite sums.  workspace: the size that mmb_grad_weight_rows_q8_workspace gives (bytes_host: HOST). */
+int mmb_grad_weight_rows_q8(int64_t M, int K, int N, int dtype, const void* codes, const void* steps, const void* dZ,
+                            int64_t dz_ld, float* dW, int64_t dw_ld, float* db, int accumulate, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+int mmb_grad_weight_rows_q8_workspace(int64_t M, int N, int K, int64_t* bytes_host);
 /* dst[i] (+)= sum_r src[r*stride + i], i < n: folds the replicated accumulators of mmb_grad_weight_rows for the
  * plain (not weight-normed) nn.Linear layers of the transformer (mmb_weight_norm_bwd_rep does it for the others). */
 int mmb_sum_replicas(int64_t n, int replicas, int64_t stride, const float* src, float* dst, int accumulate,

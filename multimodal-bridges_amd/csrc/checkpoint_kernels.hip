@@ -1,0 +1,424 @@
+// Activations kept for the reverse pass in 8 bits, and the weight gradient read from them.
+//
+// 32 consecutive features of a row share a step 2^e: e is the smallest exponent (>= -127) with 127 * 2^e >= max |x|, the
+// codes are round(x / 2^e) in [-127, 127], ties to even.  Both divisions are by powers of two, so a code depends on no
+// rounding but its own, and a value stands for at most half a step off: |xhat - x| <= 2^(e-1) <= max|x| / 127.  An integer
+// grid over a shared step holds a block of like-sized activations about four times closer than an 8-bit float would (whose
+// three mantissa bits spend the range on small values).
+// step byte = e + 127; 255 marks a block that held an infinity or a NaN: it comes back as NaN, never as a finite value.
+//
+// A code is an integer of 7 bits: code * 2^e is EXACT in bf16.  The weight gradient dW = dZ^T Xhat therefore needs ONE bf16
+// plane for Xhat and three for a float dZ (exact split, truncated 8 + 8 + 8 bits; two for fp16, one for bf16): three matrix
+// products where float activations need six, and a quarter of the bytes.
+#include "common.h"
+
+namespace mmb {
+namespace ckpt {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T> __device__ __forceinline__ float max_of();
+template <> __device__ __forceinline__ float max_of<float>() { return 3.4028234663852886e38f; }
+template <> __device__ __forceinline__ float max_of<__bf16>() { return 3.3895313892515355e38f; }
+template <> __device__ __forceinline__ float max_of<_Float16>() { return 65504.0f; }
+
+__device__ __forceinline__ float step_of(uint32_t s) {      // 2^(s - 127); s == 0: the subnormal 2^-127; 255: NaN
+  return __uint_as_float(s == 255u ? 0x7fc00000u : s == 0u ? 0x00400000u : s << 23);
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* __restrict__ p, int k, int K, float v[8]) {
+  if constexpr (VEC) {
+    if (k >= K) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    } else if constexpr (sizeof(T) == 4) {
+      const float4 a = *reinterpret_cast<const float4*>(p + k), b = *reinterpret_cast<const float4*>(p + k + 4);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      T t[8];
+      const uint4 a = *reinterpret_cast<const uint4*>(p + k);
+      __builtin_memcpy(t, &a, 16);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? (float)p[k + i] : 0.0f;
+  }
+}
+
+// a thread owns 8 features, four neighbouring lanes one block of 32
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+encode_kernel(int64_t M, int K, int nb, const T* __restrict__ x, int64_t x_ld, int8_t* __restrict__ codes, uint8_t* __restrict__ steps) {
+  const int64_t n = M * nb * 4;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
+    const int64_t blk = t >> 2, row = blk / nb;
+    const int k = (int)(blk - row * nb) * 32 + (int)(t & 3) * 8;
+    float v[8];
+    load8<T, VEC>(x + row * x_ld, k, K, v);
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
+    uint32_t s = 255u;
+    uint2 packed = make_uint2(0u, 0u);
+    if (top < 0x7f800000u) {
+      // max = 1.m 2^(E-127); 127 = 1.984375 2^6 (mantissa 0x7e0000)
+      const int e = (int)(top >> 23) - 6 + ((top & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+      s = (uint32_t)max(e, 0);
+      const float inv = __uint_as_float((254u - s) << 23);              // 2^-(s - 127), s <= 249
+      const float lim = s >= 249u ? 63.0f : 127.0f;                     // (64 * 2^122 would leave the range of a float)
+      int q[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = (int)fminf(fmaxf(rintf(v[i] * inv), -lim), lim);
+      packed.x = (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | (uint32_t)q[3] << 24;
+      packed.y = (q[4] & 255) | (q[5] & 255) << 8 | (q[6] & 255) << 16 | (uint32_t)q[7] << 24;
+    }
+    *reinterpret_cast<uint2*>(codes + t * 8) = packed;
+    if ((t & 3) == 0) steps[blk] = (uint8_t)s;
+  }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+decode_kernel(int64_t M, int K, int nb, const int8_t* __restrict__ codes, const uint8_t* __restrict__ steps, T* __restrict__ y, int64_t y_ld) {
+  const int64_t n = M * nb * 4;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
+    const int64_t blk = t >> 2, row = blk / nb;
+    const int k = (int)(blk - row * nb) * 32 + (int)(t & 3) * 8;
+    const uint2 c = *reinterpret_cast<const uint2*>(codes + t * 8);
+    const uint32_t s = steps[blk];
+    const float st = step_of(s), big = max_of<T>();
+    T o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t w = i < 4 ? c.x : c.y;
+      float f = (float)(int8_t)(w >> (8 * (i & 3))) * st;
+      if (s != 255u) f = fminf(fmaxf(f, -big), big);      // (a code next to the type's largest value may round past it)
+      o[i] = (T)f;
+    }
+    T* p = y + row * y_ld + k;
+    if constexpr (VEC) {
+      if (k < K) {
+        if constexpr (sizeof(T) == 4) {
+          *reinterpret_cast<float4*>(p) = make_float4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<float4*>(p + 4) = make_float4(o[4], o[5], o[6], o[7]);
+        } else {
+          uint4 a;
+          __builtin_memcpy(&a, o, 16);
+          *reinterpret_cast<uint4*>(p) = a;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k + i < K) p[i] = o[i];
+    }
+  }
+}
+
+// ---- dW (N, K) = dZ^T (N, M) . Xhat (M, K), db (N) = column sums of dZ -------------------------------------------
+// A workgroup owns a 128 x 128 tile of dW over a range of rows and walks the range 32 rows at a time: dZ and Xhat go to
+// LDS transposed (contraction index last) and in bf16 planes, four waves compute 64 x 64 each.  The rows are split over
+// workgroups to fill the chip; partial tiles are summed by a second launch in a fixed order (no atomics: equal inputs give
+// equal bits).
+constexpr int BN = 128, BK = 128, MS = 32, PITCH = MS + 8;
+
+template <typename T> struct Planes;
+template <> struct Planes<float> { static constexpr int n = 3; };
+template <> struct Planes<_Float16> { static constexpr int n = 2; };
+template <> struct Planes<__bf16> { static constexpr int n = 1; };
+
+struct GwArgs {
+  int64_t M;
+  int N, K, nb, nt, kt, splits;
+  int64_t rows;                                   // rows a split walks, a multiple of MS
+  const int8_t* codes;
+  const uint8_t* steps;
+  const void* dz;
+  int64_t dz_ld, codes_ld;
+  float *pw, *pb;                                 // partial sums (splits, N, K), (splits, N)
+};
+
+// four rows x four columns of dZ -> PL planes of four column vectors of four rows (two words each)
+template <typename T>
+__device__ __forceinline__ void planes4(const float v[4][4], int c, uint2* out) {
+  uint32_t b[3][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float x = v[j][c];
+    const uint32_t hi = __float_as_uint(x) & 0xffff0000u;
+    b[0][j] = hi;
+    if constexpr (Planes<T>::n > 1) {
+      const float r = x - __uint_as_float(hi);
+      const uint32_t mid = __float_as_uint(r) & 0xffff0000u;
+      b[1][j] = mid;
+      if constexpr (Planes<T>::n > 2) b[2][j] = __float_as_uint(r - __uint_as_float(mid));
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < Planes<T>::n; ++p) {
+    out[p].x = __builtin_amdgcn_perm(b[p][1], b[p][0], 0x07060302u);
+    out[p].y = __builtin_amdgcn_perm(b[p][3], b[p][2], 0x07060302u);
+  }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256, 2) gw_kernel(GwArgs a) {
+  constexpr int PL = Planes<T>::n;
+  __shared__ __attribute__((aligned(16))) uint16_t As[PL][BN * PITCH];
+  __shared__ __attribute__((aligned(16))) uint16_t Bs[BK * PITCH];
+  const int tiles = a.nt * a.kt;
+  // all tiles of one row range on one XCD (workgroup ids go round the eight): they read the same rows
+  const int64_t y = blockIdx.x >> 3;
+  const int split = (int)(y / tiles) * 8 + (int)(blockIdx.x & 7), tile = (int)(y % tiles);
+  if (split >= a.splits) return;
+  const int n0 = (tile % a.nt) * BN, k0 = (tile / a.nt) * BK;
+  const int64_t m0 = (int64_t)split * a.rows, m1 = min(a.M, m0 + a.rows);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
+  const int wn = (wave & 1) * 64, wk = (wave >> 1) * 64;
+  // loads: four rows x four columns a thread, the 32 threads of a half wave along a row
+  const int quad = threadIdx.x >> 5, c4 = (threadIdx.x & 31) * 4;
+  const bool n_ok = n0 + c4 < a.N, k_ok = k0 + c4 < a.nb * 32;
+  f32x16 acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+  float db[4] = {0, 0, 0, 0};
+  float v[4][4];
+  uint32_t cw[4], sw[4];
+  auto fetch = [&](int64_t m) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t row = m + quad * 4 + j;
+      const bool in = row < m1;
+      const T* p = (const T*)a.dz + row * a.dz_ld + n0 + c4;
+      if constexpr (VEC) {
+        if (in && n_ok) {
+          if constexpr (sizeof(T) == 4) {
+            const float4 f = *reinterpret_cast<const float4*>(p);
+            v[j][0] = f.x; v[j][1] = f.y; v[j][2] = f.z; v[j][3] = f.w;
+          } else {
+            T t[4];
+            const uint2 f = *reinterpret_cast<const uint2*>(p);
+            __builtin_memcpy(t, &f, 8);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[j][c] = (float)t[c];
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[j][c] = 0.0f;
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[j][c] = in && n0 + c4 + c < a.N ? (float)p[c] : 0.0f;
+      }
+      cw[j] = 0u;
+      sw[j] = 0u;
+      if (in && k_ok) {
+        cw[j] = *reinterpret_cast<const uint32_t*>(a.codes + row * a.codes_ld + k0 + c4);
+        sw[j] = a.steps[row * a.nb + (k0 + c4) / 32];
+      }
+    }
+  };
+  fetch(m0);
+  for (int64_t m = m0; m < m1; m += MS) {
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      uint2 w[PL];
+      planes4<T>(v, c, w);
+#pragma unroll
+      for (int p = 0; p < PL; ++p) *reinterpret_cast<uint2*>(&As[p][(c4 + c) * PITCH + quad * 4]) = w[p];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) db[c] += v[j][c];
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      uint32_t b[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = __float_as_uint((float)(int8_t)(cw[j] >> (8 * c)) * step_of(sw[j]));
+      uint2 w;
+      w.x = __builtin_amdgcn_perm(b[1], b[0], 0x07060302u);
+      w.y = __builtin_amdgcn_perm(b[3], b[2], 0x07060302u);
+      *reinterpret_cast<uint2*>(&Bs[(c4 + c) * PITCH + quad * 4]) = w;
+    }
+    if (m + MS < m1) fetch(m + MS);
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < MS / 16; ++s) {
+      u32x4 bf[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) bf[j] = *reinterpret_cast<const u32x4*>(&Bs[(wk + 32 * j + col) * PITCH + 16 * s + 8 * h]);
+#pragma unroll
+      for (int p = PL - 1; p >= 0; --p)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const bf16x8 af = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(&As[p][(wn + 32 * i + col) * PITCH + 16 * s + 8 * h]));
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af, __builtin_bit_cast(bf16x8, bf[j]), acc[i][j], 0, 0, 0);
+        }
+    }
+  }
+  float* pw = a.pw + (int64_t)split * a.N * a.K;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int n = n0 + wn + 32 * i + (r >> 2) * 8 + h * 4 + (r & 3), k = k0 + wk + 32 * j + col;
+        if (n < a.N && k < a.K) pw[(int64_t)n * a.K + k] = acc[i][j][r];
+      }
+  if (tile / a.nt == 0) {                          // column sums: the tiles of the first K window
+    float* red = reinterpret_cast<float*>(Bs);     // 8 quads x 128 columns
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 4; ++c) red[quad * BN + c4 + c] = db[c];
+    __syncthreads();
+    if (threadIdx.x < BN && n0 + threadIdx.x < a.N) {
+      float s = 0.0f;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) s += red[q * BN + threadIdx.x];
+      a.pb[(int64_t)split * a.N + n0 + threadIdx.x] = s;
+    }
+  }
+}
+
+// dW, db from the partial sums of the row ranges
+__global__ void __launch_bounds__(256)
+gw_fold_kernel(int splits, int64_t nw, int N, int K, const float* __restrict__ pw, const float* __restrict__ pb, float* __restrict__ dW,
+               int64_t dw_ld, float* __restrict__ db, int accumulate) {
+  const int64_t n = nw + N;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    float s = 0.0f;
+    if (i < nw) {
+      for (int p = 0; p < splits; ++p) s += pw[(int64_t)p * nw + i];
+      float* d = dW + i / K * dw_ld + i % K;
+      *d = accumulate ? *d + s : s;
+    } else if (db) {
+      for (int p = 0; p < splits; ++p) s += pb[(int64_t)p * N + (i - nw)];
+      db[i - nw] = accumulate ? db[i - nw] + s : s;
+    }
+  }
+}
+
+// Row ranges: enough workgroups for two on every CU, no range shorter than 8 steps, and no more partial sums than a quarter
+// of what the operands themselves hold (they are written and read once more).
+static void gw_plan(int64_t M, int N, int K, int* nt, int* kt, int* splits, int64_t* rows) {
+  *nt = (N + BN - 1) / BN;
+  *kt = (K + BK - 1) / BK;
+  const int64_t tiles = (int64_t)*nt * *kt;
+  int64_t s = (512 + tiles - 1) / tiles;
+  const int64_t most = (M + 8 * MS - 1) / (8 * MS), fit = M * ((int64_t)K + 4 * N) / (32 * (int64_t)N * K) + 1;
+  if (s > most) s = most;
+  if (s > fit) s = fit;
+  if (s < 1) s = 1;
+  *rows = (M + s * MS - 1) / (s * MS) * MS;
+  *splits = (int)((M + *rows - 1) / *rows);
+}
+
+static int check_q8(const char* who, int64_t M, int K, const void* codes, const void* steps) {
+  MMB_REQUIRE(M > 0 && K > 0 && K <= (1 << 20), "%s: M must be positive, K in 1..2^20 (got %lld, %d)", who, (long long)M, K);
+  MMB_REQUIRE(codes && steps, "%s: codes or steps is NULL", who);
+  MMB_REQUIRE(((uintptr_t)codes & 15) == 0, "%s: codes must be 16-byte aligned", who);
+  return MMB_OK;
+}
+
+template <typename T>
+static int encode(int64_t M, int K, const void* x, int64_t x_ld, void* codes, void* steps, hipStream_t st) {
+  const int nb = (K + 31) / 32, grid = stream_grid(M * nb * 4, 256);
+  const bool vec = K % 8 == 0 && ((uintptr_t)x & 15) == 0 && x_ld * (int64_t)sizeof(T) % 16 == 0;
+  if (vec) encode_kernel<T, true><<<grid, 256, 0, st>>>(M, K, nb, (const T*)x, x_ld, (int8_t*)codes, (uint8_t*)steps);
+  else encode_kernel<T, false><<<grid, 256, 0, st>>>(M, K, nb, (const T*)x, x_ld, (int8_t*)codes, (uint8_t*)steps);
+  return check_launch("mmb_checkpoint_rows");
+}
+template <typename T>
+static int decode(int64_t M, int K, const void* codes, const void* steps, void* y, int64_t y_ld, hipStream_t st) {
+  const int nb = (K + 31) / 32, grid = stream_grid(M * nb * 4, 256);
+  const bool vec = K % 8 == 0 && ((uintptr_t)y & 15) == 0 && y_ld * (int64_t)sizeof(T) % 16 == 0;
+  if (vec) decode_kernel<T, true><<<grid, 256, 0, st>>>(M, K, nb, (const int8_t*)codes, (const uint8_t*)steps, (T*)y, y_ld);
+  else decode_kernel<T, false><<<grid, 256, 0, st>>>(M, K, nb, (const int8_t*)codes, (const uint8_t*)steps, (T*)y, y_ld);
+  return check_launch("mmb_restore_rows");
+}
+template <typename T>
+static int grad_weight(GwArgs& a, float* dW, int64_t dw_ld, float* db, int accumulate, hipStream_t st) {
+  const bool vec = a.N % 4 == 0 && ((uintptr_t)a.dz & 15) == 0 && a.dz_ld * (int64_t)sizeof(T) % (4 * sizeof(T)) == 0;
+  const int64_t blocks = (int64_t)(a.splits + 7) / 8 * 8 * a.nt * a.kt;
+  MMB_REQUIRE(blocks <= 0x7fffffffLL, "mmb_grad_weight_rows_q8: %lld workgroups", (long long)blocks);
+  if (vec) gw_kernel<T, true><<<(unsigned)blocks, 256, 0, st>>>(a);
+  else gw_kernel<T, false><<<(unsigned)blocks, 256, 0, st>>>(a);
+  int rc = check_launch("mmb_grad_weight_rows_q8");
+  if (rc != MMB_OK) return rc;
+  const int64_t nw = (int64_t)a.N * a.K;
+  gw_fold_kernel<<<stream_grid(nw + a.N, 256), 256, 0, st>>>(a.splits, nw, a.N, a.K, a.pw, a.pb, dW, dw_ld, db, accumulate);
+  return check_launch("mmb_grad_weight_rows_q8 (fold)");
+}
+
+}  // namespace ckpt
+}  // namespace mmb
+
+using namespace mmb;
+using namespace mmb::ckpt;
+
+extern "C" int mmb_checkpoint_rows(int64_t M, int K, int dtype, const void* x, int64_t x_ld, void* codes, void* steps, void* stream) {
+  if (int rc = check_q8("mmb_checkpoint_rows", M, K, codes, steps)) return rc;
+  MMB_REQUIRE(x && x_ld >= K, "mmb_checkpoint_rows: x is NULL or its leading dimension smaller than its row");
+  hipStream_t st = as_stream(stream);
+  if (dtype == MMB_DT_F32) return encode<float>(M, K, x, x_ld, codes, steps, st);
+  if (dtype == MMB_DT_BF16) return encode<__bf16>(M, K, x, x_ld, codes, steps, st);
+  if (dtype == MMB_DT_F16) return encode<_Float16>(M, K, x, x_ld, codes, steps, st);
+  set_error("mmb_checkpoint_rows: unknown dtype %d", dtype);
+  return MMB_ERR_INVALID_ARG;
+}
+
+extern "C" int mmb_restore_rows(int64_t M, int K, int dtype, const void* codes, const void* steps, void* y, int64_t y_ld, void* stream) {
+  if (int rc = check_q8("mmb_restore_rows", M, K, codes, steps)) return rc;
+  MMB_REQUIRE(y && y_ld >= K, "mmb_restore_rows: y is NULL or its leading dimension smaller than its row");
+  hipStream_t st = as_stream(stream);
+  if (dtype == MMB_DT_F32) return decode<float>(M, K, codes, steps, y, y_ld, st);
+  if (dtype == MMB_DT_BF16) return decode<__bf16>(M, K, codes, steps, y, y_ld, st);
+  if (dtype == MMB_DT_F16) return decode<_Float16>(M, K, codes, steps, y, y_ld, st);
+  set_error("mmb_restore_rows: unknown dtype %d", dtype);
+  return MMB_ERR_INVALID_ARG;
+}
+
+extern "C" int mmb_grad_weight_rows_q8_workspace(int64_t M, int N, int K, int64_t* bytes_host) {
+  MMB_REQUIRE(M > 0 && N > 0 && K > 0 && bytes_host, "mmb_grad_weight_rows_q8_workspace: sizes must be positive, bytes_host not NULL");
+  int nt, kt, splits;
+  int64_t rows;
+  gw_plan(M, N, K, &nt, &kt, &splits, &rows);
+  *bytes_host = (int64_t)splits * ((int64_t)N * K + N) * 4;
+  return MMB_OK;
+}
+
+extern "C" int mmb_grad_weight_rows_q8(int64_t M, int K, int N, int dtype, const void* codes, const void* steps, const void* dZ,
+                                       int64_t dz_ld, float* dW, int64_t dw_ld, float* db, int accumulate, void* workspace,
+                                       int64_t workspace_bytes, void* stream) {
+  if (int rc = check_q8("mmb_grad_weight_rows_q8", M, K, codes, steps)) return rc;
+  MMB_REQUIRE(N > 0 && N <= (1 << 20) && dZ && dz_ld >= N && dW && dw_ld >= K,
+              "mmb_grad_weight_rows_q8: N in 1..2^20, dZ, dW not NULL, leading dimensions no smaller than their rows");
+  GwArgs a = {M, N, K, (K + 31) / 32, 0, 0, 0, 0, (const int8_t*)codes, (const uint8_t*)steps, dZ, dz_ld, 0, nullptr, nullptr};
+  a.codes_ld = (int64_t)a.nb * 32;
+  gw_plan(M, N, K, &a.nt, &a.kt, &a.splits, &a.rows);
+  const int64_t need = (int64_t)a.splits * ((int64_t)N * K + N) * 4;
+  MMB_REQUIRE(workspace && workspace_bytes >= need, "mmb_grad_weight_rows_q8: workspace of %lld bytes needed, got %lld", (long long)need,
+              (long long)(workspace ? workspace_bytes : 0));
+  a.pw = (float*)workspace;
+  a.pb = a.pw + (int64_t)a.splits * N * K;
+  hipStream_t st = as_stream(stream);
+  if (dtype == MMB_DT_F32) return grad_weight<float>(a, dW, dw_ld, db, accumulate, st);
+  if (dtype == MMB_DT_BF16) return grad_weight<__bf16>(a, dW, dw_ld, db, accumulate, st);
+  if (dtype == MMB_DT_F16) return grad_weight<_Float16>(a, dW, dw_ld, db, accumulate, st);
+  set_error("mmb_grad_weight_rows_q8: unknown dtype %d", dtype);
+  return MMB_ERR_INVALID_ARG;
+}

@@ -1,0 +1,419 @@
+// Shared parts of the cross-attention kernels (cross_attention.hip: forward, cross_attention_bwd.hip: reverse).
+//
+// Both passes are built from 32x32 matrix-core tiles in which a lane owns one COLUMN of the score matrix:
+//   forward / dq :  S^T (keys x queries)  = K Q^T      a lane holds 16 keys of one query per tile
+//   dk, dv       :  S   (queries x keys)  = Q K^T      a lane holds 16 queries of one key per tile
+// so softmax statistics are per-lane scalars, and the accumulator registers of S (or P, dS) ARE the B operand of the
+// next product: 32x32x16 wants, for one column, eight consecutive contraction indices per lane half, the accumulator
+// holds {4h..4h+3, 8+4h..8+4h+3} of every 16 -- a permutation of the contraction index, which the A operand (stored
+// transposed in LDS) is written with.  No cross-lane traffic, no LDS round trip for P.
+#pragma once
+#include "common.h"
+
+namespace mmb {
+namespace xattn {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// row of accumulator register r in a 32x32 tile, for lane half h
+__device__ __forceinline__ int crow(int r, int h) { return (r >> 2) * 8 + h * 4 + (r & 3); }
+
+template <typename T> struct Traits;
+template <> struct Traits<float> { static constexpr int EPC = 4; };       // elements of one 16-byte chunk
+template <> struct Traits<__bf16> { static constexpr int EPC = 8; };
+template <> struct Traits<_Float16> { static constexpr int EPC = 8; };
+
+// 8 (16-bit types) or 4 (float) elements, one 16-byte chunk
+template <typename T, bool VEC>
+__device__ __forceinline__ u32x4 load_chunk(const T* __restrict__ p, int d, int D, bool ok) {
+  constexpr int E = Traits<T>::EPC;
+  u32x4 r = {0u, 0u, 0u, 0u};
+  if constexpr (VEC) {
+    if (ok && d < D) r = *reinterpret_cast<const u32x4*>(p + d);
+  } else {
+    if (ok) {
+      T t[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) t[i] = d + i < D ? p[d + i] : (T)0.0f;
+      __builtin_memcpy(&r, t, 16);
+    }
+  }
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (sizeof(T) == 2) {
+    if constexpr (__is_same(T, __bf16))
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  } else {
+    // four steps of two: lane half h supplies contraction indices 4h .. 4h+3 of the eight that the chunk pair covers
+    const f32x4 af = __builtin_bit_cast(f32x4, a), bf = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(af[i], bf[i], c, 0, 0, 0);
+    return c;
+  }
+}
+
+// eight accumulator values, rounded to T (nearest even): one B operand of the next product
+template <typename T>
+__device__ __forceinline__ u32x4 pack8(const f32x16& s, int r0) {
+  T t[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = (T)s[r0 + i];
+  u32x4 r;
+  __builtin_memcpy(&r, t, 16);
+  return r;
+}
+
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.0f;
+  return z;
+}
+
+// LDS hand-over inside one wave (in order in hardware; the fence keeps the compiler from moving accesses across)
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+constexpr int kChunk = 512;                       // raw slots one compaction step looks at
+
+// Appends the slots n in [lo, min(lo + kChunk, hi)) with maskf[n] != 0 to list[], in order; returns how many.
+// One wave; all eight loads are in flight together.
+__device__ __forceinline__ int compact_chunk(const float* __restrict__ maskf, int lo, int hi, int* list) {
+  const int lane = threadIdx.x & 63;
+  float f[kChunk / 64];
+#pragma unroll
+  for (int c = 0; c < kChunk / 64; ++c) {
+    const int n = lo + c * 64 + lane;
+    f[c] = n < hi ? maskf[n] : 0.0f;
+  }
+  int at = 0;
+#pragma unroll
+  for (int c = 0; c < kChunk / 64; ++c) {
+    const bool ok = f[c] != 0.0f;
+    const unsigned long long bal = __ballot(ok);
+    if (ok) list[at + __popcll(bal & ((1ull << lane) - 1ull))] = lo + c * 64 + lane;
+    at += __popcll(bal);
+  }
+  return at;
+}
+
+// list[i] = slot of the (first + i)-th kept slot of maskf[0, N), for i < n; -1 where there is none.  One wave.
+__device__ __forceinline__ void compact_select(const float* __restrict__ maskf, int N, int first, int n, int* list) {
+  const int lane = threadIdx.x & 63;
+  for (int i = lane; i < n; i += 64) list[i] = -1;
+  wave_sync();
+  int at = 0;
+  for (int lo = 0; lo < N && at < first + n; lo += kChunk) {
+    float f[kChunk / 64];
+#pragma unroll
+    for (int c = 0; c < kChunk / 64; ++c) {
+      const int s = lo + c * 64 + lane;
+      f[c] = s < N ? maskf[s] : 0.0f;
+    }
+#pragma unroll
+    for (int c = 0; c < kChunk / 64; ++c) {
+      const bool ok = f[c] != 0.0f;
+      const unsigned long long bal = __ballot(ok);
+      const int o = at + __popcll(bal & ((1ull << lane) - 1ull)) - first;
+      if (ok && o >= 0 && o < n) list[o] = lo + c * 64 + lane;
+      at += __popcll(bal);
+    }
+  }
+}
+
+// The kept slots of [lo, hi), handed out in tiles.  list: LDS, kChunk + 64 ints, shared by the TEAM waves that walk
+// together (TEAM == 1: one wave on its own).  Without a mask nothing is listed: slot(i) is lo + i.
+template <int TEAM>
+struct SlotTiles {
+  const float* maskf;
+  int raw, hi, head, cnt;
+  int* list;
+  int* cnt_sh;
+  __device__ __forceinline__ void init(const float* m, int lo, int hi_, int* l, int* c) {
+    maskf = m; raw = lo; hi = hi_; head = cnt = 0; list = l; cnt_sh = c;
+  }
+  static __device__ __forceinline__ void sync() {
+    if constexpr (TEAM == 1) wave_sync();
+    else __syncthreads();
+  }
+  // number of slots of the next tile (0: done); slot(i), i < number, stays valid until the next call
+  __device__ __forceinline__ int next(int tile) {
+    if (maskf == nullptr) {
+      head = raw;
+      const int n = min(tile, hi - raw);
+      raw += max(n, 0);
+      return max(n, 0);
+    }
+    head += cur;
+    cur = 0;
+    while (cnt - head < tile && raw < hi) {
+      sync();                                     // everyone is done with the list
+      if (TEAM == 1 || threadIdx.x < 64) {
+        const int lane = threadIdx.x & 63, left = cnt - head;      // left < tile <= 64: one slot a lane
+        const int keep = lane < left ? list[head + lane] : 0;
+        wave_sync();
+        if (lane < left) list[lane] = keep;
+        wave_sync();
+        const int c = left + compact_chunk(maskf, raw, hi, list + left);
+        if (TEAM > 1 && lane == 0) *cnt_sh = c;
+        if (TEAM == 1) cnt = c;
+      }
+      sync();
+      if constexpr (TEAM > 1) cnt = *cnt_sh;
+      head = 0;
+      raw += kChunk;
+    }
+    cur = min(tile, cnt - head);
+    return cur;
+  }
+  __device__ __forceinline__ int slot(int i) const { return maskf == nullptr ? head + i : list[head + i]; }
+  int cur = 0;
+};
+
+// ---- one tile of rows in LDS -------------------------------------------------------------------------------------
+// Row-major:   [ROWS][DP + pad]; 16-byte chunks; pitch 4 words past a multiple of 64 banks: b128 reads of 32 rows at one
+//              chunk column spread over all banks.
+// Transposed:  [DP][ROWS + 8] (16-bit types only), the row index permuted inside every 16 as the accumulators hold it.
+template <typename T, int DP> constexpr int row_pitch() { return DP + (sizeof(T) == 2 ? 8 : 4); }
+template <int ROWS> constexpr int tr_pitch() { return ROWS + 8; }
+
+// position of row 4*quad inside a transposed row
+__device__ __forceinline__ int tr_pos(int quad) { return (quad >> 2) * 16 + (quad & 1) * 8 + ((quad >> 1) & 1) * 4; }
+
+// four rows x eight columns (16-bit) -> eight columns x four rows
+__device__ __forceinline__ void transpose_store(const u32x4 r[4], uint16_t* dst, int pitch) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint2 lo, hi;
+    lo.x = __builtin_amdgcn_perm(r[1][w], r[0][w], 0x05040100u);
+    lo.y = __builtin_amdgcn_perm(r[3][w], r[2][w], 0x05040100u);
+    hi.x = __builtin_amdgcn_perm(r[1][w], r[0][w], 0x07060302u);
+    hi.y = __builtin_amdgcn_perm(r[3][w], r[2][w], 0x07060302u);
+    *reinterpret_cast<uint2*>(dst + (2 * w) * pitch) = lo;
+    *reinterpret_cast<uint2*>(dst + (2 * w + 1) * pitch) = hi;
+  }
+}
+
+// Registers of one thread's share of a ROWS x DP tile: items of four rows x one chunk column.
+template <typename T, int DP, int ROWS, int NT>
+struct TileRegs {
+  static constexpr int E = Traits<T>::EPC, CH = DP / E, QUADS = ROWS / 4, ITEMS = QUADS * CH, PER = (ITEMS + NT - 1) / NT;
+  u32x4 r[PER][4];
+  // item -> (quad, chunk): four chunk columns of one quad beside each other (64 contiguous bytes of a row), then the quads
+  static __device__ __forceinline__ void where(int it, int& quad, int& ch) {
+    constexpr int C4 = CH < 4 ? CH : 4;
+    const int c = it % C4, rest = it / C4;
+    quad = rest % QUADS;
+    ch = (rest / QUADS) * C4 + c;
+  }
+  template <bool VEC, typename RowOf>
+  __device__ __forceinline__ void load(int tid, int n, int D, RowOf row_of) {
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int it = p * NT + tid;
+      int quad, ch;
+      where(it, quad, ch);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = quad * 4 + j;
+        const bool ok = row < n && (ITEMS % NT == 0 || it < ITEMS);
+        r[p][j] = load_chunk<T, VEC>(ok ? row_of(row) : nullptr, ch * E, D, ok);
+      }
+    }
+  }
+  __device__ __forceinline__ void store_rows(int tid, T* dst) const {
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int it = p * NT + tid;
+      if (ITEMS % NT != 0 && it >= ITEMS) break;
+      int quad, ch;
+      where(it, quad, ch);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<u32x4*>(dst + (quad * 4 + j) * row_pitch<T, DP>() + ch * E) = r[p][j];
+    }
+  }
+  __device__ __forceinline__ void store_tr(int tid, T* dst) const {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int p = 0; p < PER; ++p) {
+        const int it = p * NT + tid;
+        if (ITEMS % NT != 0 && it >= ITEMS) break;
+        int quad, ch;
+        where(it, quad, ch);
+        transpose_store(r[p], reinterpret_cast<uint16_t*>(dst) + ch * E * tr_pitch<ROWS>() + tr_pos(quad), tr_pitch<ROWS>());
+      }
+    }
+  }
+};
+
+// acc (32 x 32, register rows = contraction-major) += A_rows[row0 .. row0+31][:] . b, over the DP features of b's chunks
+template <typename T, int DP>
+__device__ __forceinline__ f32x16 dot_rows(const T* __restrict__ rows, int row0, const u32x4* b, f32x16 acc) {
+  constexpr int E = Traits<T>::EPC;
+  const int lane = threadIdx.x & 63;
+  const T* p = rows + (row0 + (lane & 31)) * row_pitch<T, DP>() + (lane >> 5) * E;
+#pragma unroll
+  for (int s = 0; s < DP / (2 * E); ++s) acc = mfma<T>(*reinterpret_cast<const u32x4*>(p + s * 2 * E), b[s], acc);
+  return acc;
+}
+
+// out[t] (features 32t.. x columns) += X^T . w, the contraction over the 32 rows row0.. that w's registers run over.
+// 16-bit: X from its transposed copy; float: X row-major, one element a lane and step.
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void dot_cols(const T* __restrict__ x, int row0, const f32x16& w, f32x16* out) {
+  const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const u32x4 b = pack8<T>(w, 8 * g);
+#pragma unroll
+      for (int t = 0; t < DP / 32; ++t)
+        out[t] = mfma<T>(*reinterpret_cast<const u32x4*>(x + (32 * t + col) * tr_pitch<ROWS>() + row0 + 16 * g + 8 * h), b, out[t]);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+      for (int t = 0; t < DP / 32; ++t)
+        out[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[(row0 + crow(r, h)) * row_pitch<T, DP>() + 32 * t + col], w[r], out[t], 0, 0, 0);
+  }
+}
+
+// chunks of one row as a B operand: chunk s of lane half h covers features (2s + h) * E ..
+template <typename T, int DP, bool VEC>
+__device__ __forceinline__ void load_row(u32x4* b, const T* __restrict__ p, int D, bool ok) {
+  constexpr int E = Traits<T>::EPC;
+  const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int s = 0; s < DP / (2 * E); ++s) b[s] = load_chunk<T, VEC>(p, (2 * s + h) * E, D, ok);
+}
+
+// a 32-bit value rounded to T.  The barrier keeps the compiler from folding the product before it into a mixed-precision
+// multiply in some instances and not in others (one rounding or two: results would depend on the alignment of a row).
+template <typename T>
+__device__ __forceinline__ T round_to(float x) {
+  if constexpr (__is_same(T, _Float16)) asm("" : "+v"(x));
+  return (T)x;
+}
+
+// Half precision holds nothing below 2^-24: gradients of scores (a probability times a small number) would vanish.  A lane's
+// column of them is scaled by a power of two, chosen from the largest magnitude so far (kept between 2^12 and 2^14), and so is
+// what the column has summed; values 2^-38 below the largest are lost, which is below the sum's own rounding.
+struct ColScale {
+  float sc = 0x1p100f;
+  __device__ __forceinline__ void fit(f32x16& w, f32x16* acc, int n_acc) {
+    float top = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(w[r]));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    if (__any(top * sc >= 0x1p14f)) {
+      const int ex = (int)(__float_as_uint(top) >> 23);                       // 2^(ex - 127) <= top
+      const float want = __uint_as_float((uint32_t)min(max(266 - ex, 27), 227) << 23);   // top * want in [2^12, 2^13)
+      const float nw = top * sc >= 0x1p14f ? fminf(want, sc) : sc;
+      const float f = nw / sc;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        if (t < n_acc)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[t][r] *= f;
+      sc = nw;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) w[r] *= sc;
+  }
+};
+
+// column `lane & 31` of acc (features x columns) times mul -> one row of D features
+template <typename T, int DP, bool VEC>
+__device__ __forceinline__ void store_col(T* __restrict__ p, const f32x16* acc, float mul, int D) {
+  const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * t + 8 * g + 4 * h;
+      T v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = round_to<T>(acc[t][4 * g + i] * mul);
+      if constexpr (VEC) {                        // D is a multiple of the chunk: four features are in or out together
+        if (d < D) __builtin_memcpy(__builtin_assume_aligned(p + d, 4 * sizeof(T)), v, 4 * sizeof(T));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (d + i < D) p[d + i] = v[i];
+      }
+    }
+}
+
+// Workgroup id -> (unit, item): units (clouds, or (cloud, key head) pairs when there are few clouds) are dealt to the
+// eight XCDs in turn and all items of a unit stay on one XCD, whose L2 then holds the rows they share.
+struct GridMap {
+  int units, items, swizzle;
+  __host__ __device__ int64_t blocks() const { return (int64_t)(swizzle ? (units + 7) / 8 * 8 : units) * items; }
+  __device__ __forceinline__ bool decode(int64_t id, int& unit, int& item) const {
+    if (!swizzle) {
+      unit = (int)(id / items);
+      item = (int)(id - (int64_t)unit * items);
+      return true;
+    }
+    const int64_t y = id >> 3;
+    unit = (int)(y / items) * 8 + (int)(id & 7);
+    item = (int)(y % items);
+    return unit < units;
+  }
+};
+inline GridMap grid_map(int B, int nkv, int per_head) {
+  GridMap g;
+  if (B % 8 == 0 || B >= 64) g = {B, nkv * per_head, 1};
+  else if ((int64_t)B * nkv >= 64 || (B * nkv) % 8 == 0) g = {B * nkv, per_head, 1};
+  else g = {B * nkv, per_head, 0};
+  return g;
+}
+
+// zeros in the rows r0 .. r0 + rows - 1 (row = slot * g + head of the group) whose slot the mask drops
+template <int NT, typename T>
+__device__ __forceinline__ void zero_masked_rows(T* __restrict__ out, int64_t ld, const float* __restrict__ maskf, int r0, int rows,
+                                                 int g, int D) {
+  const int work = rows * D;
+  for (int e = threadIdx.x; e < work; e += NT) {
+    const int r = e / D, d = e - r * D, n = (r0 + r) / g, gi = (r0 + r) - n * g;
+    if (maskf[n] == 0.0f) out[(int64_t)n * ld + gi * D + d] = (T)0.0f;
+  }
+}
+
+// the rows of a tile: list of compacted slots (from first_c on), row -> (slot, head of the group)
+struct RowTile {
+  int first_c, g;
+  const int* list;
+  __device__ __forceinline__ bool locate(int r, int N, bool masked, int& n, int& gi) const {
+    const int c = r / g;
+    gi = r - c * g;
+    n = masked ? list[c - first_c] : (c < N ? c : -1);
+    return n >= 0;
+  }
+};
+
+struct Shape {
+  int B, Nq, Nk, nh, nkv, D, g;                   // g = nh / nkv query heads share one key head
+};
+
+inline int pad_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+int check_shape(const char* who, int B, int Nq, int Nk, int nh, int nkv, int D, int dtype, float scale);
+inline bool chunk_aligned(const void* p, int64_t ld, int es) { return ((uintptr_t)p & 15) == 0 && ld * es % 16 == 0; }
+
+}  // namespace xattn
+}  // namespace mmb

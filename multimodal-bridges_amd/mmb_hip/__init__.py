@@ -124,6 +124,21 @@ SIGNATURES = {
     "mmb_sum_replicas": [C.c_int64, C.c_int, C.c_int64, c_f32p, c_f32p, C.c_int, c_stream],
     "mmb_adamw_clip_step": [C.c_int64, C.c_int64, c_f32p, c_f32p, c_f32p, c_f32p, C.c_float, C.c_float, C.c_float,
                             C.c_float, C.c_float, C.c_int64, C.c_float, c_f32p, c_f32p, C.c_int, c_stream],
+    "mmb_cross_attention_fwd": [C.c_int] * 7 + [C.c_void_p, C.c_int64] * 3 + [c_f32p, c_f32p, C.c_float, C.c_void_p, C.c_int64,
+                                c_f32p, C.c_void_p, C.c_int64, c_stream],
+    "mmb_cross_attention_bwd": [C.c_int] * 7 + [C.c_void_p, C.c_int64] * 3 + [c_f32p, c_f32p, C.c_float] +
+                               [C.c_void_p, C.c_int64] * 2 + [c_f32p] + [C.c_void_p, C.c_int64] * 4 + [c_stream],
+    "mmb_cross_attention_workspace": [C.c_int] * 8 + [C.POINTER(C.c_int64)],
+    "mmb_head_norm_rotate_fwd": [C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int64, c_f32p, c_f32p, C.c_float,
+                                 c_f32p, C.c_int64, C.c_int, c_f32p, C.c_int, C.c_int, C.c_void_p, C.c_int64, c_stream],
+    "mmb_head_norm_rotate_bwd": [C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                 c_f32p, c_f32p, C.c_float, c_f32p, C.c_int64, C.c_int, c_f32p, C.c_int, C.c_int, C.c_void_p,
+                                 C.c_int64, c_f32p, c_f32p, c_f32p, c_stream],
+    "mmb_checkpoint_rows": [C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, c_stream],
+    "mmb_restore_rows": [C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, c_stream],
+    "mmb_grad_weight_rows_q8": [C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, c_f32p,
+                                C.c_int64, c_f32p, C.c_int, C.c_void_p, C.c_int64, c_stream],
+    "mmb_grad_weight_rows_q8_workspace": [C.c_int64, C.c_int, C.c_int, C.POINTER(C.c_int64)],
     "mmb_toy_rows": [C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, c_f32p, C.c_int64, c_f32p, c_i64p, c_f32p, c_f32p,
                      c_stream],
     "mmb_toy_embedding_bwd": [C.c_int64, C.c_int, C.c_int, c_i64p, c_f32p, C.c_int64, C.c_int, c_f32p, c_stream],

@@ -671,6 +671,239 @@ def sum_replicas(src, dst, accumulate=False):
     return dst
 
 
+# ------------------------------------------------------------------------ conditional transformer
+DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _rows(t, name, dtype=None, rows=None, width=None, device=None):
+    """Checks a 2-D row matrix (a column slice of a wider one is fine) and returns its address and leading dimension."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        raise MMBError(f"{name}: expected a 2-D tensor of rows")
+    if not t.is_cuda:
+        raise MMBError(f"{name}: tensor lives on {t.device}; the HIP path has no CPU fallback")
+    if t.dtype not in DT or (dtype is not None and t.dtype != dtype):
+        raise MMBError(f"{name}: expected dtype {dtype or 'float32, bfloat16 or float16'}, got {t.dtype}")
+    if device is not None and t.device != device:
+        raise MMBError(f"{name}: tensor lives on {t.device}, the call's other tensors on {device}")
+    if (rows is not None and t.shape[0] != rows) or (width is not None and t.shape[1] != width):
+        raise MMBError(f"{name}: expected {rows if rows is not None else '(any)'} rows of "
+                       f"{width if width is not None else '(any)'}, got {tuple(t.shape)}")
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        raise MMBError(f"{name}: unit inner stride required")
+    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if ld < t.shape[1]:
+        raise MMBError(f"{name}: rows overlap (row stride {ld}, width {t.shape[1]})")
+    return t.data_ptr(), ld
+
+
+def _vec(t, name, n, device):
+    """float32 vector of n elements (or None) on the call's device"""
+    if t is not None and t.device != device:
+        raise MMBError(f"{name}: tensor lives on {t.device}, the call's other tensors on {device}")
+    if t is not None and t.numel() != n:
+        raise MMBError(f"{name}: expected {n} elements, got {t.numel()}")
+    return f32(t, name)
+
+
+def _key_mask(mi, name, B, N, device):
+    if mi is None:
+        return None
+    if mi.B != B or mi.N != N:
+        raise MMBError(f"{name}: mask of {mi.B} x {mi.N} slots for {B} x {N} rows")
+    return _vec(mi.maskf, name, B * N, device)
+
+
+def _xattn_args(q, k, v, B, nheads, nheads_kv, scale):
+    nkv = nheads if nheads_kv is None else nheads_kv
+    if B <= 0 or nheads <= 0 or nkv <= 0 or nheads % nkv:
+        raise MMBError(f"cross_attention: B = {B}, nheads = {nheads} must be positive and a multiple of nheads_kv = {nkv}")
+    qp = _rows(q, "q")
+    if q.shape[0] % B or q.shape[1] % nheads or q.numel() == 0:
+        raise MMBError(f"cross_attention: q of shape {tuple(q.shape)} is not {B} clouds of {nheads} heads")
+    D = q.shape[1] // nheads
+    kp = _rows(k, "k", q.dtype, None, nkv * D, q.device)
+    vp = _rows(v, "v", q.dtype, k.shape[0], nkv * D, q.device)
+    if k.shape[0] % B or k.shape[0] == 0:
+        raise MMBError(f"cross_attention: {k.shape[0]} key rows are not {B} clouds")
+    scale = D ** -0.5 if scale is None else float(scale)
+    return nkv, D, q.shape[0] // B, k.shape[0] // B, scale, qp + kp + vp
+
+
+def _workspace(name, *args, device):
+    n = C.c_int64(0)
+    call(name, *args, C.byref(n))
+    return (torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None), n.value
+
+
+def cross_attention_fwd(q, k, v, B, nheads, nheads_kv=None, mq=None, mk=None, scale=None, want_lse=False, out=None):
+    """Cross attention: the slots of B clouds attend to the slots of B others, of another length.
+    q (B*Nq, nheads*D); k, v (B*Nk, nheads_kv*D), e.g. column slices of one projection's rows; float32, bfloat16 or float16.
+    nheads_kv divides nheads: groups of query heads share a key head.  mq, mk: MaskInfo of the query / key slots (None: all
+    real); padded keys take no part, padded queries get zero rows (whatever the padded rows hold), as does a query without a
+    key.  scale: D ** -0.5 by default.  Returns out (B*Nq, nheads*D), with want_lse (out, lse (B, nheads, Nq) float32)."""
+    nkv, D, Nq, Nk, scale, ptrs = _xattn_args(q, k, v, B, nheads, nheads_kv, scale)
+    dev = q.device
+    with torch.cuda.device(dev):
+        if out is None:
+            out = torch.empty(B * Nq, nheads * D, dtype=q.dtype, device=dev)
+        op = _rows(out, "out", q.dtype, B * Nq, nheads * D, dev)
+        lse = torch.empty(B, nheads, Nq, dtype=torch.float32, device=dev) if want_lse else None
+        shape = (B, Nq, Nk, nheads, nkv, D, DT[q.dtype])
+        ws, n = _workspace("mmb_cross_attention_workspace", *shape, 0, device=dev)
+        call("mmb_cross_attention_fwd", *shape, *ptrs, _key_mask(mq, "mq", B, Nq, dev), _key_mask(mk, "mk", B, Nk, dev), _fl(scale),
+             *op, f32(lse), None if ws is None else ws.data_ptr(), n, stream())
+    return (out, lse) if want_lse else out
+
+
+def cross_attention_bwd(q, k, v, out, dout, lse, B, nheads, nheads_kv=None, mq=None, mk=None, scale=None, dq=None, dk=None,
+                        dv=None):
+    """(dq, dk, dv) of cross_attention_fwd from its out, lse and dout = d loss / d out; the arguments as there.  Gradients
+    are overwritten (dq, dk, dv given: rows that may be column slices), zero for padded slots.  Equal inputs, equal bits."""
+    nkv, D, Nq, Nk, scale, ptrs = _xattn_args(q, k, v, B, nheads, nheads_kv, scale)
+    dev = q.device
+    with torch.cuda.device(dev):
+        dq = torch.empty(B * Nq, nheads * D, dtype=q.dtype, device=dev) if dq is None else dq
+        dk = torch.empty(B * Nk, nkv * D, dtype=q.dtype, device=dev) if dk is None else dk
+        dv = torch.empty(B * Nk, nkv * D, dtype=q.dtype, device=dev) if dv is None else dv
+        o = [_rows(t, name, q.dtype, B * n, h * D, dev) for t, name, n, h in
+             ((out, "out", Nq, nheads), (dout, "dout", Nq, nheads), (dq, "dq", Nq, nheads), (dk, "dk", Nk, nkv), (dv, "dv", Nk, nkv))]
+        shape = (B, Nq, Nk, nheads, nkv, D, DT[q.dtype])
+        ws, n = _workspace("mmb_cross_attention_workspace", *shape, 1, device=dev)
+        call("mmb_cross_attention_bwd", *shape, *ptrs, _key_mask(mq, "mq", B, Nq, dev), _key_mask(mk, "mk", B, Nk, dev), _fl(scale),
+             *o[0], *o[1], _vec(lse, "lse", B * nheads * Nq, dev), *o[2], *o[3], *o[4], ws.data_ptr(), n, stream())
+    return dq, dk, dv
+
+
+ROTATE_LAYOUTS = {"half": 0, "interleaved": 1}
+
+
+def _head_args(x, nheads, weight, nheads2, weight2, eps, pos, freq, layout):
+    xp = _rows(x, "x")
+    if nheads <= 0 or nheads2 < 0 or x.shape[0] == 0 or x.shape[1] == 0 or x.shape[1] % (nheads + nheads2):
+        raise MMBError(f"head_norm_rotate: x of shape {tuple(x.shape)} is not rows of {nheads} + {nheads2} heads")
+    if layout not in ROTATE_LAYOUTS:
+        raise MMBError(f"head_norm_rotate: unknown layout {layout!r}")
+    if (pos is None) != (freq is None):
+        raise MMBError("head_norm_rotate: pos and freq come together")
+    D = x.shape[1] // (nheads + nheads2)
+    pp, n_pairs, axes = (None, 0), 0, 0
+    if pos is not None:
+        if pos.dtype != torch.float32:
+            raise MMBError(f"pos: expected dtype torch.float32, got {pos.dtype}")
+        pp, n_pairs, axes = _rows(pos, "pos", torch.float32, x.shape[0], None, x.device), freq.numel(), pos.shape[1]
+    args = (x.shape[0], nheads, nheads2, D, DT[x.dtype])
+    tail = (_vec(weight, "weight", D, x.device), _vec(weight2, "weight2", D, x.device), _fl(eps), *pp, axes,
+            _vec(freq, "freq", n_pairs, x.device), n_pairs, ROTATE_LAYOUTS[layout])
+    return D, args, xp, tail
+
+
+def head_norm_rotate_fwd(x, nheads, weight=None, nheads2=0, weight2=None, eps=1e-6, pos=None, freq=None, layout="half", out=None):
+    """Every head of x (M, (nheads + nheads2) * D) divided by its root mean square, times weight (D; weight2 for the last
+    nheads2 heads: the keys of packed [q | k] rows; None: ones), then turned by the row's position.
+    pos (M, axes) float32, freq (pairs) float32: pair p of the first 2 * pairs features of a head turns by
+    pos[row, p // (pairs // axes)] * freq[p]; layout "half" pairs (p, p + pairs), "interleaved" (2p, 2p + 1).  The
+    particles' own (eta, phi) as positions make scores depend on distances in that plane.  out may be x."""
+    D, args, xp, tail = _head_args(x, nheads, weight, nheads2, weight2, eps, pos, freq, layout)
+    with torch.cuda.device(x.device):
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+        op = _rows(out, "out", x.dtype, x.shape[0], x.shape[1], x.device)
+        call("mmb_head_norm_rotate_fwd", *args, *xp, *tail, *op, stream())
+    return out
+
+
+HEAD_NORM_MAX_BLOCKS = 1024
+
+
+def head_norm_rotate_bwd(x, dy, nheads, weight=None, nheads2=0, weight2=None, eps=1e-6, pos=None, freq=None, layout="half", dx=None):
+    """(dx, dweight, dweight2) of head_norm_rotate_fwd from its INPUT x and dy; a weight that was None has gradient None.
+    dx may be dy.  No gradient reaches pos and freq."""
+    D, args, xp, tail = _head_args(x, nheads, weight, nheads2, weight2, eps, pos, freq, layout)
+    dev = x.device
+    with torch.cuda.device(dev):
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if dx is None else dx
+        gp = _rows(dy, "dy", x.dtype, x.shape[0], x.shape[1], dev)
+        op = _rows(dx, "dx", x.dtype, x.shape[0], x.shape[1], dev)
+        dw = [torch.empty(D, dtype=torch.float32, device=dev) if w is not None else None for w in (weight, weight2)]
+        ws = torch.empty(2 * D * HEAD_NORM_MAX_BLOCKS, dtype=torch.float32, device=dev)
+        call("mmb_head_norm_rotate_bwd", *args, *xp, *gp, *tail, *op, f32(dw[0]), f32(dw[1]), f32(ws), stream())
+    return dx, dw[0], dw[1]
+
+
+class Q8Rows:
+    """Rows kept in 8 bits: codes (M, 32*ceil(K/32)) int8 and one step per 32 features (M, ceil(K/32)) uint8, see
+    mmb_checkpoint_rows.  A little over a quarter of the float32 rows."""
+    __slots__ = ("codes", "steps", "K")
+
+    def __init__(self, codes, steps, K):
+        nb = (K + 31) // 32
+        if codes.dim() != 2 or steps.dim() != 2 or codes.shape[1] != 32 * nb or steps.shape != (codes.shape[0], nb):
+            raise MMBError(f"Q8Rows: codes {tuple(codes.shape)} and steps {tuple(steps.shape)} do not hold rows of {K}")
+        if codes.device != steps.device:
+            raise MMBError(f"Q8Rows: codes live on {codes.device}, steps on {steps.device}")
+        self.codes, self.steps, self.K = codes, steps, K
+
+    @property
+    def shape(self):
+        return (self.codes.shape[0], self.K)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def args(self):
+        return self.codes.shape[0], self.K, _chk(self.codes, torch.int8, "codes"), _chk(self.steps, torch.uint8, "steps")
+
+
+def checkpoint_rows(x):
+    """x (M, K) float32 / bfloat16 / float16 rows -> Q8Rows"""
+    xp = _rows(x, "x")
+    if x.numel() == 0:
+        raise MMBError("checkpoint_rows: no rows")
+    M, K = x.shape
+    nb = (K + 31) // 32
+    with torch.cuda.device(x.device):
+        q8 = Q8Rows(torch.empty(M, 32 * nb, dtype=torch.int8, device=x.device),
+                    torch.empty(M, nb, dtype=torch.uint8, device=x.device), K)
+        _, _, cp, sp = q8.args()
+        call("mmb_checkpoint_rows", M, K, DT[x.dtype], *xp, cp, sp, stream())
+    return q8
+
+
+def restore_rows(q8, dtype=torch.float32, out=None):
+    """The (M, K) rows that a Q8Rows stands for."""
+    M, K, cp, sp = q8.args()
+    with torch.cuda.device(q8.device):
+        if out is None:
+            if dtype not in DT:
+                raise MMBError(f"restore_rows: dtype {dtype} is not float32, bfloat16 or float16")
+            out = torch.empty(M, K, dtype=dtype, device=q8.device)
+        op = _rows(out, "out", None, M, K, q8.device)
+        call("mmb_restore_rows", M, K, DT[out.dtype], cp, sp, *op, stream())
+    return out
+
+
+def grad_weight_rows_q8(q8, dZ, dW=None, db=None, accumulate=False, want_db=True):
+    """dW (N, K) = dZ^T X, db (N) = colsum(dZ) for X kept as a Q8Rows (mmb_grad_weight_rows on restored rows would read four
+    times the bytes).  dW, db given: written there (dW may be a column slice), added to what they hold if accumulate."""
+    M, K, cp, sp = q8.args()
+    zp = _rows(dZ, "dZ", None, M, None, q8.device)
+    N = dZ.shape[1]
+    if N == 0:
+        raise MMBError("grad_weight_rows_q8: dZ has no columns")
+    if accumulate and dW is None:
+        raise MMBError("grad_weight_rows_q8: accumulate needs dW")
+    dev = q8.device
+    with torch.cuda.device(dev):
+        if dW is None:
+            dW = torch.empty(N, K, dtype=torch.float32, device=dev)
+            db = torch.empty(N, dtype=torch.float32, device=dev) if db is None and want_db else db
+        wp = _rows(dW, "dW", torch.float32, N, K, dev)
+        ws, n = _workspace("mmb_grad_weight_rows_q8_workspace", M, N, K, device=dev)
+        call("mmb_grad_weight_rows_q8", M, K, N, DT[dZ.dtype], cp, sp, *zp, *wp, _vec(db, "db", N, dev), int(bool(accumulate)),
+             ws.data_ptr(), n, stream())
+    return dW, db
+
+
 # ------------------------------------------------------------------------ optimizer step
 ADAMW_WS = 1024
 

@@ -1,0 +1,119 @@
+"""CPU: what the conditional transformer's entry points refuse -- in the tensor layer, and in the C ABI, where the checks run
+on the host before any launch (the addresses handed over here are never touched)."""
+import ctypes as C
+
+import pytest
+import torch
+
+P = 0x1000                                                     # a 16-byte aligned address
+
+
+def rc_of(name, *args):
+    import mmb_hip
+    h = mmb_hip.lib()
+    return getattr(h, name)(*args), h.mmb_last_error()
+
+
+def fwd(**kw):
+    a = dict(B=1, Nq=4, Nk=8, nh=2, nkv=1, D=16, dt=0, q=P, q_ld=32, k=P, k_ld=16, v=P, v_ld=16, mq=None, mk=None, scale=0.25, out=P,
+             out_ld=32, lse=None, ws=None, n=0, stream=None)
+    a.update(kw)
+    return rc_of("mmb_cross_attention_fwd", *a.values())
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(B=0), b"positive"), (dict(Nq=0), b"positive"), (dict(Nk=0), b"positive"), (dict(Nk=-3), b"positive"),
+    (dict(nh=3, nkv=2), b"multiple"), (dict(nkv=0), b"multiple"), (dict(D=0), b"head width"), (dict(D=129), b"head width"),
+    (dict(dt=3), b"dtype"), (dict(scale=0.0), b"scale"), (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale"),
+    (dict(scale=float("inf")), b"scale"), (dict(q=None), b"NULL"), (dict(k=None), b"NULL"), (dict(v=None), b"NULL"),
+    (dict(out=None), b"NULL"), (dict(q_ld=31), b"leading"), (dict(k_ld=15), b"leading"), (dict(v_ld=15), b"leading"),
+    (dict(out_ld=31), b"leading"), (dict(Nq=1, Nk=100000), b"workspace"), (dict(Nq=1, Nk=100000, ws=P, n=16), b"workspace"),
+])
+def test_cross_attention_fwd_refuses(kw, word):
+    rc, msg = fwd(**kw)
+    assert rc == -1 and b"mmb_cross_attention_fwd" in msg and word in msg, msg
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(lse=None), b"NULL"), (dict(dout=None), b"NULL"), (dict(dk=None), b"NULL"), (dict(dq_ld=31), b"leading"),
+    (dict(dv_ld=15), b"leading"), (dict(ws=None), b"workspace"), (dict(n=1 * 2 * 4 * 4 - 1), b"workspace"), (dict(D=200), b"head width"),
+])
+def test_cross_attention_bwd_refuses(kw, word):
+    a = dict(B=1, Nq=4, Nk=8, nh=2, nkv=1, D=16, dt=1, q=P, q_ld=32, k=P, k_ld=16, v=P, v_ld=16, mq=None, mk=None, scale=0.25, out=P,
+             out_ld=32, dout=P, dout_ld=32, lse=P, dq=P, dq_ld=32, dk=P, dk_ld=16, dv=P, dv_ld=16, ws=P, n=1 << 20, stream=None)
+    a.update(kw)
+    rc, msg = rc_of("mmb_cross_attention_bwd", *a.values())
+    assert rc == -1 and b"mmb_cross_attention_bwd" in msg and word in msg, msg
+
+
+def test_workspace_sizes():
+    n = C.c_int64(-1)
+    assert rc_of("mmb_cross_attention_workspace", 64, 128, 150, 4, 4, 32, 0, 0, C.byref(n))[0] == 0 and n.value == 0
+    assert rc_of("mmb_cross_attention_workspace", 1, 1, 100000, 4, 1, 128, 1, 0, C.byref(n))[0] == 0 and n.value > 0
+    assert rc_of("mmb_cross_attention_workspace", 3, 5, 7, 4, 1, 8, 1, 1, C.byref(n))[0] == 0 and n.value >= 3 * 4 * 5 * 4
+    assert rc_of("mmb_cross_attention_workspace", 3, 5, 7, 4, 3, 8, 1, 1, C.byref(n))[0] == -1
+    assert rc_of("mmb_grad_weight_rows_q8_workspace", 1000, 64, 32, C.byref(n))[0] == 0 and n.value >= (64 * 32 + 64) * 4
+    assert rc_of("mmb_grad_weight_rows_q8_workspace", 0, 64, 32, C.byref(n))[0] == -1
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(M=0), b"positive"), (dict(nh=0), b"positive"), (dict(nh2=-1), b"nheads2"), (dict(D=257, x_ld=10000, y_ld=10000), b"head width"),
+    (dict(dt=9), b"dtype"), (dict(x=None), b"NULL"), (dict(y=None), b"NULL"), (dict(x_ld=47), b"leading"), (dict(y_ld=47), b"leading"),
+    (dict(eps=0.0), b"eps"), (dict(pairs=9), b"fit"), (dict(pairs=-1), b"fit"), (dict(pos=None), b"need pos"), (dict(freq=None), b"need pos"),
+    (dict(axes=3), b"divides"), (dict(axes=0), b"divides"), (dict(pos_ld=1, axes=2), b"divides"), (dict(layout=2), b"layout"),
+])
+def test_head_norm_refuses(kw, word):
+    a = dict(M=3, nh=2, nh2=1, D=16, dt=0, x=P, x_ld=48, w=P, w2=P, eps=1e-6, pos=P, pos_ld=2, axes=2, freq=P, pairs=8, layout=0, y=P,
+             y_ld=48, stream=None)
+    a.update(kw)
+    rc, msg = rc_of("mmb_head_norm_rotate_fwd", *a.values())
+    assert rc == -1 and word in msg, msg
+    b = list(a.values())
+    rc, msg = rc_of("mmb_head_norm_rotate_bwd", *b[:7], P, 48, *b[7:18], None, None, P, None)
+    assert rc == -1 and word in msg, msg
+
+
+def test_head_norm_bwd_refuses():
+    a = [3, 2, 1, 16, 0, P, 48, P, 48, P, P, 1e-6, P, 2, 2, P, 8, 0, P, 48, None, None, P, None]
+    for i, bad, word in ((7, None, b"dy"), (8, 47, b"dy"), (22, None, b"partials")):
+        b = list(a)
+        b[i] = bad
+        rc, msg = rc_of("mmb_head_norm_rotate_bwd", *b)
+        assert rc == -1 and word in msg, msg
+
+
+@pytest.mark.parametrize("name,args,word", [
+    ("mmb_checkpoint_rows", (0, 8, 0, P, 8, P, P, None), b"positive"), ("mmb_checkpoint_rows", (4, 0, 0, P, 8, P, P, None), b"positive"),
+    ("mmb_checkpoint_rows", (4, 8, 5, P, 8, P, P, None), b"dtype"), ("mmb_checkpoint_rows", (4, 8, 0, None, 8, P, P, None), b"x is NULL"),
+    ("mmb_checkpoint_rows", (4, 8, 0, P, 7, P, P, None), b"leading"), ("mmb_checkpoint_rows", (4, 8, 0, P, 8, None, P, None), b"NULL"),
+    ("mmb_checkpoint_rows", (4, 8, 0, P, 8, P + 1, P, None), b"aligned"), ("mmb_restore_rows", (4, 8, 0, P, None, P, 8, None), b"NULL"),
+    ("mmb_restore_rows", (4, 8, 0, P, P, None, 8, None), b"NULL"), ("mmb_restore_rows", (4, 8, 0, P, P, P, 7, None), b"leading"),
+    ("mmb_restore_rows", (4, 8, 7, P, P, P, 8, None), b"dtype"),
+    ("mmb_grad_weight_rows_q8", (4, 8, 0, 0, P, P, P, 8, P, 8, P, 0, P, 1 << 20, None), b"N in"),
+    ("mmb_grad_weight_rows_q8", (4, 8, 4, 0, P, P, None, 8, P, 8, P, 0, P, 1 << 20, None), b"NULL"),
+    ("mmb_grad_weight_rows_q8", (4, 8, 4, 0, P, P, P, 3, P, 8, P, 0, P, 1 << 20, None), b"leading"),
+    ("mmb_grad_weight_rows_q8", (4, 8, 4, 0, P, P, P, 8, P, 7, P, 0, P, 1 << 20, None), b"leading"),
+    ("mmb_grad_weight_rows_q8", (4, 8, 4, 0, P, P, P, 8, P, 8, P, 0, P, 4, None), b"workspace"),
+    ("mmb_grad_weight_rows_q8", (4, 8, 4, 0, P, P, P, 8, P, 8, P, 0, None, 1 << 20, None), b"workspace"),
+    ("mmb_grad_weight_rows_q8", (4, 8, 4, 4, P, P, P, 8, P, 8, P, 0, P, 1 << 20, None), b"dtype"),
+])
+def test_checkpoints_refuse(name, args, word):
+    rc, msg = rc_of(name, *args)
+    assert rc == -1 and word in msg, msg
+
+
+def test_tensor_layer_refuses_host_tensors_and_wrong_shapes():
+    from mmb_hip import ops, MMBError
+    x = torch.zeros(8, 32)
+    for call in (lambda: ops.cross_attention_fwd(x, x, x, 2, 2), lambda: ops.cross_attention_bwd(x, x, x, x, x, x, 2, 2),
+                 lambda: ops.head_norm_rotate_fwd(x, 2), lambda: ops.head_norm_rotate_bwd(x, x, 2), lambda: ops.checkpoint_rows(x),
+                 lambda: ops.restore_rows(ops.Q8Rows(torch.zeros(2, 32, dtype=torch.int8), torch.zeros(2, 1, dtype=torch.uint8), 20)),
+                 lambda: ops.grad_weight_rows_q8(ops.Q8Rows(torch.zeros(2, 32, dtype=torch.int8), torch.zeros(2, 1, dtype=torch.uint8), 32), x)):
+        with pytest.raises(MMBError, match="CPU fallback"):
+            call()
+    with pytest.raises(MMBError, match="hold rows"):
+        ops.Q8Rows(torch.zeros(2, 32, dtype=torch.int8), torch.zeros(2, 1, dtype=torch.uint8), 33)
+    with pytest.raises(MMBError, match="hold rows"):
+        ops.Q8Rows(torch.zeros(2, 32, dtype=torch.int8), torch.zeros(3, 1, dtype=torch.uint8), 32)
+    with pytest.raises(MMBError, match="multiple"):
+        ops.cross_attention_fwd(x, x, x, 2, 3, 2)
