@@ -123,11 +123,15 @@ decode_kernel(int64_t M, int K, int nb, const int8_t* __restrict__ codes, const 
 }
 
 // ---- dW (N, K) = dZ^T (N, M) . Xhat (M, K), db (N) = column sums of dZ -------------------------------------------
-// A workgroup owns a 128 x 128 tile of dW over a range of rows and walks the range 32 rows at a time: dZ and Xhat go to
-// LDS transposed (contraction index last) and in bf16 planes, four waves compute 64 x 64 each.  The rows are split over
-// workgroups to fill the chip; partial tiles are summed by a second launch in a fixed order (no atomics: equal inputs give
-// equal bits).
-constexpr int BN = 128, BK = 128, MS = 32, PITCH = MS + 8;
+// A workgroup owns a 128 x BK tile of dW (BK = 128 or 256) over a range of rows and walks the range 32 rows at a time; four
+// waves compute 64 x BK/2 each.  dZ (in bf16 planes) and Xhat lie in LDS as they come, row by row; the matrix operands want
+// eight consecutive ROWS of one column, which the transposing LDS read supplies (four rows of 16 columns per 16 lanes), so
+// nothing is transposed in registers.  Row pitch 16 banks past a multiple of 64: the four rows of such a read do not meet.
+// Two buffers, one barrier a step; the rows of the step after next are in registers meanwhile.
+// The rows are split over workgroups to fill the chip; partial tiles are summed by a second launch in a fixed order (no
+// atomics: equal inputs give equal bits).
+constexpr int BN = 128, MS = 32;
+constexpr int pitch_of(int cols) { return cols + 32; }
 
 template <typename T> struct Planes;
 template <> struct Planes<float> { static constexpr int n = 3; };
@@ -141,130 +145,168 @@ struct GwArgs {
   const int8_t* codes;
   const uint8_t* steps;
   const void* dz;
-  int64_t dz_ld, codes_ld;
+  int64_t dz_ld;
   float *pw, *pb;                                 // partial sums (splits, N, K), (splits, N)
 };
 
-// four rows x four columns of dZ -> PL planes of four column vectors of four rows (two words each)
-template <typename T>
-__device__ __forceinline__ void planes4(const float v[4][4], int c, uint2* out) {
-  uint32_t b[3][4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float x = v[j][c];
-    const uint32_t hi = __float_as_uint(x) & 0xffff0000u;
-    b[0][j] = hi;
-    if constexpr (Planes<T>::n > 1) {
-      const float r = x - __uint_as_float(hi);
-      const uint32_t mid = __float_as_uint(r) & 0xffff0000u;
-      b[1][j] = mid;
-      if constexpr (Planes<T>::n > 2) b[2][j] = __float_as_uint(r - __uint_as_float(mid));
-    }
-  }
-#pragma unroll
-  for (int p = 0; p < Planes<T>::n; ++p) {
-    out[p].x = __builtin_amdgcn_perm(b[p][1], b[p][0], 0x07060302u);
-    out[p].y = __builtin_amdgcn_perm(b[p][3], b[p][2], 0x07060302u);
-  }
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// rows 8h .. 8h+7 (h: lane half) of column (lane & 31) of a row-major LDS block: two transposing reads of four rows
+__device__ __forceinline__ u32x4 read_cols(const uint16_t* p, int pitch) {
+  union { s16x4 h[2]; u32x4 v; } r;
+  r.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+  r.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * pitch));
+  return r.v;
 }
 
-template <typename T, bool VEC>
+template <typename T, int BK>
+constexpr int gw_lds() { return 2 * MS * (Planes<T>::n * pitch_of(BN) + pitch_of(BK)) * 2; }
+
+template <typename T, int BK, bool VEC>
 __global__ void __launch_bounds__(256, 2) gw_kernel(GwArgs a) {
-  constexpr int PL = Planes<T>::n;
-  __shared__ __attribute__((aligned(16))) uint16_t As[PL][BN * PITCH];
-  __shared__ __attribute__((aligned(16))) uint16_t Bs[BK * PITCH];
+  constexpr int PL = Planes<T>::n, PA = pitch_of(BN), PB = pitch_of(BK), NJ = BK / 64, XC = MS * BK / 16 / 256;
+  extern __shared__ __attribute__((aligned(16))) uint16_t gw_sm[];
+  constexpr int BUF = MS * (PL * PA + PB);
   const int tiles = a.nt * a.kt;
   // all tiles of one row range on one XCD (workgroup ids go round the eight): they read the same rows
   const int64_t y = blockIdx.x >> 3;
   const int split = (int)(y / tiles) * 8 + (int)(blockIdx.x & 7), tile = (int)(y % tiles);
   if (split >= a.splits) return;
   const int n0 = (tile % a.nt) * BN, k0 = (tile / a.nt) * BK;
+  const bool sums = tile / a.nt == 0;              // the tiles of the first K window also sum dZ's columns
   const int64_t m0 = (int64_t)split * a.rows, m1 = min(a.M, m0 + a.rows);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
-  const int wn = (wave & 1) * 64, wk = (wave >> 1) * 64;
-  // loads: four rows x four columns a thread, the 32 threads of a half wave along a row
-  const int quad = threadIdx.x >> 5, c4 = (threadIdx.x & 31) * 4;
-  const bool n_ok = n0 + c4 < a.N, k_ok = k0 + c4 < a.nb * 32;
-  f32x16 acc[2][2];
+  const int wn = (wave & 1) * 64, wk = (wave >> 1) * (BK / 2);
+  // transposing reads: lane j of 16 addresses row j >> 2, four columns from 4 (j & 3)
+  const int tr_row = 8 * h + ((lane & 15) >> 2), tr_col = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+  // loads: dZ rows (tid >> 4) and + 16, eight columns; Xhat 16 codes a chunk
+  const int zr = threadIdx.x >> 4, zc = (threadIdx.x & 15) * 8;
+  f32x16 acc[2][NJ];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-  float db[4] = {0, 0, 0, 0};
-  float v[4][4];
-  uint32_t cw[4], sw[4];
+  float db[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  constexpr int ZW = sizeof(T) == 4 ? 8 : 4;       // words of eight elements
+  uint32_t zw[2][ZW];
+  u32x4 cw[XC];
+  uint32_t sw[XC];
   auto fetch = [&](int64_t m) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t row = m + quad * 4 + j;
-      const bool in = row < m1;
-      const T* p = (const T*)a.dz + row * a.dz_ld + n0 + c4;
-      if constexpr (VEC) {
-        if (in && n_ok) {
-          if constexpr (sizeof(T) == 4) {
-            const float4 f = *reinterpret_cast<const float4*>(p);
-            v[j][0] = f.x; v[j][1] = f.y; v[j][2] = f.z; v[j][3] = f.w;
-          } else {
-            T t[4];
-            const uint2 f = *reinterpret_cast<const uint2*>(p);
-            __builtin_memcpy(t, &f, 8);
+    for (int j = 0; j < 2; ++j) {
+      const int64_t row = m + zr + 16 * j;
+      const T* p = (const T*)a.dz + row * a.dz_ld + n0 + zc;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) v[j][c] = (float)t[c];
+      for (int w = 0; w < ZW; ++w) zw[j][w] = 0u;
+      if (row < m1) {
+        if constexpr (VEC) {
+          if (n0 + zc < a.N) {
+#pragma unroll
+            for (int w = 0; w < ZW / 4; ++w) {
+              const u32x4 t = *reinterpret_cast<const u32x4*>(p + w * 4);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) zw[j][4 * w + i] = t[i];
+            }
           }
         } else {
+          T t[8];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) v[j][c] = 0.0f;
+          for (int i = 0; i < 8; ++i) t[i] = n0 + zc + i < a.N ? p[i] : (T)0.0f;
+          __builtin_memcpy(zw[j], t, sizeof(t));
         }
-      } else {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) v[j][c] = in && n0 + c4 + c < a.N ? (float)p[c] : 0.0f;
       }
-      cw[j] = 0u;
+    }
+#pragma unroll
+    for (int j = 0; j < XC; ++j) {
+      const int it = threadIdx.x + 256 * j, c = (it % (BK / 16)) * 16;
+      const int64_t row = m + it / (BK / 16);
+      cw[j] = u32x4{0u, 0u, 0u, 0u};
       sw[j] = 0u;
-      if (in && k_ok) {
-        cw[j] = *reinterpret_cast<const uint32_t*>(a.codes + row * a.codes_ld + k0 + c4);
-        sw[j] = a.steps[row * a.nb + (k0 + c4) / 32];
+      if (row < m1 && k0 + c < a.nb * 32) {
+        cw[j] = *reinterpret_cast<const u32x4*>(a.codes + row * (a.nb * 32) + k0 + c);
+        sw[j] = a.steps[row * a.nb + (k0 + c) / 32];
+      }
+    }
+  };
+  auto put = [&](uint16_t* buf) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint16_t* dst = buf + (zr + 16 * j) * PA + zc;
+      float f[8];
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(zw[j][i]);
+      } else {
+        T t[8];
+        __builtin_memcpy(t, zw[j], 16);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = (float)t[i];
+      }
+      if (sums) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) db[i] += f[i];
+      }
+      if constexpr (PL == 1) {
+        *reinterpret_cast<u32x4*>(dst) = u32x4{zw[j][0], zw[j][1], zw[j][2], zw[j][3]};
+      } else {                                     // truncated planes: x = hi + mid (+ lo) exactly
+#pragma unroll
+        for (int p = 0; p < PL; ++p) {
+          u32x4 w;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(__float_as_uint(f[2 * i + 1]), __float_as_uint(f[2 * i]), 0x07060302u);
+          *reinterpret_cast<u32x4*>(dst + p * MS * PA) = w;
+          if (p + 1 < PL) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] -= __uint_as_float(__float_as_uint(f[i]) & 0xffff0000u);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < XC; ++j) {
+      const int it = threadIdx.x + 256 * j;
+      uint16_t* dst = buf + MS * PL * PA + (it / (BK / 16)) * PB + (it % (BK / 16)) * 16;
+      // code * step with the code as an unsigned byte, offset by 128: (u - 128) step, exact in one fused step
+      const float st = step_of(sw[j]), off = -128.0f * st;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t u = cw[j][2 * q + i] ^ 0x80808080u;
+          const float x0 = fmaf((float)(u & 255u), st, off), x1 = fmaf((float)((u >> 8) & 255u), st, off),
+                      x2 = fmaf((float)((u >> 16) & 255u), st, off), x3 = fmaf((float)(u >> 24), st, off);
+          w[2 * i] = __builtin_amdgcn_perm(__float_as_uint(x1), __float_as_uint(x0), 0x07060302u);
+          w[2 * i + 1] = __builtin_amdgcn_perm(__float_as_uint(x3), __float_as_uint(x2), 0x07060302u);
+        }
+        *reinterpret_cast<u32x4*>(dst + 8 * q) = w;
       }
     }
   };
   fetch(m0);
-  for (int64_t m = m0; m < m1; m += MS) {
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint2 w[PL];
-      planes4<T>(v, c, w);
-#pragma unroll
-      for (int p = 0; p < PL; ++p) *reinterpret_cast<uint2*>(&As[p][(c4 + c) * PITCH + quad * 4]) = w[p];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) db[c] += v[j][c];
-    }
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint32_t b[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = __float_as_uint((float)(int8_t)(cw[j] >> (8 * c)) * step_of(sw[j]));
-      uint2 w;
-      w.x = __builtin_amdgcn_perm(b[1], b[0], 0x07060302u);
-      w.y = __builtin_amdgcn_perm(b[3], b[2], 0x07060302u);
-      *reinterpret_cast<uint2*>(&Bs[(c4 + c) * PITCH + quad * 4]) = w;
-    }
+  int p = 0;
+  for (int64_t m = m0; m < m1; m += MS, p ^= 1) {
+    uint16_t* buf = gw_sm + p * BUF;
+    put(buf);
     if (m + MS < m1) fetch(m + MS);
-    __syncthreads();
+    __syncthreads();                               // (the other buffer's readers passed here after their products)
+    const uint16_t* As = buf + tr_row * PA + wn + tr_col;
+    const uint16_t* Bs = buf + MS * PL * PA + tr_row * PB + wk + tr_col;
 #pragma unroll
     for (int s = 0; s < MS / 16; ++s) {
-      u32x4 bf[2];
+      u32x4 bf[NJ];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) bf[j] = *reinterpret_cast<const u32x4*>(&Bs[(wk + 32 * j + col) * PITCH + 16 * s + 8 * h]);
+      for (int j = 0; j < NJ; ++j) bf[j] = read_cols(Bs + 16 * s * PB + 32 * j, PB);
 #pragma unroll
-      for (int p = PL - 1; p >= 0; --p)
+      for (int q = PL - 1; q >= 0; --q)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const bf16x8 af = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(&As[p][(wn + 32 * i + col) * PITCH + 16 * s + 8 * h]));
+          const bf16x8 af = __builtin_bit_cast(bf16x8, read_cols(As + q * MS * PA + 16 * s * PA + 32 * i, PA));
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < NJ; ++j)
             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af, __builtin_bit_cast(bf16x8, bf[j]), acc[i][j], 0, 0, 0);
         }
     }
@@ -273,58 +315,74 @@ __global__ void __launch_bounds__(256, 2) gw_kernel(GwArgs a) {
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int n = n0 + wn + 32 * i + (r >> 2) * 8 + h * 4 + (r & 3), k = k0 + wk + 32 * j + col;
         if (n < a.N && k < a.K) pw[(int64_t)n * a.K + k] = acc[i][j][r];
       }
-  if (tile / a.nt == 0) {                          // column sums: the tiles of the first K window
-    float* red = reinterpret_cast<float*>(Bs);     // 8 quads x 128 columns
+  if (sums) {
+    float* red = reinterpret_cast<float*>(gw_sm);  // 16 row groups x 128 columns
     __syncthreads();
 #pragma unroll
-    for (int c = 0; c < 4; ++c) red[quad * BN + c4 + c] = db[c];
+    for (int i = 0; i < 8; ++i) red[zr * BN + zc + i] = db[i];
     __syncthreads();
     if (threadIdx.x < BN && n0 + threadIdx.x < a.N) {
       float s = 0.0f;
 #pragma unroll
-      for (int q = 0; q < 8; ++q) s += red[q * BN + threadIdx.x];
+      for (int q = 0; q < 16; ++q) s += red[q * BN + threadIdx.x];
       a.pb[(int64_t)split * a.N + n0 + threadIdx.x] = s;
     }
   }
 }
 
-// dW, db from the partial sums of the row ranges
+// dW, db from the partial sums of the row ranges: eight threads share the ranges of one element, joined in LDS
 __global__ void __launch_bounds__(256)
 gw_fold_kernel(int splits, int64_t nw, int N, int K, const float* __restrict__ pw, const float* __restrict__ pb, float* __restrict__ dW,
                int64_t dw_ld, float* __restrict__ db, int accumulate) {
-  const int64_t n = nw + N;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    float s = 0.0f;
-    if (i < nw) {
-      for (int p = 0; p < splits; ++p) s += pw[(int64_t)p * nw + i];
-      float* d = dW + i / K * dw_ld + i % K;
-      *d = accumulate ? *d + s : s;
-    } else if (db) {
-      for (int p = 0; p < splits; ++p) s += pb[(int64_t)p * N + (i - nw)];
-      db[i - nw] = accumulate ? db[i - nw] + s : s;
-    }
+  __shared__ float red[8][33];
+  const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int64_t i = (int64_t)blockIdx.x * 32 + c;
+  float s = 0.0f;
+  if (i < nw) {
+#pragma unroll 4
+    for (int p = g; p < splits; p += 8) s += pw[(int64_t)p * nw + i];
+  } else if (i < nw + N) {
+    for (int p = g; p < splits; p += 8) s += pb[(int64_t)p * N + (i - nw)];
+  }
+  red[g][c] = s;
+  __syncthreads();
+  if (g != 0 || i >= nw + N) return;
+#pragma unroll
+  for (int q = 1; q < 8; ++q) s += red[q][c];
+  if (i < nw) {
+    float* d = dW + i / K * dw_ld + i % K;
+    *d = accumulate ? *d + s : s;
+  } else if (db) {
+    db[i - nw] = accumulate ? db[i - nw] + s : s;
   }
 }
 
 // Row ranges: enough workgroups for two on every CU, no range shorter than 8 steps, and no more partial sums than a quarter
 // of what the operands themselves hold (they are written and read once more).
-static void gw_plan(int64_t M, int N, int K, int* nt, int* kt, int* splits, int64_t* rows) {
-  *nt = (N + BN - 1) / BN;
-  *kt = (K + BK - 1) / BK;
-  const int64_t tiles = (int64_t)*nt * *kt;
+struct GwPlan {
+  int bk, nt, kt, splits;
+  int64_t rows;
+};
+static GwPlan gw_plan(int64_t M, int N, int K) {
+  GwPlan p;
+  p.bk = K > 128 ? 256 : 128;
+  p.nt = (N + BN - 1) / BN;
+  p.kt = (K + p.bk - 1) / p.bk;
+  const int64_t tiles = (int64_t)p.nt * p.kt;
   int64_t s = (512 + tiles - 1) / tiles;
   const int64_t most = (M + 8 * MS - 1) / (8 * MS), fit = M * ((int64_t)K + 4 * N) / (32 * (int64_t)N * K) + 1;
   if (s > most) s = most;
   if (s > fit) s = fit;
   if (s < 1) s = 1;
-  *rows = (M + s * MS - 1) / (s * MS) * MS;
-  *splits = (int)((M + *rows - 1) / *rows);
+  p.rows = (M + s * MS - 1) / (s * MS) * MS;
+  p.splits = (int)((M + p.rows - 1) / p.rows);
+  return p;
 }
 
 static int check_q8(const char* who, int64_t M, int K, const void* codes, const void* steps) {
@@ -350,17 +408,30 @@ static int decode(int64_t M, int K, const void* codes, const void* steps, void* 
   else decode_kernel<T, false><<<grid, 256, 0, st>>>(M, K, nb, (const int8_t*)codes, (const uint8_t*)steps, (T*)y, y_ld);
   return check_launch("mmb_restore_rows");
 }
-template <typename T>
-static int grad_weight(GwArgs& a, float* dW, int64_t dw_ld, float* db, int accumulate, hipStream_t st) {
-  const bool vec = a.N % 4 == 0 && ((uintptr_t)a.dz & 15) == 0 && a.dz_ld * (int64_t)sizeof(T) % (4 * sizeof(T)) == 0;
+template <typename T, int BK, bool VEC>
+static int launch_gw(const GwArgs& a, hipStream_t st) {
+  constexpr int bytes = gw_lds<T, BK>();
+  auto kern = gw_kernel<T, BK, VEC>;
+  static PerDeviceOnce once;
+  if (bytes > 64 * 1024 &&
+      !once.run([&] { return hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess; })) {
+    set_error("mmb_grad_weight_rows_q8: the runtime refuses %d bytes of LDS", bytes);
+    return MMB_ERR_LAUNCH;
+  }
   const int64_t blocks = (int64_t)(a.splits + 7) / 8 * 8 * a.nt * a.kt;
   MMB_REQUIRE(blocks <= 0x7fffffffLL, "mmb_grad_weight_rows_q8: %lld workgroups", (long long)blocks);
-  if (vec) gw_kernel<T, true><<<(unsigned)blocks, 256, 0, st>>>(a);
-  else gw_kernel<T, false><<<(unsigned)blocks, 256, 0, st>>>(a);
-  int rc = check_launch("mmb_grad_weight_rows_q8");
+  kern<<<(unsigned)blocks, 256, bytes, st>>>(a);
+  return check_launch("mmb_grad_weight_rows_q8");
+}
+template <typename T>
+static int grad_weight(GwArgs& a, int bk, float* dW, int64_t dw_ld, float* db, int accumulate, hipStream_t st) {
+  const bool vec = a.N % 8 == 0 && ((uintptr_t)a.dz & 15) == 0 && a.dz_ld * (int64_t)sizeof(T) % 16 == 0;
+  const int64_t nw = (int64_t)a.N * a.K, fold = (nw + a.N + 31) / 32;
+  MMB_REQUIRE(fold <= 0x7fffffffLL, "mmb_grad_weight_rows_q8: dW of %lld values", (long long)nw);
+  int rc = bk == 256 ? (vec ? launch_gw<T, 256, true>(a, st) : launch_gw<T, 256, false>(a, st))
+                     : (vec ? launch_gw<T, 128, true>(a, st) : launch_gw<T, 128, false>(a, st));
   if (rc != MMB_OK) return rc;
-  const int64_t nw = (int64_t)a.N * a.K;
-  gw_fold_kernel<<<stream_grid(nw + a.N, 256), 256, 0, st>>>(a.splits, nw, a.N, a.K, a.pw, a.pb, dW, dw_ld, db, accumulate);
+  gw_fold_kernel<<<(unsigned)fold, 256, 0, st>>>(a.splits, nw, a.N, a.K, a.pw, a.pb, dW, dw_ld, db, accumulate);
   return check_launch("mmb_grad_weight_rows_q8 (fold)");
 }
 
@@ -394,10 +465,7 @@ extern "C" int mmb_restore_rows(int64_t M, int K, int dtype, const void* codes, 
 
 extern "C" int mmb_grad_weight_rows_q8_workspace(int64_t M, int N, int K, int64_t* bytes_host) {
   MMB_REQUIRE(M > 0 && N > 0 && K > 0 && bytes_host, "mmb_grad_weight_rows_q8_workspace: sizes must be positive, bytes_host not NULL");
-  int nt, kt, splits;
-  int64_t rows;
-  gw_plan(M, N, K, &nt, &kt, &splits, &rows);
-  *bytes_host = (int64_t)splits * ((int64_t)N * K + N) * 4;
+  *bytes_host = (int64_t)gw_plan(M, N, K).splits * ((int64_t)N * K + N) * 4;
   return MMB_OK;
 }
 
@@ -407,18 +475,17 @@ extern "C" int mmb_grad_weight_rows_q8(int64_t M, int K, int N, int dtype, const
   if (int rc = check_q8("mmb_grad_weight_rows_q8", M, K, codes, steps)) return rc;
   MMB_REQUIRE(N > 0 && N <= (1 << 20) && dZ && dz_ld >= N && dW && dw_ld >= K,
               "mmb_grad_weight_rows_q8: N in 1..2^20, dZ, dW not NULL, leading dimensions no smaller than their rows");
-  GwArgs a = {M, N, K, (K + 31) / 32, 0, 0, 0, 0, (const int8_t*)codes, (const uint8_t*)steps, dZ, dz_ld, 0, nullptr, nullptr};
-  a.codes_ld = (int64_t)a.nb * 32;
-  gw_plan(M, N, K, &a.nt, &a.kt, &a.splits, &a.rows);
+  const GwPlan p = gw_plan(M, N, K);
+  GwArgs a = {M, N, K, (K + 31) / 32, p.nt, p.kt, p.splits, p.rows, (const int8_t*)codes, (const uint8_t*)steps, dZ, dz_ld, nullptr, nullptr};
   const int64_t need = (int64_t)a.splits * ((int64_t)N * K + N) * 4;
   MMB_REQUIRE(workspace && workspace_bytes >= need, "mmb_grad_weight_rows_q8: workspace of %lld bytes needed, got %lld", (long long)need,
               (long long)(workspace ? workspace_bytes : 0));
   a.pw = (float*)workspace;
   a.pb = a.pw + (int64_t)a.splits * N * K;
   hipStream_t st = as_stream(stream);
-  if (dtype == MMB_DT_F32) return grad_weight<float>(a, dW, dw_ld, db, accumulate, st);
-  if (dtype == MMB_DT_BF16) return grad_weight<__bf16>(a, dW, dw_ld, db, accumulate, st);
-  if (dtype == MMB_DT_F16) return grad_weight<_Float16>(a, dW, dw_ld, db, accumulate, st);
+  if (dtype == MMB_DT_F32) return grad_weight<float>(a, p.bk, dW, dw_ld, db, accumulate, st);
+  if (dtype == MMB_DT_BF16) return grad_weight<__bf16>(a, p.bk, dW, dw_ld, db, accumulate, st);
+  if (dtype == MMB_DT_F16) return grad_weight<_Float16>(a, p.bk, dW, dw_ld, db, accumulate, st);
   set_error("mmb_grad_weight_rows_q8: unknown dtype %d", dtype);
   return MMB_ERR_INVALID_ARG;
 }
