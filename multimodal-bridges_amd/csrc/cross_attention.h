@@ -4,9 +4,10 @@
 //   forward / dq :  S^T (keys x queries)  = K Q^T      a lane holds 16 keys of one query per tile
 //   dk, dv       :  S   (queries x keys)  = Q K^T      a lane holds 16 queries of one key per tile
 // so softmax statistics are per-lane scalars, and the accumulator registers of S (or P, dS) ARE the B operand of the
-// next product: 32x32x16 wants, for one column, eight consecutive contraction indices per lane half, the accumulator
-// holds {4h..4h+3, 8+4h..8+4h+3} of every 16 -- a permutation of the contraction index, which the A operand (stored
-// transposed in LDS) is written with.  No cross-lane traffic, no LDS round trip for P.
+// next product: 32x32x16 wants, for one column, eight contraction indices per lane half, the accumulator holds
+// {4h..4h+3, 8+4h..8+4h+3} of every 16 -- a permutation of the contraction index, which the A operand is read with.  No
+// cross-lane traffic, no LDS round trip for P.  The A operand of that product is the transpose of a tile that lies row by
+// row in LDS; in 16 bits the transposing LDS read supplies it, so a tile is stored once and serves both products.
 #pragma once
 #include "common.h"
 
@@ -184,105 +185,81 @@ struct SlotTiles {
 };
 
 // ---- one tile of rows in LDS -------------------------------------------------------------------------------------
-// Row-major:   [ROWS][DP + pad]; 16-byte chunks; pitch 4 words past a multiple of 64 banks: b128 reads of 32 rows at one
-//              chunk column spread over all banks.
-// Transposed:  [DP][ROWS + 8] (16-bit types only), the row index permuted inside every 16 as the accumulators hold it.
-template <typename T, int DP> constexpr int row_pitch() { return DP + (sizeof(T) == 2 ? 8 : 4); }
-template <int ROWS> constexpr int tr_pitch() { return ROWS + 8; }
-
-// position of row 4*quad inside a transposed row
-__device__ __forceinline__ int tr_pos(int quad) { return (quad >> 2) * 16 + (quad & 1) * 8 + ((quad >> 1) & 1) * 4; }
-
-// four rows x eight columns (16-bit) -> eight columns x four rows
-__device__ __forceinline__ void transpose_store(const u32x4 r[4], uint16_t* dst, int pitch) {
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    uint2 lo, hi;
-    lo.x = __builtin_amdgcn_perm(r[1][w], r[0][w], 0x05040100u);
-    lo.y = __builtin_amdgcn_perm(r[3][w], r[2][w], 0x05040100u);
-    hi.x = __builtin_amdgcn_perm(r[1][w], r[0][w], 0x07060302u);
-    hi.y = __builtin_amdgcn_perm(r[3][w], r[2][w], 0x07060302u);
-    *reinterpret_cast<uint2*>(dst + (2 * w) * pitch) = lo;
-    *reinterpret_cast<uint2*>(dst + (2 * w + 1) * pitch) = hi;
-  }
+// float:  row-major, pitch DP + 4 (b128 reads of 32 rows at one chunk column spread over all banks).
+// 16-bit: row-major without padding, the 16-byte chunks of a row permuted by an exclusive-or with a function of the row
+//         that serves both kinds of read: 16 rows at one chunk column (the scores) and four rows of 16 columns (the
+//         transposing read of the second product) each fall on 64 different banks.
+template <typename T, int DP> constexpr int row_pitch() { return sizeof(T) == 2 ? DP : DP + 4; }
+template <int DP>
+__device__ __forceinline__ int swizzle(int row) {
+  return DP == 128 ? ((row & 3) << 2 | ((row >> 2) & 3)) : DP == 64 ? (((row >> 1) & 1) << 2 | ((row >> 2) & 3)) : (row >> 2) & 3;
 }
+template <typename T, int DP>
+__device__ __forceinline__ int chunk_at(int row, int ch) {                  // element offset of chunk ch of a row
+  constexpr int E = Traits<T>::EPC;
+  if constexpr (sizeof(T) == 2) return row * DP + ((ch ^ swizzle<DP>(row)) * E);
+  else return row * row_pitch<T, DP>() + ch * E;
+}
+template <typename T, int DP, int ROWS>
+constexpr int tile_bytes() { return ROWS * row_pitch<T, DP>() * (int)sizeof(T); }
 
-// Registers of one thread's share of a ROWS x DP tile: items of four rows x one chunk column.
+// Registers of one thread's share of a ROWS x DP tile: 16-byte chunks, the chunks of a row beside each other.
 template <typename T, int DP, int ROWS, int NT>
 struct TileRegs {
-  static constexpr int E = Traits<T>::EPC, CH = DP / E, QUADS = ROWS / 4, ITEMS = QUADS * CH, PER = (ITEMS + NT - 1) / NT;
-  u32x4 r[PER][4];
-  // item -> (quad, chunk): four chunk columns of one quad beside each other (64 contiguous bytes of a row), then the quads
-  static __device__ __forceinline__ void where(int it, int& quad, int& ch) {
-    constexpr int C4 = CH < 4 ? CH : 4;
-    const int c = it % C4, rest = it / C4;
-    quad = rest % QUADS;
-    ch = (rest / QUADS) * C4 + c;
-  }
+  static constexpr int E = Traits<T>::EPC, CH = DP / E, ITEMS = ROWS * CH, PER = (ITEMS + NT - 1) / NT;
+  u32x4 r[PER];
   template <bool VEC, typename RowOf>
   __device__ __forceinline__ void load(int tid, int n, int D, RowOf row_of) {
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
-      const int it = p * NT + tid;
-      int quad, ch;
-      where(it, quad, ch);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int row = quad * 4 + j;
-        const bool ok = row < n && (ITEMS % NT == 0 || it < ITEMS);
-        r[p][j] = load_chunk<T, VEC>(ok ? row_of(row) : nullptr, ch * E, D, ok);
-      }
+      const int it = p * NT + tid, row = it / CH;
+      const bool ok = row < n && (ITEMS % NT == 0 || it < ITEMS);
+      r[p] = load_chunk<T, VEC>(ok ? row_of(row) : nullptr, (it % CH) * E, D, ok);
     }
   }
-  __device__ __forceinline__ void store_rows(int tid, T* dst) const {
+  __device__ __forceinline__ void store(int tid, T* dst) const {
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
       const int it = p * NT + tid;
       if (ITEMS % NT != 0 && it >= ITEMS) break;
-      int quad, ch;
-      where(it, quad, ch);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<u32x4*>(dst + (quad * 4 + j) * row_pitch<T, DP>() + ch * E) = r[p][j];
-    }
-  }
-  __device__ __forceinline__ void store_tr(int tid, T* dst) const {
-    if constexpr (sizeof(T) == 2) {
-#pragma unroll
-      for (int p = 0; p < PER; ++p) {
-        const int it = p * NT + tid;
-        if (ITEMS % NT != 0 && it >= ITEMS) break;
-        int quad, ch;
-        where(it, quad, ch);
-        transpose_store(r[p], reinterpret_cast<uint16_t*>(dst) + ch * E * tr_pitch<ROWS>() + tr_pos(quad), tr_pitch<ROWS>());
-      }
+      *reinterpret_cast<u32x4*>(dst + chunk_at<T, DP>(it / CH, it % CH)) = r[p];
     }
   }
 };
 
 // acc (32 x 32, register rows = contraction-major) += A_rows[row0 .. row0+31][:] . b, over the DP features of b's chunks
 template <typename T, int DP>
-__device__ __forceinline__ f32x16 dot_rows(const T* __restrict__ rows, int row0, const u32x4* b, f32x16 acc) {
+__device__ __forceinline__ f32x16 dot_rows(const T* rows, int row0, const u32x4* b, f32x16 acc) {
   constexpr int E = Traits<T>::EPC;
-  const int lane = threadIdx.x & 63;
-  const T* p = rows + (row0 + (lane & 31)) * row_pitch<T, DP>() + (lane >> 5) * E;
+  const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
 #pragma unroll
-  for (int s = 0; s < DP / (2 * E); ++s) acc = mfma<T>(*reinterpret_cast<const u32x4*>(p + s * 2 * E), b[s], acc);
+  for (int s = 0; s < DP / (2 * E); ++s)
+    acc = mfma<T>(*reinterpret_cast<const u32x4*>(rows + row0 * row_pitch<T, DP>() + chunk_at<T, DP>(r, 2 * s + h)), b[s], acc);
   return acc;
 }
 
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
 // out[t] (features 32t.. x columns) += X^T . w, the contraction over the 32 rows row0.. that w's registers run over.
-// 16-bit: X from its transposed copy; float: X row-major, one element a lane and step.
-template <typename T, int DP, int ROWS>
-__device__ __forceinline__ void dot_cols(const T* __restrict__ x, int row0, const f32x16& w, f32x16* out) {
+// 16-bit: X^T by the transposing read: the 16 lanes that hold 16 columns address four rows (lane j: row j >> 2, columns
+// from 4 (j & 3)) and receive four rows of their own column.  float: one element a lane and step.
+template <typename T, int DP>
+__device__ __forceinline__ void dot_cols(const T* x, int row0, const f32x16& w, f32x16* out) {
   const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
   if constexpr (sizeof(T) == 2) {
+    const int r4 = 4 * h + ((lane & 15) >> 2), cc = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), half = (lane & 1) * 4;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const u32x4 b = pack8<T>(w, 8 * g);
 #pragma unroll
-      for (int t = 0; t < DP / 32; ++t)
-        out[t] = mfma<T>(*reinterpret_cast<const u32x4*>(x + (32 * t + col) * tr_pitch<ROWS>() + row0 + 16 * g + 8 * h), b, out[t]);
+      for (int t = 0; t < DP / 32; ++t) {
+        union { s16x4 v[2]; u32x4 a; } f;
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          f.v[r] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(x + (row0 + 16 * g) * DP + chunk_at<T, DP>(8 * r + r4, 4 * t + cc) + half));
+        out[t] = mfma<T>(f.a, b, out[t]);
+      }
     }
   } else {
 #pragma unroll
@@ -314,26 +291,25 @@ __device__ __forceinline__ T round_to(float x) {
 // column of them is scaled by a power of two, chosen from the largest magnitude so far (kept between 2^12 and 2^14), and so is
 // what the column has summed; values 2^-38 below the largest are lost, which is below the sum's own rounding.
 struct ColScale {
-  float sc = 0x1p100f;
+  float sc = 0x1p60f;                              // (products of halves stay below 2^52: no overflow in 32 bits)
+  // w already carries sc
   __device__ __forceinline__ void fit(f32x16& w, f32x16* acc, int n_acc) {
     float top = 0.0f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(w[r]));
     top = fmaxf(top, __shfl_xor(top, 32));
-    if (__any(top * sc >= 0x1p14f)) {
+    if (__any(top >= 0x1p14f)) {
       const int ex = (int)(__float_as_uint(top) >> 23);                       // 2^(ex - 127) <= top
-      const float want = __uint_as_float((uint32_t)min(max(266 - ex, 27), 227) << 23);   // top * want in [2^12, 2^13)
-      const float nw = top * sc >= 0x1p14f ? fminf(want, sc) : sc;
-      const float f = nw / sc;
+      const float f = top >= 0x1p14f ? __uint_as_float((uint32_t)max(266 - ex, 12) << 23) : 1.0f;      // top * f in [2^12, 2^13)
 #pragma unroll
       for (int t = 0; t < 4; ++t)
         if (t < n_acc)
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[t][r] *= f;
-      sc = nw;
-    }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) w[r] *= sc;
+      for (int r = 0; r < 16; ++r) w[r] *= f;
+      sc *= f;
+    }
   }
 };
 
@@ -384,14 +360,20 @@ inline GridMap grid_map(int B, int nkv, int per_head) {
   return g;
 }
 
-// zeros in the rows r0 .. r0 + rows - 1 (row = slot * g + head of the group) whose slot the mask drops
-template <int NT, typename T>
+// zeros in the rows r0 .. r0 + rows - 1 (row = slot * g + head of the group) whose slot the mask drops; four lanes a row
+template <int NT, bool VEC, typename T>
 __device__ __forceinline__ void zero_masked_rows(T* __restrict__ out, int64_t ld, const float* __restrict__ maskf, int r0, int rows,
                                                  int g, int D) {
-  const int work = rows * D;
-  for (int e = threadIdx.x; e < work; e += NT) {
-    const int r = e / D, d = e - r * D, n = (r0 + r) / g, gi = (r0 + r) - n * g;
-    if (maskf[n] == 0.0f) out[(int64_t)n * ld + gi * D + d] = (T)0.0f;
+  constexpr int E = Traits<T>::EPC;
+  for (int r = threadIdx.x >> 2; r < rows; r += NT / 4) {
+    const int n = g == 1 ? r0 + r : (r0 + r) / g, gi = r0 + r - n * g;
+    if (maskf[n] != 0.0f) continue;
+    T* o = out + (int64_t)n * ld + gi * D;
+    if constexpr (VEC) {
+      for (int d = (threadIdx.x & 3) * E; d < D; d += 4 * E) *reinterpret_cast<u32x4*>(o + d) = u32x4{0u, 0u, 0u, 0u};
+    } else {
+      for (int d = threadIdx.x & 3; d < D; d += 4) o[d] = (T)0.0f;
+    }
   }
 }
 

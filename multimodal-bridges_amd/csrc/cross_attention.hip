@@ -30,12 +30,9 @@ struct FwdArgs {
   GridMap map;
 };
 
-template <typename T, int DP, int NW, int TK>
-constexpr int team_lds() {
-  constexpr int kb = TK * row_pitch<T, DP>() * (int)sizeof(T);
-  constexpr int vb = sizeof(T) == 2 ? DP * tr_pitch<TK>() * (int)sizeof(T) : kb;
-  return kb + vb;
-}
+// K and V tiles; the team form has two of each, so that one barrier a tile is enough
+template <typename T, int DP, int TK, bool SPLIT>
+constexpr int kv_lds() { return 2 * (SPLIT ? 1 : 2) * tile_bytes<T, DP, TK>(); }
 
 // One tile of n keys (K rows and V in LDS): scores, running softmax, o += V^T P.
 template <typename T, int DP, int TK>
@@ -73,19 +70,21 @@ __device__ __forceinline__ void attend(const T* __restrict__ Ks, const T* __rest
   for (int st = 0; st < TK / 32; ++st)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      s[st][r] = __builtin_amdgcn_exp2f((s[st][r] - ms) * c);
+      // 16-bit inputs: one fused step (the rounding of ms * c moves all p of a row alike and cancels); float: the
+      // difference first, which is exact next to the maximum
+      s[st][r] = __builtin_amdgcn_exp2f(sizeof(T) == 2 ? fmaf(s[st][r], c, -ms * c) : (s[st][r] - ms) * c);
       l += s[st][r];
     }
   // p is rounded to the inputs' type for the product (16-bit types: half a step of a value in [0, 1], the size of the
   // output's own rounding; l sums the unrounded values), the sums over keys stay in 32 bits
 #pragma unroll
-  for (int st = 0; st < TK / 32; ++st) dot_cols<T, DP, TK>(Vs, 32 * st, s[st], acc);
+  for (int st = 0; st < TK / 32; ++st) dot_cols<T, DP>(Vs, 32 * st, s[st], acc);
 }
 
 template <typename T, int DP, int NW, int TK, bool SPLIT, bool VEC>
 __global__ void __launch_bounds__(64 * NW, 2) fwd_kernel(FwdArgs a) {
   constexpr int NT = 64 * NW, TEAM = SPLIT ? 1 : NW, TT = 64 * TEAM, ROWS = SPLIT ? 32 : 32 * NW;
-  constexpr int TILE = team_lds<T, DP, TEAM, TK>(), NTILE = SPLIT ? NW : 1;
+  constexpr int TILE = kv_lds<T, DP, TK, SPLIT>(), NTILE = SPLIT ? NW : 1;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   int* lists = reinterpret_cast<int*>(lds + TILE * NTILE);                  // key list(s), then the row list
   int* qlist = lists + NTILE * (kChunk + 64 + 4);
@@ -107,7 +106,7 @@ __global__ void __launch_bounds__(64 * NW, 2) fwd_kernel(FwdArgs a) {
     if (threadIdx.x < 64) compact_select(mq, sh.Nq, rt.first_c, min(ROWS, R) / sh.g + 2, qlist);
     if (split == 0) {                             // slots of masked queries: zero rows, no log-sum
       const int rows = min(ROWS, R - r0);
-      zero_masked_rows<NT>((T*)a.out + (int64_t)b * sh.Nq * a.out_ld + (int64_t)hk * sh.g * sh.D, a.out_ld, mq, r0, rows, sh.g, sh.D);
+      zero_masked_rows<NT, VEC>((T*)a.out + (int64_t)b * sh.Nq * a.out_ld + (int64_t)hk * sh.g * sh.D, a.out_ld, mq, r0, rows, sh.g, sh.D);
       for (int r = threadIdx.x; r < rows && a.lse; r += NT) {
         const int n = (r0 + r) / sh.g, gi = (r0 + r) - n * sh.g;
         if (mq[n] == 0.0f) a.lse[((int64_t)b * sh.nh + hk * sh.g + gi) * sh.Nq + n] = -INFINITY;
@@ -134,8 +133,8 @@ __global__ void __launch_bounds__(64 * NW, 2) fwd_kernel(FwdArgs a) {
     lo = (int)min((int64_t)sh.Nk, (int64_t)(split * NW + wave) * a.chunk);
     hi = (int)min((int64_t)sh.Nk, (int64_t)lo + a.chunk);
   }
-  T* Ks = reinterpret_cast<T*>(lds + team * TILE);
-  T* Vs = Ks + TK * row_pitch<T, DP>();
+  T* tiles = reinterpret_cast<T*>(lds + team * TILE);
+  constexpr int TILE_E = TK * row_pitch<T, DP>();
   int* list = lists + team * (kChunk + 64 + 4);
   SlotTiles<TEAM> keys;
   keys.init(mk, lo, hi, list, list + kChunk + 64);
@@ -145,15 +144,16 @@ __global__ void __launch_bounds__(64 * NW, 2) fwd_kernel(FwdArgs a) {
   int nk = keys.next(TK);
   kr.template load<VEC>(tid, nk, sh.D, [&](int i) { return kb + (int64_t)keys.slot(i) * a.k_ld; });
   vr.template load<VEC>(tid, nk, sh.D, [&](int i) { return vb + (int64_t)keys.slot(i) * a.v_ld; });
-  while (nk > 0) {
-    SlotTiles<TEAM>::sync();                      // the tile before this one has been read
-    kr.store_rows(tid, Ks);
-    if constexpr (sizeof(T) == 2) vr.store_tr(tid, Vs);
-    else vr.store_rows(tid, Vs);
+  for (int buf = 0; nk > 0; buf ^= SPLIT ? 0 : 1) {
+    if constexpr (SPLIT) wave_sync();             // one buffer: the tile before this one has been read (LDS is in order)
+    T* Ks = tiles + buf * 2 * TILE_E;
+    T* Vs = Ks + TILE_E;
+    kr.store(tid, Ks);
+    vr.store(tid, Vs);
     const int nn = keys.next(TK);                 // the next tile's rows come in while this one is worked on
     kr.template load<VEC>(tid, nn, sh.D, [&](int i) { return kb + (int64_t)keys.slot(i) * a.k_ld; });
     vr.template load<VEC>(tid, nn, sh.D, [&](int i) { return vb + (int64_t)keys.slot(i) * a.v_ld; });
-    SlotTiles<TEAM>::sync();
+    SlotTiles<TEAM>::sync();                      // (team: whoever passes here has read the other buffer)
     attend<T, DP, TK>(Ks, Vs, nk, qf, c, m, l, acc);
     nk = nn;
   }
@@ -292,13 +292,11 @@ static Plan fwd_plan(const Shape& s) {
 
 template <typename T, int DP, int NW, int TK, bool SPLIT, bool VEC>
 static int launch_fwd(const FwdArgs& a, hipStream_t st) {
-  constexpr int TEAM = SPLIT ? 1 : NW, NTILE = SPLIT ? NW : 1;
-  constexpr int tile_bytes = team_lds<T, DP, TEAM, TK>() * NTILE + (NTILE * (kChunk + 64 + 4) + 32 * NW + 4) * 4;
-  constexpr int join_bytes = SPLIT ? (NW * 64 + NW * DP * 33) * 4 + (NTILE * (kChunk + 64 + 4) + 32 * NW + 4) * 4 : 0;
-  constexpr int bytes = tile_bytes > join_bytes ? tile_bytes : join_bytes;
+  constexpr int NTILE = SPLIT ? NW : 1, tiles = kv_lds<T, DP, TK, SPLIT>() * NTILE, lists = NTILE * (kChunk + 64 + 4) * 4;
+  constexpr int bytes = tiles + lists + (32 * NW + 4) * 4;
   static_assert(bytes <= 160 * 1024, "LDS");
-  // the join buffers may not reach the row list behind the tiles
-  static_assert(!SPLIT || (NW * 64 + NW * DP * 33) * 4 <= team_lds<T, DP, TEAM, TK>() * NTILE + NTILE * (kChunk + 64 + 4) * 4, "join");
+  // the join buffers may not reach the row list behind tiles and key lists
+  static_assert(!SPLIT || (NW * 64 + NW * DP * 33) * 4 <= tiles + lists, "join");
   auto kern = fwd_kernel<T, DP, NW, TK, SPLIT, VEC>;
   static PerDeviceOnce once;
   if (bytes > 64 * 1024 &&
@@ -317,7 +315,7 @@ static int launch_fwd(const FwdArgs& a, hipStream_t st) {
 
 template <typename T, int DP, bool VEC>
 static int pick_nw(const Plan& p, const FwdArgs& a, hipStream_t st) {
-  // keys per tile: 64 in 16 bits (K and V^T of a 128-wide head: 36 KB), 32 in float (34 KB)
+  // keys per tile: 64 in 16 bits (two K and V tiles of a 128-wide head: 64 KB), 32 in float (68 KB)
   constexpr int TK = sizeof(T) == 2 ? 64 : 32;
   if (p.split) return launch_fwd<T, DP, 4, 32, true, VEC>(a, st);
   if (p.nw == 4) return launch_fwd<T, DP, 4, TK, false, VEC>(a, st);

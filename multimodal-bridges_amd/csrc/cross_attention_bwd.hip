@@ -4,10 +4,12 @@
 //   dp_ij = do_i . v_j      delta_i = sum_j p_ij dp_ij = do_i . o_i      ds_ij = p_ij (dp_ij - delta_i)
 //   dv_j  = sum_i p_ij do_i      dq_i = scale sum_j ds_ij k_j      dk_j = scale sum_i ds_ij q_i
 //
-// Two launches, each owning its outputs, so that every sum runs in a fixed order and nothing is accumulated with atomics:
-// dq (a wave owns 32 query rows and walks the keys; it also writes delta), then dk and dv (a wave owns 32 keys and walks
-// the queries of every head that shares them).  That recomputes s and dp once: 7 products instead of the 5 that one launch
-// with atomically summed dq would need.
+// Two kinds of workgroups, each owning its outputs, so that every sum runs in a fixed order and nothing is accumulated with
+// atomics: for dq a wave owns 32 query rows and walks the keys, for dk and dv a wave owns 32 keys and walks the queries of
+// every head that shares them.  That recomputes s and dp once: 7 products instead of the 5 that one kind with atomically
+// summed dq would need.  Both need delta: a short launch computes it and both kinds then run side by side in one launch (the
+// waves of one kind alone are too few to cover each other's latencies); with so few keys that a row is in registers at once,
+// the dq workgroups run first and take delta from p and dp themselves, free of the rounding of out.
 #include "cross_attention.h"
 
 namespace mmb {
@@ -21,37 +23,53 @@ struct BwdArgs {
   float scale;
   void *dq, *dk, *dv;
   float* delta;                                   // (B, nheads, Nq)
-  int tiles;
-  GridMap map;
+  bool few_keys;                                  // dq workgroups find delta themselves
+  int tiles_q, tiles_k;
+  GridMap map_q, map_k;
+  unsigned n_dkv;                                 // workgroups of this launch that own keys
 };
 
-// p from a raw score.  The product and the difference are rounded apart: a row with a single key, whose log-sum IS its
-// rounded score, gets exactly 1.
-__device__ __forceinline__ float prob(float s, float scale, float lse) {
+// log2 of a power of two
+__device__ __forceinline__ float log2_pow2(float x) { return (float)((int)(__float_as_uint(x) >> 23) - 127); }
+
+// p from a raw score; st: lse, for 16-bit types in units of log 2.  float: the product and the difference are rounded apart,
+// so that a row with a single key, whose log-sum IS its rounded score, gets exactly 1.
+template <typename T>
+__device__ __forceinline__ float prob(float s, float scale, float c, float st) {
 #pragma clang fp contract(off)
+  if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -st));
   const float t = s * scale;
-  return __builtin_amdgcn_exp2f((t - lse) * kLog2e);
+  return __builtin_amdgcn_exp2f((t - st) * kLog2e);
+}
+// a row without a key (or only scores of -inf): p = 0
+template <typename T>
+__device__ __forceinline__ float row_stat(float lse) {
+  return lse == -INFINITY ? INFINITY : sizeof(T) == 2 ? lse * kLog2e : lse;
 }
 
-// half precision: p in [0, 1] takes this factor into the product (p = 1 / Nk of a long list would be subnormal)
-constexpr float kHalfP = 4096.0f;
+// half precision: p in [0, 1] takes 2^12 into the product (p = 1 / Nk of a long list would be subnormal)
+constexpr float kHalfLog = 12.0f, kHalfP = 4096.0f;
 
-template <typename T, int DP, int TK>
-constexpr int dq_lds() {
-  constexpr int rows = TK * row_pitch<T, DP>() * (int)sizeof(T);
-  return 2 * rows + (sizeof(T) == 2 ? DP * tr_pitch<TK>() * (int)sizeof(T) : 0);
+// keys of a dq tile, queries of a dk / dv tile: as many as leave two workgroups on a CU room for their registers
+template <typename T, int DP> constexpr int dq_tile() { return sizeof(T) == 2 ? 64 : 32; }
+template <typename T, int DP> constexpr int dkv_tile() { return sizeof(T) == 2 && DP <= 64 ? 64 : 32; }
+
+constexpr int kListInts = kChunk + 64 + 4;
+template <typename T, int DP, int NW>
+constexpr int bwd_lds() {
+  constexpr int a = 4 * tile_bytes<T, DP, dq_tile<T, DP>()>(), b = 4 * tile_bytes<T, DP, dkv_tile<T, DP>()>() + 4 * dkv_tile<T, DP>() * 4;
+  return (a > b ? a : b) + (kListInts + 32 * NW + 4) * 4;
 }
 
 template <typename T, int DP, int NW, bool VEC>
-__global__ void __launch_bounds__(64 * NW, 2) dq_kernel(BwdArgs a) {
-  constexpr int NT = 64 * NW, TK = 32, ROWS = 32 * NW;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  int* list = reinterpret_cast<int*>(lds + dq_lds<T, DP, TK>());
-  int* qlist = list + kChunk + 64 + 4;
-  const Shape sh = a.sh;
+__device__ __forceinline__ void dq_body(const BwdArgs& a, int64_t id, char* lds) {
+  constexpr int NT = 64 * NW, TK = dq_tile<T, DP>(), ROWS = 32 * NW, TILE_E = TK * row_pitch<T, DP>();
+  int* list = reinterpret_cast<int*>(lds + 4 * tile_bytes<T, DP, TK>());
+  int* qlist = list + kListInts;
+  const Shape& sh = a.sh;
   int unit, item;
-  if (!a.map.decode(blockIdx.x, unit, item)) return;
-  const int pair = a.map.units == sh.B ? unit * sh.nkv + item / a.tiles : unit, tile = item % a.tiles;
+  if (!a.map_q.decode(id, unit, item)) return;
+  const int pair = a.map_q.units == sh.B ? unit * sh.nkv + item / a.tiles_q : unit, tile = item % a.tiles_q;
   const int b = pair / sh.nkv, hk = pair - b * sh.nkv;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
   const int R = sh.g * sh.Nq, r0 = tile * ROWS;
@@ -60,7 +78,7 @@ __global__ void __launch_bounds__(64 * NW, 2) dq_kernel(BwdArgs a) {
   RowTile rt = {r0 / sh.g, sh.g, qlist};
   if (mq) {
     if (threadIdx.x < 64) compact_select(mq, sh.Nq, rt.first_c, min(ROWS, R) / sh.g + 2, qlist);
-    zero_masked_rows<NT>((T*)a.dq + (int64_t)b * sh.Nq * a.dq_ld + (int64_t)hk * sh.g * sh.D, a.dq_ld, mq, r0, min(ROWS, R - r0), sh.g, sh.D);
+    zero_masked_rows<NT, VEC>((T*)a.dq + (int64_t)b * sh.Nq * a.dq_ld + (int64_t)hk * sh.g * sh.D, a.dq_ld, mq, r0, min(ROWS, R - r0), sh.g, sh.D);
     __syncthreads();
     if (qlist[0] < 0) return;
   }
@@ -75,29 +93,14 @@ __global__ void __launch_bounds__(64 * NW, 2) dq_kernel(BwdArgs a) {
   load_row<T, DP, VEC>(qf, (const T*)a.q + flat * a.q_ld + (int64_t)head * sh.D, sh.D, live);
   load_row<T, DP, VEC>(gf, (const T*)a.dout + flat * a.dout_ld + (int64_t)head * sh.D, sh.D, live);
   const int64_t stat = ((int64_t)b * sh.nh + head) * sh.Nq + n;
-  float lse = live ? a.lse[stat] : INFINITY;
-  if (lse == -INFINITY) lse = INFINITY;           // a row without a key (or only scores of -inf): p = 0
-  float delta = 0.0f;
-  {
-    u32x4 of[S];
-    load_row<T, DP, VEC>(of, (const T*)a.out + flat * a.out_ld + (int64_t)head * sh.D, sh.D, live);
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      T x[E], y[E];
-      __builtin_memcpy(x, &of[s], 16);
-      __builtin_memcpy(y, &gf[s], 16);
-#pragma unroll
-      for (int i = 0; i < E; ++i) delta = fmaf((float)x[i], (float)y[i], delta);
-    }
-    delta += __shfl_xor(delta, 32);
-  }
+  const float lse = live ? row_stat<T>(a.lse[stat]) : INFINITY;
+  float delta = live && !a.few_keys ? a.delta[stat] : 0.0f;
+  const float c = a.scale * kLog2e;
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int t = 0; t < DP / 32; ++t) acc[t] = zero16();
 
-  T* Ks = reinterpret_cast<T*>(lds);
-  T* Vs = Ks + TK * row_pitch<T, DP>();
-  T* Kt = sizeof(T) == 2 ? Vs + TK * row_pitch<T, DP>() : Ks;
+  T* tiles = reinterpret_cast<T*>(lds);
   SlotTiles<NW> keys;
   keys.init(mk, 0, sh.Nk, list, list + kChunk + 64);
   const T* kb = (const T*)a.k + (int64_t)b * sh.Nk * a.k_ld + (int64_t)hk * sh.D;
@@ -106,58 +109,69 @@ __global__ void __launch_bounds__(64 * NW, 2) dq_kernel(BwdArgs a) {
   int nk = keys.next(TK);
   kr.template load<VEC>(threadIdx.x, nk, sh.D, [&](int i) { return kb + (int64_t)keys.slot(i) * a.k_ld; });
   vr.template load<VEC>(threadIdx.x, nk, sh.D, [&](int i) { return vb + (int64_t)keys.slot(i) * a.v_ld; });
-  bool first = true;
-  ColScale scale;
-  while (nk > 0) {
-    SlotTiles<NW>::sync();
-    kr.store_rows(threadIdx.x, Ks);
-    vr.store_rows(threadIdx.x, Vs);
-    kr.store_tr(threadIdx.x, Kt);
+  ColScale cs;
+  float st = lse;
+  if constexpr (__is_same(T, _Float16)) st -= log2_pow2(cs.sc);              // the scale rides on p
+  for (int buf = 0; nk > 0; buf ^= 1) {
+    T* Ks = tiles + buf * 2 * TILE_E;
+    T* Vs = Ks + TILE_E;
+    kr.store(threadIdx.x, Ks);
+    vr.store(threadIdx.x, Vs);
     const int nn = keys.next(TK);
     kr.template load<VEC>(threadIdx.x, nn, sh.D, [&](int i) { return kb + (int64_t)keys.slot(i) * a.k_ld; });
     vr.template load<VEC>(threadIdx.x, nn, sh.D, [&](int i) { return vb + (int64_t)keys.slot(i) * a.v_ld; });
     SlotTiles<NW>::sync();
-    f32x16 s = dot_rows<T, DP>(Ks, 0, qf, zero16());
-    f32x16 dp = dot_rows<T, DP>(Vs, 0, gf, zero16());
+    if (a.few_keys) {                             // at most 32 keys, all of them here: p normalised by its own sum
+      f32x16 s = dot_rows<T, DP>(Ks, 0, qf, zero16());
+      const f32x16 dp = dot_rows<T, DP>(Vs, 0, gf, zero16());
+      float sum = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = crow(r, h) < nk ? prob(s[r], a.scale, lse) : 0.0f;
-    if (first && nn == 0) {                       // the whole row is here: delta from p and dp, free of out's rounding
-      delta = 0.0f;
+      for (int r = 0; r < 16; ++r) {
+        s[r] = crow(r, h) < nk ? prob<T>(s[r], a.scale, c, lse) : 0.0f;
+        sum += s[r];
+      }
+      sum += __shfl_xor(sum, 32);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) delta = fmaf(s[r], dp[r], delta);
+      for (int r = 0; r < 16; ++r) delta = fmaf(sum == 0.0f ? 0.0f : s[r] / sum, dp[r], delta);
       delta += __shfl_xor(delta, 32);
     }
-    // ds is rounded to the inputs' type for the product, like p in the forward; the sum over keys stays in 32 bits
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
-    if constexpr (__is_same(T, _Float16)) scale.fit(s, acc, DP / 32);
-    dot_cols<T, DP, TK>(Kt, 0, s, acc);
-    first = false;
+    for (int sub = 0; sub < TK; sub += 32) {
+      f32x16 s = dot_rows<T, DP>(Ks, sub, qf, zero16());
+      const f32x16 dp = dot_rows<T, DP>(Vs, sub, gf, zero16());
+      // ds is rounded to the inputs' type for the product, like p in the forward; the sum over keys stays in 32 bits
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = prob<T>(s[r], a.scale, c, st) * (dp[r] - delta);
+      if (sub + 32 > nk) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (sub + crow(r, h) >= nk) s[r] = 0.0f;
+      }
+      if constexpr (__is_same(T, _Float16)) {
+        const float before = cs.sc;
+        cs.fit(s, acc, DP / 32);
+        if (__any(cs.sc != before)) st = lse - log2_pow2(cs.sc);
+      }
+      dot_cols<T, DP>(Ks, sub, s, acc);
+    }
     nk = nn;
   }
   if (!live) return;
-  if (h == 0) a.delta[stat] = delta;
+  if (a.few_keys && h == 0) a.delta[stat] = delta;
   store_col<T, DP, VEC>((T*)a.dq + flat * a.dq_ld + (int64_t)head * sh.D, acc,
-                        __is_same(T, _Float16) ? a.scale / scale.sc : a.scale, sh.D);
-}
-
-template <typename T, int DP>
-constexpr int dkv_lds() {
-  constexpr int rows = 32 * row_pitch<T, DP>() * (int)sizeof(T);
-  return 2 * rows + (sizeof(T) == 2 ? 2 * DP * tr_pitch<32>() * (int)sizeof(T) : 0);
+                        __is_same(T, _Float16) ? a.scale / cs.sc : a.scale, sh.D);
 }
 
 template <typename T, int DP, int NW, bool VEC>
-__global__ void __launch_bounds__(64 * NW, DP == 128 && sizeof(T) == 4 ? 1 : 2) dkv_kernel(BwdArgs a) {
-  constexpr int NT = 64 * NW, TQ = 32, COLS = 32 * NW;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  float* stats = reinterpret_cast<float*>(lds + dkv_lds<T, DP>());          // lse[32], delta[32]
-  int* list = reinterpret_cast<int*>(stats + 64);
-  int* klist = list + kChunk + 64 + 4;
-  const Shape sh = a.sh;
+__device__ __forceinline__ void dkv_body(const BwdArgs& a, int64_t id, char* lds) {
+  constexpr int NT = 64 * NW, TQ = dkv_tile<T, DP>(), COLS = 32 * NW, TILE_E = TQ * row_pitch<T, DP>();
+  float* stats = reinterpret_cast<float*>(lds + 4 * tile_bytes<T, DP, TQ>());          // two of lse[TQ], delta[TQ]
+  int* list = reinterpret_cast<int*>(stats + 4 * TQ);
+  int* klist = list + kListInts;
+  const Shape& sh = a.sh;
   int unit, item;
-  if (!a.map.decode(blockIdx.x, unit, item)) return;
-  const int pair = a.map.units == sh.B ? unit * sh.nkv + item / a.tiles : unit, tile = item % a.tiles;
+  if (!a.map_k.decode(id, unit, item)) return;
+  const int pair = a.map_k.units == sh.B ? unit * sh.nkv + item / a.tiles_k : unit, tile = item % a.tiles_k;
   const int b = pair / sh.nkv, hk = pair - b * sh.nkv;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
   const int k0 = tile * COLS;
@@ -166,8 +180,8 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && sizeof(T) == 4 ? 1 : 2) 
   if (mk) {
     if (threadIdx.x < 64) compact_select(mk, sh.Nk, k0, COLS, klist);
     const int rows = min(COLS, sh.Nk - k0);
-    zero_masked_rows<NT>((T*)a.dk + (int64_t)b * sh.Nk * a.dk_ld + (int64_t)hk * sh.D, a.dk_ld, mk, k0, rows, 1, sh.D);
-    zero_masked_rows<NT>((T*)a.dv + (int64_t)b * sh.Nk * a.dv_ld + (int64_t)hk * sh.D, a.dv_ld, mk, k0, rows, 1, sh.D);
+    zero_masked_rows<NT, VEC>((T*)a.dk + (int64_t)b * sh.Nk * a.dk_ld + (int64_t)hk * sh.D, a.dk_ld, mk, k0, rows, 1, sh.D);
+    zero_masked_rows<NT, VEC>((T*)a.dv + (int64_t)b * sh.Nk * a.dv_ld + (int64_t)hk * sh.D, a.dv_ld, mk, k0, rows, 1, sh.D);
     __syncthreads();
     if (klist[0] < 0) return;
   }
@@ -184,12 +198,11 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && sizeof(T) == 4 ? 1 : 2) 
     dk[t] = zero16();
     dv[t] = zero16();
   }
-  T* Qs = reinterpret_cast<T*>(lds);
-  T* Gs = Qs + TQ * row_pitch<T, DP>();
-  T* Qt = sizeof(T) == 2 ? Gs + TQ * row_pitch<T, DP>() : Qs;
-  T* Gt = sizeof(T) == 2 ? Qt + DP * tr_pitch<TQ>() : Gs;
+  const float c = a.scale * kLog2e;
+  T* tiles = reinterpret_cast<T*>(lds);
   TileRegs<T, DP, TQ, NT> qr, gr;
-  ColScale scale;
+  ColScale cs;
+  int buf = 0;
   for (int gi = 0; gi < sh.g; ++gi) {
     const int head = hk * sh.g + gi;
     const T* qb = (const T*)a.q + (int64_t)b * sh.Nq * a.q_ld + (int64_t)head * sh.D;
@@ -197,7 +210,6 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && sizeof(T) == 4 ? 1 : 2) 
     const int64_t stat = ((int64_t)b * sh.nh + head) * sh.Nq;
     float st_l = 0.0f, st_d = 0.0f;
     SlotTiles<NW> rows;
-    SlotTiles<NW>::sync();                        // the list of the head before this one has been read
     rows.init(mq, 0, sh.Nq, list, list + kChunk + 64);
     int nq = rows.next(TQ);
     auto fetch = [&](int n) {
@@ -205,107 +217,147 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && sizeof(T) == 4 ? 1 : 2) 
       gr.template load<VEC>(threadIdx.x, n, sh.D, [&](int i) { return gb + (int64_t)rows.slot(i) * a.dout_ld; });
       st_l = INFINITY;                            // rows past the end, and rows without a key: p = 0
       st_d = 0.0f;
-      if (threadIdx.x < 32 && threadIdx.x < n) {
+      if (threadIdx.x < TQ && threadIdx.x < n) {
         const int s = rows.slot(threadIdx.x);
-        const float v = a.lse[stat + s];
-        if (v != -INFINITY) {
-          st_l = v;
-          st_d = a.delta[stat + s];
-        }
+        st_l = row_stat<T>(a.lse[stat + s]);
+        if (st_l < INFINITY) st_d = a.delta[stat + s];
+        if (__is_same(T, _Float16)) st_l -= kHalfLog;
       }
     };
     fetch(nq);
-    while (nq > 0) {
-      SlotTiles<NW>::sync();
-      qr.store_rows(threadIdx.x, Qs);
-      gr.store_rows(threadIdx.x, Gs);
-      qr.store_tr(threadIdx.x, Qt);
-      gr.store_tr(threadIdx.x, Gt);
-      if (threadIdx.x < 32) {
-        stats[threadIdx.x] = st_l;
-        stats[32 + threadIdx.x] = st_d;
+    for (; nq > 0; buf ^= 1) {
+      T* Qs = tiles + buf * 2 * TILE_E;
+      T* Gs = Qs + TILE_E;
+      float* sl = stats + buf * 2 * TQ;
+      qr.store(threadIdx.x, Qs);
+      gr.store(threadIdx.x, Gs);
+      if (threadIdx.x < TQ) {
+        sl[threadIdx.x] = st_l;
+        sl[TQ + threadIdx.x] = st_d;
       }
       const int nn = rows.next(TQ);
       fetch(nn);
       SlotTiles<NW>::sync();
-      f32x16 s = dot_rows<T, DP>(Qs, 0, kf, zero16());
-      f32x16 dp = dot_rows<T, DP>(Gs, 0, vf, zero16());
 #pragma unroll
-      for (int g4 = 0; g4 < 4; ++g4) {
-        const float4 ls = *reinterpret_cast<const float4*>(stats + 8 * g4 + 4 * h);
-        const float4 dl = *reinterpret_cast<const float4*>(stats + 32 + 8 * g4 + 4 * h);
-        const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dv4[4] = {dl.x, dl.y, dl.z, dl.w};
+      for (int sub = 0; sub < TQ; sub += 32) {
+        f32x16 s = dot_rows<T, DP>(Qs, sub, kf, zero16());
+        f32x16 dp = dot_rows<T, DP>(Gs, sub, vf, zero16());
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 4 * g4 + i;
-          s[r] = prob(s[r], a.scale, lv[i]);
-          dp[r] = s[r] * (dp[r] - dv4[i]);
+        for (int g4 = 0; g4 < 4; ++g4) {
+          const f32x4 ls = *reinterpret_cast<const f32x4*>(sl + sub + 8 * g4 + 4 * h);
+          const f32x4 dl = *reinterpret_cast<const f32x4*>(sl + TQ + sub + 8 * g4 + 4 * h);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 4 * g4 + i;
+            s[r] = prob<T>(s[r], a.scale, c, ls[i]);
+            dp[r] = s[r] * (dp[r] - dl[i]);
+          }
         }
-      }
-      if constexpr (__is_same(T, _Float16)) {
+        if constexpr (__is_same(T, _Float16)) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] *= kHalfP;
-        scale.fit(dp, dk, DP / 32);
+          for (int r = 0; r < 16; ++r) dp[r] *= cs.sc;
+          cs.fit(dp, dk, DP / 32);
+        }
+        dot_cols<T, DP>(Gs, sub, s, dv);
+        dot_cols<T, DP>(Qs, sub, dp, dk);
       }
-      dot_cols<T, DP, TQ>(Gt, 0, s, dv);
-      dot_cols<T, DP, TQ>(Qt, 0, dp, dk);
       nq = nn;
     }
   }
   if (key < 0) return;
+  // (dp carried p's 2^12 too)
   store_col<T, DP, VEC>((T*)a.dk + flat * a.dk_ld + (int64_t)hk * sh.D, dk,
-                        __is_same(T, _Float16) ? a.scale / scale.sc : a.scale, sh.D);
+                        __is_same(T, _Float16) ? a.scale / kHalfP / cs.sc : a.scale, sh.D);
   store_col<T, DP, VEC>((T*)a.dv + flat * a.dv_ld + (int64_t)hk * sh.D, dv,
                         __is_same(T, _Float16) ? 1.0f / kHalfP : 1.0f, sh.D);
 }
 
-// ---- host --------------------------------------------------------------------------------------------------------
-static int waves_for(int64_t rows) { return rows > 64 ? 4 : rows > 32 ? 2 : 1; }
+// workgroups [0, n_dkv) own keys, the others query rows
+template <typename T, int DP, int NW, bool VEC>
+__global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) bwd_kernel(BwdArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  if (blockIdx.x < a.n_dkv) dkv_body<T, DP, NW, VEC>(a, blockIdx.x, lds);
+  else dq_body<T, DP, NW, VEC>(a, blockIdx.x - a.n_dkv, lds);
+}
 
-template <typename K>
-static int launch(K kern, PerDeviceOnce& once, const BwdArgs& a, int threads, int bytes, hipStream_t st, const char* what) {
+// delta of every (row, head): LP lanes a head, its chunks dealt to them
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) delta_kernel(BwdArgs a, int lp) {
+  constexpr int E = Traits<T>::EPC;
+  const Shape sh = a.sh;
+  const int64_t items = (int64_t)sh.B * sh.Nq * sh.nh, per = 256 / lp;
+  const int sub = threadIdx.x % lp;
+  for (int64_t it = (int64_t)blockIdx.x * per + threadIdx.x / lp; it < items; it += (int64_t)gridDim.x * per) {
+    const int64_t row = it / sh.nh;
+    const int head = (int)(it - row * sh.nh);
+    const T* o = (const T*)a.out + row * a.out_ld + (int64_t)head * sh.D;
+    const T* g = (const T*)a.dout + row * a.dout_ld + (int64_t)head * sh.D;
+    float s = 0.0f;
+    for (int ch = sub; ch * E < sh.D; ch += lp) {
+      T x[E], y[E];
+      const u32x4 u = load_chunk<T, VEC>(o, ch * E, sh.D, true), v = load_chunk<T, VEC>(g, ch * E, sh.D, true);
+      __builtin_memcpy(x, &u, 16);
+      __builtin_memcpy(y, &v, 16);
+#pragma unroll
+      for (int i = 0; i < E; ++i) s = fmaf((float)x[i], (float)y[i], s);
+    }
+    for (int o2 = lp >> 1; o2 > 0; o2 >>= 1) s += __shfl_xor(s, o2, 64);
+    if (sub == 0) {
+      const int64_t bb = row / sh.Nq;
+      a.delta[(bb * sh.nh + head) * sh.Nq + (row - bb * sh.Nq)] = s;
+    }
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------
+template <typename T, int DP, int NW, bool VEC>
+static int run_bwd(BwdArgs& a, hipStream_t st) {
+  constexpr int bytes = bwd_lds<T, DP, NW>();
+  static_assert(bytes <= 160 * 1024, "LDS");
+  auto kern = bwd_kernel<T, DP, NW, VEC>;
+  static PerDeviceOnce once;
   if (bytes > 64 * 1024 &&
       !once.run([&] { return hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess; })) {
-    set_error("%s: the runtime refuses %d bytes of LDS", what, bytes);
+    set_error("mmb_cross_attention_bwd: the runtime refuses %d bytes of LDS", bytes);
     return MMB_ERR_LAUNCH;
   }
-  kern<<<dim3((unsigned)a.map.blocks()), dim3(threads), bytes, st>>>(a);
-  return check_launch(what);
+  const Shape& s = a.sh;
+  a.tiles_q = (int)(((int64_t)s.g * s.Nq + 32 * NW - 1) / (32 * NW));
+  a.tiles_k = (int)(((int64_t)s.Nk + 32 * NW - 1) / (32 * NW));
+  a.map_q = grid_map(s.B, s.nkv, a.tiles_q);
+  a.map_k = grid_map(s.B, s.nkv, a.tiles_k);
+  const int64_t nq = a.map_q.blocks(), nk = a.map_k.blocks();
+  MMB_REQUIRE(nq + nk <= 0x7fffffffLL, "mmb_cross_attention_bwd: %lld workgroups", (long long)(nq + nk));
+  a.few_keys = s.Nk <= 32;
+  if (a.few_keys) {
+    a.n_dkv = 0;
+    kern<<<dim3((unsigned)nq), dim3(64 * NW), bytes, st>>>(a);
+    if (int rc = check_launch("mmb_cross_attention_bwd (dq)")) return rc;
+    a.n_dkv = (unsigned)nk;
+    kern<<<dim3((unsigned)nk), dim3(64 * NW), bytes, st>>>(a);
+    return check_launch("mmb_cross_attention_bwd (dk, dv)");
+  }
+  constexpr int E = Traits<T>::EPC;
+  int lp = 1;
+  while (lp * E < s.D && lp < 16) lp *= 2;
+  delta_kernel<T, VEC><<<stream_grid((int64_t)s.B * s.Nq * s.nh * lp, 256), 256, 0, st>>>(a, lp);
+  if (int rc = check_launch("mmb_cross_attention_bwd (delta)")) return rc;
+  a.n_dkv = (unsigned)nk;
+  kern<<<dim3((unsigned)(nq + nk)), dim3(64 * NW), bytes, st>>>(a);
+  return check_launch("mmb_cross_attention_bwd");
 }
-
-template <typename T, int DP, int NW, bool VEC>
-static int launch_dq(const BwdArgs& a, hipStream_t st) {
-  static PerDeviceOnce once;
-  constexpr int bytes = dq_lds<T, DP, 32>() + (kChunk + 64 + 4 + 32 * NW + 4) * 4;
-  return launch(dq_kernel<T, DP, NW, VEC>, once, a, 64 * NW, bytes, st, "mmb_cross_attention_bwd (dq)");
-}
-template <typename T, int DP, int NW, bool VEC>
-static int launch_dkv(const BwdArgs& a, hipStream_t st) {
-  static PerDeviceOnce once;
-  constexpr int bytes = dkv_lds<T, DP>() + (64 + kChunk + 64 + 4 + 32 * NW + 4) * 4;
-  return launch(dkv_kernel<T, DP, NW, VEC>, once, a, 64 * NW, bytes, st, "mmb_cross_attention_bwd (dk, dv)");
-}
-
+// waves of a workgroup (32 rows or keys each): as many as the shorter side fills, so that its workgroups do not idle
 template <typename T, int DP, bool VEC>
-static int run_bwd(BwdArgs& a, hipStream_t st) {
-  const int64_t R = (int64_t)a.sh.g * a.sh.Nq;
-  const int nw_q = waves_for(R), nw_k = waves_for(a.sh.Nk);
-  a.tiles = (int)((R + 32 * nw_q - 1) / (32 * nw_q));
-  a.map = grid_map(a.sh.B, a.sh.nkv, a.tiles);
-  MMB_REQUIRE(a.map.blocks() <= 0x7fffffffLL, "mmb_cross_attention_bwd: %lld workgroups", (long long)a.map.blocks());
-  int rc = nw_q == 4 ? launch_dq<T, DP, 4, VEC>(a, st) : nw_q == 2 ? launch_dq<T, DP, 2, VEC>(a, st) : launch_dq<T, DP, 1, VEC>(a, st);
-  if (rc != MMB_OK) return rc;
-  a.tiles = (int)(((int64_t)a.sh.Nk + 32 * nw_k - 1) / (32 * nw_k));
-  a.map = grid_map(a.sh.B, a.sh.nkv, a.tiles);
-  MMB_REQUIRE(a.map.blocks() <= 0x7fffffffLL, "mmb_cross_attention_bwd: %lld workgroups", (long long)a.map.blocks());
-  return nw_k == 4 ? launch_dkv<T, DP, 4, VEC>(a, st) : nw_k == 2 ? launch_dkv<T, DP, 2, VEC>(a, st) : launch_dkv<T, DP, 1, VEC>(a, st);
+static int pick_nw(BwdArgs& a, hipStream_t st) {
+  const int64_t R = (int64_t)a.sh.g * a.sh.Nq, m = R < a.sh.Nk ? R : a.sh.Nk;
+  return m > 64 ? run_bwd<T, DP, 4, VEC>(a, st) : m > 32 ? run_bwd<T, DP, 2, VEC>(a, st) : run_bwd<T, DP, 1, VEC>(a, st);
 }
 template <typename T, bool VEC>
 static int pick_dp(BwdArgs& a, hipStream_t st) {
   switch (pad_width(a.sh.D)) {
-    case 32: return run_bwd<T, 32, VEC>(a, st);
-    case 64: return run_bwd<T, 64, VEC>(a, st);
-    default: return run_bwd<T, 128, VEC>(a, st);
+    case 32: return pick_nw<T, 32, VEC>(a, st);
+    case 64: return pick_nw<T, 64, VEC>(a, st);
+    default: return pick_nw<T, 128, VEC>(a, st);
   }
 }
 
@@ -331,7 +383,7 @@ extern "C" int mmb_cross_attention_bwd(int B, int Nq, int Nk, int nheads, int nh
   MMB_REQUIRE(workspace && workspace_bytes >= need, "mmb_cross_attention_bwd: workspace of %lld bytes needed, got %lld",
               (long long)need, (long long)(workspace ? workspace_bytes : 0));
   BwdArgs a = {{B, Nq, Nk, nheads, nheads_kv, D, nheads / nheads_kv}, q, k, v, out, dout, q_ld, k_ld, v_ld, out_ld, dout_ld,
-               dq_ld, dk_ld, dv_ld, maskf_q, maskf_k, lse, scale, dq, dk, dv, (float*)workspace, 0, {}};
+               dq_ld, dk_ld, dv_ld, maskf_q, maskf_k, lse, scale, dq, dk, dv, (float*)workspace, false, 0, 0, {}, {}, 0};
   const int es = dtype == MMB_DT_F32 ? 4 : 2;
   const bool vec = D * es % 16 == 0 && chunk_aligned(q, q_ld, es) && chunk_aligned(k, k_ld, es) && chunk_aligned(v, v_ld, es) &&
                    chunk_aligned(out, out_ld, es) && chunk_aligned(dout, dout_ld, es) && chunk_aligned(dq, dq_ld, es) &&

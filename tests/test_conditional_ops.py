@@ -168,17 +168,30 @@ def test_cross_attention_masked_slots_hold_anything(dtype, Nq, Nk):
     assert not got["out"][Nq:2 * Nq].any()                      # the cloud without a key
 
 
-def test_cross_attention_single_key_is_exact():
-    """One kept key: out is its value row, dq and dk are exactly zero, dv the sum of dout over the group."""
-    B, Nq, Nk, nh, nkv, D = 2, 9, 40, 4, 2, 64
+@pytest.mark.parametrize("Nk,at", [(40, (17, 39)), (20, (0, 19))])
+def test_cross_attention_single_key(Nk, at):
+    """One kept key: out is its value row.  dq and dk are zero: exactly with up to 32 slots, where delta comes from the row's
+    own p and dp; else to what dp and delta = do . o -- the same D products, summed in 32 bits in two orders, so at most
+    2 (D + 2) e times the sum of their magnitudes apart -- leave of each other (p = 1 to FN; half precision adds its step)."""
+    B, Nq, nh, nkv, D = 2, 9, 4, 2, 64
     for dt in TYPES.values():
         q, k, v, do, _, _ = make(B, Nq, Nk, nh, nkv, D, dt, 3, False)
         mk = torch.zeros(B, Nk)
-        mk[0, 17], mk[1, 39] = 1, 1
+        mk[0, at[0]], mk[1, at[1]] = 1, 1
         got = run_attention(q, k, v, do, None, mk, B, nh, nkv, 0.125)
-        row = torch.stack([v.view(B, Nk, nkv, D)[b, s] for b, s in ((0, 17), (1, 39))]).repeat_interleave(nh // nkv, 1)
-        assert torch.equal(got["out"].cpu().view(B, Nq, nh, D), row[:, None].expand(B, Nq, nh, D))
-        assert not got["dq"].any() and not got["dk"].any()
+        one = lambda t: torch.stack([t.view(B, Nk, nkv, D)[b, s] for b, s in enumerate(at)]).repeat_interleave(nh // nkv, 1)  # noqa: E731
+        assert torch.equal(got["out"].cpu().view(B, Nq, nh, D), one(v)[:, None].expand(B, Nq, nh, D))
+        if Nk <= 32:
+            assert not got["dq"].any() and not got["dk"].any()
+            continue
+        ds = 2 * (D + 2) * E * (do.double().view(B, Nq, nh, D).abs() * one(v).double().abs()[:, None]).sum(-1, keepdim=True) * (1 + FN)
+        ds = ds * (1 + u(dt))                                   # (its rounding for the product)
+        t_dq = 0.125 * ds * one(k).double().abs()[:, None]
+        t_dk = 0.125 * (ds * q.double().view(B, Nq, nh, D).abs()).view(B, Nq, nkv, nh // nkv, D).sum((1, 3))
+        within(got["dq"].view(B, Nq, nh, D), torch.zeros(B, Nq, nh, D).double(), t_dq + out_step(dt, t_dq) + 1e-30, "dq")
+        dk = got["dk"].view(B, Nk, nkv, D)
+        within(torch.stack([dk[b, s] for b, s in enumerate(at)]), torch.zeros_like(t_dk), t_dk + out_step(dt, t_dk) + 1e-30, "dk")
+        assert not dk[0, :at[0]].any() and not dk[1, :at[1]].any()
 
 
 def test_cross_attention_values_that_are_not_finite():
