@@ -189,6 +189,7 @@ struct SlotTiles {
 // 16-bit: row-major without padding, the 16-byte chunks of a row permuted by an exclusive-or with a function of the row
 //         that serves both kinds of read: 16 rows at one chunk column (the scores) and four rows of 16 columns (the
 //         transposing read of the second product) each fall on 64 different banks.
+template <int DP> constexpr int feature_tiles() { return DP < 32 ? 1 : DP / 32; }      // 32-row accumulators of DP features
 template <typename T, int DP> constexpr int row_pitch() { return sizeof(T) == 2 ? DP : DP + 4; }
 template <int DP>
 __device__ __forceinline__ int swizzle(int row) {
@@ -242,6 +243,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 // out[t] (features 32t.. x columns) += X^T . w, the contraction over the 32 rows row0.. that w's registers run over.
+// (DP = 16, floats: the upper half of the feature rows multiplies what lies behind a row; it is never stored, the caller
+// keeps 16 elements behind the last row addressable.)
 // 16-bit: X^T by the transposing read: the 16 lanes that hold 16 columns address four rows (lane j: row j >> 2, columns
 // from 4 (j & 3)) and receive four rows of their own column.  float: one element a lane and step.
 template <typename T, int DP>
@@ -253,7 +256,7 @@ __device__ __forceinline__ void dot_cols(const T* x, int row0, const f32x16& w, 
     for (int g = 0; g < 2; ++g) {
       const u32x4 b = pack8<T>(w, 8 * g);
 #pragma unroll
-      for (int t = 0; t < DP / 32; ++t) {
+      for (int t = 0; t < feature_tiles<DP>(); ++t) {
         union { s16x4 v[2]; u32x4 a; } f;
 #pragma unroll
         for (int r = 0; r < 2; ++r)
@@ -265,7 +268,7 @@ __device__ __forceinline__ void dot_cols(const T* x, int row0, const f32x16& w, 
 #pragma unroll
     for (int r = 0; r < 16; ++r)
 #pragma unroll
-      for (int t = 0; t < DP / 32; ++t)
+      for (int t = 0; t < feature_tiles<DP>(); ++t)
         out[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[(row0 + crow(r, h)) * row_pitch<T, DP>() + 32 * t + col], w[r], out[t], 0, 0, 0);
   }
 }
@@ -318,7 +321,7 @@ template <typename T, int DP, bool VEC>
 __device__ __forceinline__ void store_col(T* __restrict__ p, const f32x16* acc, float mul, int D) {
   const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
-  for (int t = 0; t < DP / 32; ++t)
+  for (int t = 0; t < feature_tiles<DP>(); ++t)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = 32 * t + 8 * g + 4 * h;
@@ -334,6 +337,74 @@ __device__ __forceinline__ void store_col(T* __restrict__ p, const f32x16* acc, 
       }
     }
 }
+
+// One tile of n keys (K rows and V in LDS): scores, running softmax, o += V^T P.
+template <typename T, int DP, int TK>
+__device__ __forceinline__ void attend(const T* Ks, const T* Vs, int n, const u32x4* qf, float c,
+                                       float& m, float& l, f32x16* acc) {
+  const int h = (threadIdx.x & 63) >> 5;
+  f32x16 s[TK / 32];
+#pragma unroll
+  for (int st = 0; st < TK / 32; ++st) s[st] = dot_rows<T, DP>(Ks, 32 * st, qf, zero16());
+  if (n < TK) {
+#pragma unroll
+    for (int st = 0; st < TK / 32; ++st)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (32 * st + crow(r, h) >= n) s[st][r] = -INFINITY;
+  }
+  float top = s[0][0];
+#pragma unroll
+  for (int st = 0; st < TK / 32; ++st)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[st][r]);
+  top = fmaxf(top, __shfl_xor(top, 32));
+  const float mn = fmaxf(m, top);
+  const float ms = mn == -INFINITY ? 0.0f : mn;   // every score so far -inf: nothing to subtract
+  if (__any(mn > m)) {
+    const float alpha = __builtin_amdgcn_exp2f((m - ms) * c);
+    l *= alpha;
+#pragma unroll
+    for (int t = 0; t < feature_tiles<DP>(); ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[t][r] *= alpha;
+    m = mn;
+  }
+#pragma unroll
+  for (int st = 0; st < TK / 32; ++st)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      // 16-bit inputs: one fused step (the rounding of ms * c moves all p of a row alike and cancels); float: the
+      // difference first, which is exact next to the maximum
+      s[st][r] = __builtin_amdgcn_exp2f(sizeof(T) == 2 ? fmaf(s[st][r], c, -ms * c) : (s[st][r] - ms) * c);
+      l += s[st][r];
+    }
+  // p is rounded to the inputs' type for the product (16-bit types: half a step of a value in [0, 1], the size of the
+  // output's own rounding; l sums the unrounded values), the sums over keys stay in 32 bits
+#pragma unroll
+  for (int st = 0; st < TK / 32; ++st) dot_cols<T, DP>(Vs, 32 * st, s[st], acc);
+}
+
+// p from a raw score; st: lse, for 16-bit types in units of log 2.  float: the product and the difference are rounded apart,
+// so that a row with a single key, whose log-sum IS its rounded score, gets exactly 1.
+template <typename T>
+__device__ __forceinline__ float prob(float s, float scale, float c, float st) {
+#pragma clang fp contract(off)
+  if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -st));
+  const float t = s * scale;
+  return __builtin_amdgcn_exp2f((t - st) * kLog2e);
+}
+// a row without a key (or only scores of -inf): p = 0
+template <typename T>
+__device__ __forceinline__ float row_stat(float lse) {
+  return lse == -INFINITY ? INFINITY : sizeof(T) == 2 ? lse * kLog2e : lse;
+}
+
+// half precision: p in [0, 1] takes 2^12 into the product (p = 1 / Nk of a long list would be subnormal)
+constexpr float kHalfLog = 12.0f, kHalfP = 4096.0f;
+
+// log2 of a power of two
+__device__ __forceinline__ float log2_pow2(float x) { return (float)((int)(__float_as_uint(x) >> 23) - 127); }
 
 // Workgroup id -> (unit, item): units (clouds, or (cloud, key head) pairs when there are few clouds) are dealt to the
 // eight XCDs in turn and all items of a unit stay on one XCD, whose L2 then holds the rows they share.
@@ -392,6 +463,14 @@ struct RowTile {
 struct Shape {
   int B, Nq, Nk, nh, nkv, D, g;                   // g = nh / nkv query heads share one key head
 };
+
+// small clouds (cross_attention_resident.hip); resident_heads: key heads of a workgroup, 0 where the streaming kernels serve
+int resident_heads(const Shape& s, int dtype, bool bwd);
+int resident_fwd(const Shape& s, int hw, int dtype, bool vec, const void* q, int64_t q_ld, const void* k, int64_t k_ld, const void* v,
+                 int64_t v_ld, const float* mq, const float* mk, float scale, void* out, int64_t out_ld, float* lse, hipStream_t st);
+int resident_bwd(const Shape& s, int hw, int dtype, bool vec, const void* q, int64_t q_ld, const void* k, int64_t k_ld, const void* v,
+                 int64_t v_ld, const float* mq, const float* mk, float scale, const void* out, int64_t out_ld, const void* dout,
+                 int64_t dout_ld, const float* lse, void* dq, int64_t dq_ld, void* dk, int64_t dk_ld, void* dv, int64_t dv_ld, hipStream_t st);
 
 inline int pad_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 int check_shape(const char* who, int B, int Nq, int Nk, int nh, int nkv, int D, int dtype, float scale);

@@ -34,53 +34,6 @@ struct FwdArgs {
 template <typename T, int DP, int TK, bool SPLIT>
 constexpr int kv_lds() { return 2 * (SPLIT ? 1 : 2) * tile_bytes<T, DP, TK>(); }
 
-// One tile of n keys (K rows and V in LDS): scores, running softmax, o += V^T P.
-template <typename T, int DP, int TK>
-__device__ __forceinline__ void attend(const T* __restrict__ Ks, const T* __restrict__ Vs, int n, const u32x4* qf, float c,
-                                       float& m, float& l, f32x16* acc) {
-  const int h = (threadIdx.x & 63) >> 5;
-  f32x16 s[TK / 32];
-#pragma unroll
-  for (int st = 0; st < TK / 32; ++st) s[st] = dot_rows<T, DP>(Ks, 32 * st, qf, zero16());
-  if (n < TK) {
-#pragma unroll
-    for (int st = 0; st < TK / 32; ++st)
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (32 * st + crow(r, h) >= n) s[st][r] = -INFINITY;
-  }
-  float top = s[0][0];
-#pragma unroll
-  for (int st = 0; st < TK / 32; ++st)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[st][r]);
-  top = fmaxf(top, __shfl_xor(top, 32));
-  const float mn = fmaxf(m, top);
-  const float ms = mn == -INFINITY ? 0.0f : mn;   // every score so far -inf: nothing to subtract
-  if (__any(mn > m)) {
-    const float alpha = __builtin_amdgcn_exp2f((m - ms) * c);
-    l *= alpha;
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[t][r] *= alpha;
-    m = mn;
-  }
-#pragma unroll
-  for (int st = 0; st < TK / 32; ++st)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      // 16-bit inputs: one fused step (the rounding of ms * c moves all p of a row alike and cancels); float: the
-      // difference first, which is exact next to the maximum
-      s[st][r] = __builtin_amdgcn_exp2f(sizeof(T) == 2 ? fmaf(s[st][r], c, -ms * c) : (s[st][r] - ms) * c);
-      l += s[st][r];
-    }
-  // p is rounded to the inputs' type for the product (16-bit types: half a step of a value in [0, 1], the size of the
-  // output's own rounding; l sums the unrounded values), the sums over keys stay in 32 bits
-#pragma unroll
-  for (int st = 0; st < TK / 32; ++st) dot_cols<T, DP>(Vs, 32 * st, s[st], acc);
-}
-
 template <typename T, int DP, int NW, int TK, bool SPLIT, bool VEC>
 __global__ void __launch_bounds__(64 * NW, 2) fwd_kernel(FwdArgs a) {
   constexpr int NT = 64 * NW, TEAM = SPLIT ? 1 : NW, TT = 64 * TEAM, ROWS = SPLIT ? 32 : 32 * NW;
@@ -357,7 +310,7 @@ extern "C" int mmb_cross_attention_workspace(int B, int Nq, int Nk, int nheads, 
     return MMB_OK;
   }
   const Plan p = fwd_plan(s);
-  *bytes_host = p.nsplit > 1 ? (int64_t)B * nheads_kv * p.tiles * p.nsplit * 32 * (pad_width(D) + 2) * 4 : 0;
+  *bytes_host = p.nsplit > 1 && !resident_heads(s, dtype, false) ? (int64_t)B * nheads_kv * p.tiles * p.nsplit * 32 * (pad_width(D) + 2) * 4 : 0;
   return MMB_OK;
 }
 
@@ -371,6 +324,11 @@ extern "C" int mmb_cross_attention_fwd(int B, int Nq, int Nk, int nheads, int nh
                   v_ld >= (int64_t)nheads_kv * D,
               "mmb_cross_attention_fwd: a leading dimension is smaller than its row");
   const Shape s = {B, Nq, Nk, nheads, nheads_kv, D, nheads / nheads_kv};
+  const int es = dtype == MMB_DT_F32 ? 4 : 2;
+  const bool vec = D * es % 16 == 0 && chunk_aligned(q, q_ld, es) && chunk_aligned(k, k_ld, es) && chunk_aligned(v, v_ld, es) &&
+                   chunk_aligned(out, out_ld, es);
+  if (const int hw = resident_heads(s, dtype, false))
+    return resident_fwd(s, hw, dtype, vec, q, q_ld, k, k_ld, v, v_ld, maskf_q, maskf_k, scale, out, out_ld, lse, as_stream(stream));
   const Plan p = fwd_plan(s);
   const int64_t need = p.nsplit > 1 ? (int64_t)B * nheads_kv * p.tiles * p.nsplit * 32 * (pad_width(D) + 2) * 4 : 0;
   MMB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "mmb_cross_attention_fwd: workspace of %lld bytes needed, got %lld",
@@ -378,9 +336,6 @@ extern "C" int mmb_cross_attention_fwd(int B, int Nq, int Nk, int nheads, int nh
   FwdArgs a = {s, q, k, v, q_ld, k_ld, v_ld, out_ld, maskf_q, maskf_k, scale, out, lse, (float*)workspace, p.tiles, p.nsplit, p.chunk,
                grid_map(B, nheads_kv, p.tiles * p.nsplit)};
   MMB_REQUIRE(a.map.blocks() <= 0x7fffffffLL, "mmb_cross_attention_fwd: %lld workgroups", (long long)a.map.blocks());
-  const int es = dtype == MMB_DT_F32 ? 4 : 2;
-  const bool vec = D * es % 16 == 0 && chunk_aligned(q, q_ld, es) && chunk_aligned(k, k_ld, es) && chunk_aligned(v, v_ld, es) &&
-                   chunk_aligned(out, out_ld, es);
   hipStream_t st = as_stream(stream);
   if (dtype == MMB_DT_F32) return vec ? pick_dp<float, true>(p, a, st) : pick_dp<float, false>(p, a, st);
   if (dtype == MMB_DT_BF16) return vec ? pick_dp<__bf16, true>(p, a, st) : pick_dp<__bf16, false>(p, a, st);

@@ -29,26 +29,6 @@ struct BwdArgs {
   unsigned n_dkv;                                 // workgroups of this launch that own keys
 };
 
-// log2 of a power of two
-__device__ __forceinline__ float log2_pow2(float x) { return (float)((int)(__float_as_uint(x) >> 23) - 127); }
-
-// p from a raw score; st: lse, for 16-bit types in units of log 2.  float: the product and the difference are rounded apart,
-// so that a row with a single key, whose log-sum IS its rounded score, gets exactly 1.
-template <typename T>
-__device__ __forceinline__ float prob(float s, float scale, float c, float st) {
-#pragma clang fp contract(off)
-  if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -st));
-  const float t = s * scale;
-  return __builtin_amdgcn_exp2f((t - st) * kLog2e);
-}
-// a row without a key (or only scores of -inf): p = 0
-template <typename T>
-__device__ __forceinline__ float row_stat(float lse) {
-  return lse == -INFINITY ? INFINITY : sizeof(T) == 2 ? lse * kLog2e : lse;
-}
-
-// half precision: p in [0, 1] takes 2^12 into the product (p = 1 / Nk of a long list would be subnormal)
-constexpr float kHalfLog = 12.0f, kHalfP = 4096.0f;
 
 // keys of a dq tile, queries of a dk / dv tile: as many as leave two workgroups on a CU room for their registers
 template <typename T, int DP> constexpr int dq_tile() { return sizeof(T) == 2 ? 64 : 32; }
@@ -389,6 +369,9 @@ extern "C" int mmb_cross_attention_bwd(int B, int Nq, int Nk, int nheads, int nh
                    chunk_aligned(out, out_ld, es) && chunk_aligned(dout, dout_ld, es) && chunk_aligned(dq, dq_ld, es) &&
                    chunk_aligned(dk, dk_ld, es) && chunk_aligned(dv, dv_ld, es);
   hipStream_t st = as_stream(stream);
+  if (const int hw = resident_heads(a.sh, dtype, true))
+    return resident_bwd(a.sh, hw, dtype, vec, q, q_ld, k, k_ld, v, v_ld, maskf_q, maskf_k, scale, out, out_ld, dout, dout_ld, lse, dq,
+                        dq_ld, dk, dk_ld, dv, dv_ld, st);
   if (dtype == MMB_DT_F32) return vec ? pick_dp<float, true>(a, st) : pick_dp<float, false>(a, st);
   if (dtype == MMB_DT_BF16) return vec ? pick_dp<__bf16, true>(a, st) : pick_dp<__bf16, false>(a, st);
   return vec ? pick_dp<_Float16, true>(a, st) : pick_dp<_Float16, false>(a, st);

@@ -1,0 +1,398 @@
+// Cross attention of small clouds (jets): the keys of a head fit into LDS whole.
+//
+// With some hundred slots a cloud is a few 32 x 32 tiles a head, and what a call costs is not its products but the chain
+// mask -> kept slots -> rows -> products of every workgroup.  Here a workgroup owns one cloud and as many of its heads as LDS
+// holds: the masks are read and compacted once for all of them, the rows of these heads are read side by side (whole cache
+// lines), and after ONE barrier every wave walks its own (head, 32 rows) items without meeting the others.  The reverse does
+// this twice, with K and V resident for dq and with q and dout resident for dk and dv; delta stays in LDS between the two.
+#include "cross_attention.h"
+
+namespace mmb {
+namespace xattn {
+
+// 16-wide heads of floats keep 16-wide rows (half the score products); every other width is padded to 32, 64 or 128
+template <typename T, int DP>
+struct ResTile {
+  static constexpr int E = Traits<T>::EPC, CH = DP / E, PITCH = row_pitch<T, DP>(), FT = DP < 32 ? 1 : DP / 32;
+};
+
+struct ResArgs {
+  Shape sh;
+  const void *q, *k, *v, *out, *dout;
+  int64_t q_ld, k_ld, v_ld, out_ld, dout_ld, dq_ld, dk_ld, dv_ld;
+  const float *mq, *mk;
+  float* lse;
+  float scale;
+  void *o, *dq, *dk, *dv;
+  int hw, parts;                                  // key heads of a workgroup; workgroups that share a cloud's query tiles (forward)
+  int nkp, nqp;                                   // slots padded to 32
+  GridMap map;                                    // units = clouds, items = head groups * parts
+};
+
+// kept slots of a mask (or all), one wave; returns their number
+__device__ __forceinline__ int keep_list(const float* __restrict__ maskf, int N, int* list) {
+  if (maskf == nullptr) {
+    for (int i = threadIdx.x & 63; i < N; i += 64) list[i] = i;
+    return N;
+  }
+  int c = 0;
+  for (int lo = 0; lo < N; lo += kChunk) c += compact_chunk(maskf, lo, N, list + c);
+  return c;
+}
+
+// rows of `heads` neighbouring heads into LDS: [head][rows, padded to 32 with zeros][DP]
+template <typename T, int DP, bool VEC>
+__device__ __forceinline__ void fill(T* __restrict__ dst, int head_stride, int heads, const T* __restrict__ src, int64_t ld, const int* list, int n, int D) {
+  using R = ResTile<T, DP>;
+  const int n32 = (n + 31) & ~31, per = heads * R::CH, work = n32 * per;
+#pragma unroll 4
+  for (int it = threadIdx.x; it < work; it += blockDim.x) {
+    const int row = it / per, x = it - row * per, hd = x / R::CH, ch = x % R::CH;
+    const bool ok = row < n;
+    const u32x4 c = load_chunk<T, VEC>(ok ? src + (int64_t)list[row] * ld + (int64_t)hd * D : nullptr, ch * R::E, D, ok);
+    *reinterpret_cast<u32x4*>(dst + hd * head_stride + chunk_at<T, DP>(row, ch)) = c;
+  }
+}
+
+template <typename T, int DP, int NW, bool VEC>
+__global__ void __launch_bounds__(64 * NW, DP == 128 ? 2 : 3) res_fwd_kernel(ResArgs a) {
+  using R = ResTile<T, DP>;
+  constexpr int S = DP / (2 * R::E);
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const Shape& sh = a.sh;
+  int b, item;
+  if (!a.map.decode(blockIdx.x, b, item)) return;
+  const int hk0 = item / a.parts * a.hw, part = item % a.parts;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
+  const int head_stride = a.nkp * R::PITCH;
+  T* Ks = reinterpret_cast<T*>(lds);
+  T* Vs = Ks + a.hw * head_stride;
+  int* klist = reinterpret_cast<int*>(Vs + a.hw * head_stride + 16);
+  int* qlist = klist + a.nkp;
+  int* counts = qlist + a.nqp;
+  const float* mq = a.mq ? a.mq + (int64_t)b * sh.Nq : nullptr;
+  const float* mk = a.mk ? a.mk + (int64_t)b * sh.Nk : nullptr;
+  if (wave == 0) {
+    const int c = keep_list(mk, sh.Nk, klist);
+    if (lane == 0) counts[0] = c;
+  }
+  if (wave == NW - 1) {
+    const int c = keep_list(mq, sh.Nq, qlist);
+    if (lane == 0) counts[1] = c;
+  }
+  const int heads = a.hw * sh.g, h0 = hk0 * sh.g;
+  if (mq && part == 0) {                          // masked queries: zero rows over all heads of the workgroup, no log-sum
+    zero_masked_rows<64 * NW, VEC>((T*)a.o + (int64_t)b * sh.Nq * a.out_ld + (int64_t)h0 * sh.D, a.out_ld, mq, 0, sh.Nq, 1, heads * sh.D);
+    if (a.lse)
+      for (int i = threadIdx.x; i < heads * sh.Nq; i += 64 * NW) {
+        const int hd = i / sh.Nq, n = i - hd * sh.Nq;
+        if (mq[n] == 0.0f) a.lse[((int64_t)b * sh.nh + h0 + hd) * sh.Nq + n] = -INFINITY;
+      }
+  }
+  __syncthreads();
+  const int nk = counts[0], nq = counts[1];
+  const int64_t krow = (int64_t)b * sh.Nk;
+  fill<T, DP, VEC>(Ks, head_stride, a.hw, (const T*)a.k + krow * a.k_ld + (int64_t)hk0 * sh.D, a.k_ld, klist, nk, sh.D);
+  fill<T, DP, VEC>(Vs, head_stride, a.hw, (const T*)a.v + krow * a.v_ld + (int64_t)hk0 * sh.D, a.v_ld, klist, nk, sh.D);
+  const float c = a.scale * kLog2e;
+  const int qt = (nq + 31) >> 5, items = heads * qt, step = NW * a.parts;
+  const T* qb = (const T*)a.q + (int64_t)b * sh.Nq * a.q_ld + (int64_t)h0 * sh.D;
+  u32x4 nf[S];                                    // the next item's query rows
+  auto fetch = [&](int it) {
+    const int hd = it / qt, r = (it - hd * qt) * 32 + col;
+    const bool ok = it < items && r < nq;
+    load_row<T, DP, VEC>(nf, ok ? qb + (int64_t)qlist[r] * a.q_ld + (int64_t)hd * sh.D : nullptr, sh.D, ok);
+  };
+  int it = part * NW + wave;
+  if (qt) fetch(it);
+  __syncthreads();
+  for (; it < items; it += step) {
+    const int hd = it / qt, r = (it - hd * qt) * 32 + col;
+    u32x4 qf[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) qf[s] = nf[s];
+    fetch(it + step);
+    const T* kh = Ks + (hd / sh.g) * head_stride;
+    const T* vh = Vs + (hd / sh.g) * head_stride;
+    f32x16 acc[R::FT];
+#pragma unroll
+    for (int t = 0; t < R::FT; ++t) acc[t] = zero16();
+    float m = -INFINITY, l = 0.0f;
+    for (int kt = 0; kt < nk; kt += 32) attend<T, DP, 32>(kh + kt * R::PITCH, vh + kt * R::PITCH, nk - kt, qf, c, m, l, acc);
+    l += __shfl_xor(l, 32);
+    if (r < nq) {
+      const int n = qlist[r];
+      store_col<T, DP, VEC>((T*)a.o + ((int64_t)b * sh.Nq + n) * a.out_ld + (int64_t)(h0 + hd) * sh.D, acc, l == 0.0f ? 0.0f : 1.0f / l, sh.D);
+      if (a.lse && h == 0) a.lse[((int64_t)b * sh.nh + h0 + hd) * sh.Nq + n] = l == 0.0f ? -INFINITY : m * a.scale + logf(l);
+    }
+  }
+}
+
+template <typename T, int DP, int NW, bool VEC>
+__global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(ResArgs a) {
+  using R = ResTile<T, DP>;
+  constexpr int S = DP / (2 * R::E), E = R::E;
+  constexpr bool HALF = __is_same(T, _Float16);
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const Shape& sh = a.sh;
+  int b, item;
+  if (!a.map.decode(blockIdx.x, b, item)) return;
+  const int hk0 = item * a.hw, heads = a.hw * sh.g, h0 = hk0 * sh.g;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
+  const int ks = a.nkp * R::PITCH, qs = a.nqp * R::PITCH, big = max(a.hw * ks, heads * qs);
+  T* A0 = reinterpret_cast<T*>(lds);              // K, then q
+  T* A1 = A0 + big;                               // V, then dout
+  float* sl = reinterpret_cast<float*>(A1 + big + 16);                      // [head][nqp] log-sums, then deltas
+  float* sd = sl + heads * a.nqp;
+  int* klist = reinterpret_cast<int*>(sd + heads * a.nqp);
+  int* qlist = klist + a.nkp;
+  int* counts = qlist + a.nqp;
+  const float* mq = a.mq ? a.mq + (int64_t)b * sh.Nq : nullptr;
+  const float* mk = a.mk ? a.mk + (int64_t)b * sh.Nk : nullptr;
+  if (wave == 0) {
+    const int c = keep_list(mk, sh.Nk, klist);
+    if (lane == 0) counts[0] = c;
+  }
+  if (wave == NW - 1) {
+    const int c = keep_list(mq, sh.Nq, qlist);
+    if (lane == 0) counts[1] = c;
+  }
+  const int64_t krow = (int64_t)b * sh.Nk, qrow = (int64_t)b * sh.Nq;
+  if (mq) zero_masked_rows<64 * NW, VEC>((T*)a.dq + qrow * a.dq_ld + (int64_t)h0 * sh.D, a.dq_ld, mq, 0, sh.Nq, 1, heads * sh.D);
+  if (mk) {
+    zero_masked_rows<64 * NW, VEC>((T*)a.dk + krow * a.dk_ld + (int64_t)hk0 * sh.D, a.dk_ld, mk, 0, sh.Nk, 1, a.hw * sh.D);
+    zero_masked_rows<64 * NW, VEC>((T*)a.dv + krow * a.dv_ld + (int64_t)hk0 * sh.D, a.dv_ld, mk, 0, sh.Nk, 1, a.hw * sh.D);
+  }
+  __syncthreads();
+  const int nk = counts[0], nq = counts[1];
+  const float c = a.scale * kLog2e;
+  const T* qb = (const T*)a.q + qrow * a.q_ld + (int64_t)h0 * sh.D;
+  const T* gb = (const T*)a.dout + qrow * a.dout_ld + (int64_t)h0 * sh.D;
+  const T* ob = (const T*)a.out + qrow * a.out_ld + (int64_t)h0 * sh.D;
+  const T* kb = (const T*)a.k + krow * a.k_ld + (int64_t)hk0 * sh.D;
+  const T* vb = (const T*)a.v + krow * a.v_ld + (int64_t)hk0 * sh.D;
+
+  // ---- dq: keys resident
+  fill<T, DP, VEC>(A0, ks, a.hw, kb, a.k_ld, klist, nk, sh.D);
+  fill<T, DP, VEC>(A1, ks, a.hw, vb, a.v_ld, klist, nk, sh.D);
+  const int qt = (nq + 31) >> 5, kt = (nk + 31) >> 5;
+  u32x4 nqf[S], ngf[S], nof[S];
+  float nl = INFINITY;
+  auto fetch_q = [&](int it) {
+    const int hd = it / qt, r = (it - hd * qt) * 32 + col;
+    const bool ok = it < heads * qt && r < nq;
+    const int64_t n = ok ? qlist[r] : 0;
+    load_row<T, DP, VEC>(nqf, qb + n * a.q_ld + (int64_t)hd * sh.D, sh.D, ok);
+    load_row<T, DP, VEC>(ngf, gb + n * a.dout_ld + (int64_t)hd * sh.D, sh.D, ok);
+    load_row<T, DP, VEC>(nof, ob + n * a.out_ld + (int64_t)hd * sh.D, sh.D, ok);
+    nl = ok ? row_stat<T>(a.lse[((int64_t)b * sh.nh + h0 + hd) * sh.Nq + n]) : INFINITY;
+  };
+  if (qt) fetch_q(wave);
+  __syncthreads();
+  for (int it = wave; it < heads * qt; it += NW) {
+    const int hd = it / qt, r0 = (it - hd * qt) * 32;
+    u32x4 qf[S], gf[S];
+    float delta = 0.0f;
+    const float lse = nl;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      qf[s] = nqf[s];
+      gf[s] = ngf[s];
+      T x[E], y[E];
+      __builtin_memcpy(x, &nof[s], 16);
+      __builtin_memcpy(y, &gf[s], 16);
+#pragma unroll
+      for (int i = 0; i < E; ++i) delta = fmaf((float)x[i], (float)y[i], delta);
+    }
+    delta += __shfl_xor(delta, 32);
+    fetch_q(it + NW);
+    const T* kh = A0 + (hd / sh.g) * ks;
+    const T* vh = A1 + (hd / sh.g) * ks;
+    f32x16 acc[R::FT];
+#pragma unroll
+    for (int t = 0; t < R::FT; ++t) acc[t] = zero16();
+    if (nk <= 32) {                               // the whole row at once: delta from p and dp (as few_keys elsewhere)
+      f32x16 s = dot_rows<T, DP>(kh, 0, qf, zero16());
+      const f32x16 dp = dot_rows<T, DP>(vh, 0, gf, zero16());
+      float sum = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[r] = crow(r, h) < nk ? prob<T>(s[r], a.scale, c, lse) : 0.0f;
+        sum += s[r];
+      }
+      sum += __shfl_xor(sum, 32);
+      delta = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) delta = fmaf(sum == 0.0f ? 0.0f : s[r] / sum, dp[r], delta);
+      delta += __shfl_xor(delta, 32);
+    }
+    if (h == 0) {
+      sl[hd * a.nqp + r0 + col] = HALF ? lse - kHalfLog : lse;
+      sd[hd * a.nqp + r0 + col] = lse == INFINITY ? 0.0f : delta;
+    }
+    ColScale cs;
+    float st = HALF ? lse - log2_pow2(cs.sc) : lse;
+    for (int kt0 = 0; kt0 < nk; kt0 += 32) {
+      f32x16 s = dot_rows<T, DP>(kh, kt0, qf, zero16());
+      const f32x16 dp = dot_rows<T, DP>(vh, kt0, gf, zero16());
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = prob<T>(s[r], a.scale, c, st) * (dp[r] - delta);
+      if (kt0 + 32 > nk) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (kt0 + crow(r, h) >= nk) s[r] = 0.0f;
+      }
+      if constexpr (HALF) {
+        const float before = cs.sc;
+        cs.fit(s, acc, R::FT);
+        if (__any(cs.sc != before)) st = lse - log2_pow2(cs.sc);
+      }
+      dot_cols<T, DP>(kh, kt0, s, acc);
+    }
+    if (r0 + col < nq)
+      store_col<T, DP, VEC>((T*)a.dq + (qrow + qlist[r0 + col]) * a.dq_ld + (int64_t)(h0 + hd) * sh.D, acc, HALF ? a.scale / cs.sc : a.scale, sh.D);
+  }
+  // ---- dk, dv: queries resident
+  u32x4 kf[S], vf[S];
+  auto fetch_k = [&](int it) {
+    const int hd = it / kt, r = (it - hd * kt) * 32 + col;
+    const bool ok = it < a.hw * kt && r < nk;
+    const int64_t n = ok ? klist[r] : 0;
+    load_row<T, DP, VEC>(kf, kb + n * a.k_ld + (int64_t)hd * sh.D, sh.D, ok);
+    load_row<T, DP, VEC>(vf, vb + n * a.v_ld + (int64_t)hd * sh.D, sh.D, ok);
+  };
+  if (kt) fetch_k(wave);
+  __syncthreads();                                // K and V have been read
+  fill<T, DP, VEC>(A0, qs, heads, qb, a.q_ld, qlist, nq, sh.D);
+  fill<T, DP, VEC>(A1, qs, heads, gb, a.dout_ld, qlist, nq, sh.D);
+  __syncthreads();
+  for (int it = wave; it < a.hw * kt; it += NW) {
+    const int hd = it / kt, r = (it - hd * kt) * 32 + col;
+    if (it != wave) fetch_k(it);
+    f32x16 dk[R::FT], dv[R::FT];
+#pragma unroll
+    for (int t = 0; t < R::FT; ++t) {
+      dk[t] = zero16();
+      dv[t] = zero16();
+    }
+    ColScale cs;
+    for (int gi = 0; gi < sh.g; ++gi) {
+      const T* qh = A0 + (hd * sh.g + gi) * qs;
+      const T* gh = A1 + (hd * sh.g + gi) * qs;
+      const float* lh = sl + (hd * sh.g + gi) * a.nqp;
+      const float* dh = sd + (hd * sh.g + gi) * a.nqp;
+      for (int q0 = 0; q0 < nq; q0 += 32) {
+        f32x16 s = dot_rows<T, DP>(qh, q0, kf, zero16());
+        f32x16 dp = dot_rows<T, DP>(gh, q0, vf, zero16());
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4) {
+          const f32x4 ls = *reinterpret_cast<const f32x4*>(lh + q0 + 8 * g4 + 4 * h);
+          const f32x4 dl = *reinterpret_cast<const f32x4*>(dh + q0 + 8 * g4 + 4 * h);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r2 = 4 * g4 + i;
+            s[r2] = prob<T>(s[r2], a.scale, c, ls[i]);      // (rows past the end: log-sum +inf, p = 0)
+            dp[r2] = s[r2] * (dp[r2] - dl[i]);
+          }
+        }
+        if constexpr (HALF) {
+#pragma unroll
+          for (int r2 = 0; r2 < 16; ++r2) dp[r2] *= cs.sc;
+          cs.fit(dp, dk, R::FT);
+        }
+        dot_cols<T, DP>(gh, q0, s, dv);
+        dot_cols<T, DP>(qh, q0, dp, dk);
+      }
+    }
+    if (r < nk) {
+      const int64_t n = krow + klist[r];
+      store_col<T, DP, VEC>((T*)a.dk + n * a.dk_ld + (int64_t)(hk0 + hd) * sh.D, dk, HALF ? a.scale / kHalfP / cs.sc : a.scale, sh.D);
+      store_col<T, DP, VEC>((T*)a.dv + n * a.dv_ld + (int64_t)(hk0 + hd) * sh.D, dv, HALF ? 1.0f / kHalfP : 1.0f, sh.D);
+    }
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------
+constexpr int kResBudget = 80 * 1024;             // two workgroups on a CU
+constexpr int kResWaves = 4;
+
+static int res_width(int D, int dtype) { return dtype == MMB_DT_F32 && D <= 16 ? 16 : pad_width(D); }
+static int64_t res_bytes(const Shape& s, int dtype, int hw, bool bwd) {
+  const int es = dtype == MMB_DT_F32 ? 4 : 2, dp = res_width(s.D, dtype), pitch = es == 2 ? dp : dp + 4;
+  const int64_t nkp = (s.Nk + 31) / 32 * 32, nqp = (s.Nq + 31) / 32 * 32;
+  int64_t rows = hw * nkp;
+  if (bwd && (int64_t)hw * s.g * nqp > rows) rows = (int64_t)hw * s.g * nqp;
+  return 2 * rows * pitch * es + 16 * es + (bwd ? 2 * (int64_t)hw * s.g * nqp * 4 : 0) + (nkp + nqp + 4) * 4;
+}
+// Key heads of a workgroup (0: the cloud is not small).  As many as two workgroups on a CU leave room for, of those that
+// divide the heads; at least as many clouds as half the CUs, below which the streaming kernels spread one cloud better; a
+// query tile that is at least half full.
+int resident_heads(const Shape& s, int dtype, bool bwd) {
+  if (s.Nk > 1024 || s.Nq > 1024 || s.Nq < 16 || (int64_t)s.B * s.nkv < 256) return 0;
+  int best = 0;
+  for (int hw = 1; hw <= s.nkv && hw <= 8; ++hw)
+    if (s.nkv % hw == 0 && res_bytes(s, dtype, hw, bwd) <= kResBudget && (hw == 1 || (int64_t)s.B * (s.nkv / hw) >= 512)) best = hw;
+  return best;
+}
+
+template <bool BWD, typename T, int DP, bool VEC>
+static int launch_res(ResArgs& a, int64_t bytes, hipStream_t st) {
+  constexpr int NW = kResWaves;
+  void (*kern)(ResArgs);
+  if constexpr (BWD) kern = res_bwd_kernel<T, DP, NW, VEC>;
+  else kern = res_fwd_kernel<T, DP, NW, VEC>;
+  static PerDeviceOnce once;
+  if (!once.run([&] { return hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, kResBudget) == hipSuccess; })) {
+    set_error("mmb_cross_attention: the runtime refuses %d bytes of LDS", kResBudget);
+    return MMB_ERR_LAUNCH;
+  }
+  kern<<<dim3((unsigned)a.map.blocks()), dim3(64 * NW), (size_t)bytes, st>>>(a);
+  return check_launch(BWD ? "mmb_cross_attention_bwd (resident)" : "mmb_cross_attention_fwd (resident)");
+}
+template <bool BWD, typename T, bool VEC>
+static int pick_res(ResArgs& a, int dtype, int64_t bytes, hipStream_t st) {
+  switch (res_width(a.sh.D, dtype)) {
+    case 16:
+      if constexpr (sizeof(T) == 4) return launch_res<BWD, T, 16, VEC>(a, bytes, st);
+    case 32: return launch_res<BWD, T, 32, VEC>(a, bytes, st);
+    case 64: return launch_res<BWD, T, 64, VEC>(a, bytes, st);
+    default: return launch_res<BWD, T, 128, VEC>(a, bytes, st);
+  }
+}
+template <bool BWD>
+static int run_res(ResArgs& a, int dtype, bool vec, hipStream_t st) {
+  const Shape& s = a.sh;
+  a.nkp = (s.Nk + 31) / 32 * 32;
+  a.nqp = (s.Nq + 31) / 32 * 32;
+  const int groups = s.nkv / a.hw;
+  // forward: a cloud's query tiles over several workgroups while the chip is not full
+  a.parts = 1;
+  if (!BWD)
+    while ((int64_t)s.B * groups * a.parts < 1024 && a.parts * kResWaves < a.hw * s.g * (a.nqp / 32)) a.parts *= 2;
+  a.map = {s.B, groups * a.parts, s.B % 8 == 0 || s.B >= 64 ? 1 : 0};
+  MMB_REQUIRE(a.map.blocks() <= 0x7fffffffLL, "mmb_cross_attention: %lld workgroups", (long long)a.map.blocks());
+  const int64_t bytes = res_bytes(s, dtype, a.hw, BWD);
+  if (dtype == MMB_DT_F32) return vec ? pick_res<BWD, float, true>(a, dtype, bytes, st) : pick_res<BWD, float, false>(a, dtype, bytes, st);
+  if (dtype == MMB_DT_BF16) return vec ? pick_res<BWD, __bf16, true>(a, dtype, bytes, st) : pick_res<BWD, __bf16, false>(a, dtype, bytes, st);
+  return vec ? pick_res<BWD, _Float16, true>(a, dtype, bytes, st) : pick_res<BWD, _Float16, false>(a, dtype, bytes, st);
+}
+
+int resident_fwd(const Shape& s, int hw, int dtype, bool vec, const void* q, int64_t q_ld, const void* k, int64_t k_ld, const void* v,
+                 int64_t v_ld, const float* mq, const float* mk, float scale, void* out, int64_t out_ld, float* lse, hipStream_t st) {
+  ResArgs a = {};
+  a.sh = s; a.hw = hw; a.q = q; a.q_ld = q_ld; a.k = k; a.k_ld = k_ld; a.v = v; a.v_ld = v_ld; a.mq = mq; a.mk = mk; a.scale = scale;
+  a.o = out; a.out_ld = out_ld; a.lse = lse;
+  return run_res<false>(a, dtype, vec, st);
+}
+int resident_bwd(const Shape& s, int hw, int dtype, bool vec, const void* q, int64_t q_ld, const void* k, int64_t k_ld, const void* v,
+                 int64_t v_ld, const float* mq, const float* mk, float scale, const void* out, int64_t out_ld, const void* dout,
+                 int64_t dout_ld, const float* lse, void* dq, int64_t dq_ld, void* dk, int64_t dk_ld, void* dv, int64_t dv_ld, hipStream_t st) {
+  ResArgs a = {};
+  a.sh = s; a.hw = hw; a.q = q; a.q_ld = q_ld; a.k = k; a.k_ld = k_ld; a.v = v; a.v_ld = v_ld; a.mq = mq; a.mk = mk; a.scale = scale;
+  a.out = out; a.out_ld = out_ld; a.dout = dout; a.dout_ld = dout_ld; a.lse = const_cast<float*>(lse);
+  a.dq = dq; a.dq_ld = dq_ld; a.dk = dk; a.dk_ld = dk_ld; a.dv = dv; a.dv_ld = dv_ld;
+  return run_res<true>(a, dtype, vec, st);
+}
+
+}  // namespace xattn
+}  // namespace mmb

@@ -127,6 +127,13 @@ SHAPES = [  # B, Nq, Nk, nh, nkv, D, masked
     (8, 100, 96, 2, 1, 33, True),                               # odd head width: scalar loads
     (2, 130, 70, 3, 3, 1, False),
     (4, 5, 600, 4, 4, 8, True),
+    (64, 150, 128, 4, 4, 16, True),                             # many small clouds: their keys stay in LDS
+    (70, 40, 50, 8, 4, 32, True),
+    (128, 16, 20, 4, 2, 64, True),
+    (300, 33, 150, 2, 1, 12, True),
+    (256, 20, 40, 1, 1, 128, False),
+    (66, 17, 200, 4, 4, 21, True),
+    (500, 18, 1, 2, 2, 8, False),
 ]
 
 
