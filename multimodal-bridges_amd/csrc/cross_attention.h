@@ -338,14 +338,10 @@ __device__ __forceinline__ void store_col(T* __restrict__ p, const f32x16* acc, 
     }
 }
 
-// One tile of n keys (K rows and V in LDS): scores, running softmax, o += V^T P.
+// Running softmax over one tile of n keys: raw scores in s become p; m, l and what acc has summed follow the maximum.
 template <typename T, int DP, int TK>
-__device__ __forceinline__ void attend(const T* Ks, const T* Vs, int n, const u32x4* qf, float c,
-                                       float& m, float& l, f32x16* acc) {
+__device__ __forceinline__ void softmax_step(f32x16* s, int n, float c, float& m, float& l, f32x16* acc) {
   const int h = (threadIdx.x & 63) >> 5;
-  f32x16 s[TK / 32];
-#pragma unroll
-  for (int st = 0; st < TK / 32; ++st) s[st] = dot_rows<T, DP>(Ks, 32 * st, qf, zero16());
   if (n < TK) {
 #pragma unroll
     for (int st = 0; st < TK / 32; ++st)
@@ -379,6 +375,15 @@ __device__ __forceinline__ void attend(const T* Ks, const T* Vs, int n, const u3
       s[st][r] = __builtin_amdgcn_exp2f(sizeof(T) == 2 ? fmaf(s[st][r], c, -ms * c) : (s[st][r] - ms) * c);
       l += s[st][r];
     }
+}
+
+// One tile of n keys (K rows and V in LDS): scores, running softmax, o += V^T P.
+template <typename T, int DP, int TK>
+__device__ __forceinline__ void attend(const T* Ks, const T* Vs, int n, const u32x4* qf, float c, float& m, float& l, f32x16* acc) {
+  f32x16 s[TK / 32];
+#pragma unroll
+  for (int st = 0; st < TK / 32; ++st) s[st] = dot_rows<T, DP>(Ks, 32 * st, qf, zero16());
+  softmax_step<T, DP, TK>(s, n, c, m, l, acc);
   // p is rounded to the inputs' type for the product (16-bit types: half a step of a value in [0, 1], the size of the
   // output's own rounding; l sums the unrounded values), the sums over keys stay in 32 bits
 #pragma unroll
@@ -460,15 +465,26 @@ struct RowTile {
   }
 };
 
+// kept slots of a mask (or all), one wave; returns their number
+__device__ __forceinline__ int keep_list(const float* __restrict__ maskf, int N, int* list) {
+  if (maskf == nullptr) {
+    for (int i = threadIdx.x & 63; i < N; i += 64) list[i] = i;
+    return N;
+  }
+  int c = 0;
+  for (int lo = 0; lo < N; lo += kChunk) c += compact_chunk(maskf, lo, N, list + c);
+  return c;
+}
+
 struct Shape {
   int B, Nq, Nk, nh, nkv, D, g;                   // g = nh / nkv query heads share one key head
 };
 
-// small clouds (cross_attention_resident.hip); resident_heads: key heads of a workgroup, 0 where the streaming kernels serve
-int resident_heads(const Shape& s, int dtype, bool bwd);
-int resident_fwd(const Shape& s, int hw, int dtype, bool vec, const void* q, int64_t q_ld, const void* k, int64_t k_ld, const void* v,
+// small clouds (cross_attention_resident.hip)
+bool resident_fits(const Shape& s, int dtype, bool bwd);
+int resident_fwd(const Shape& s, int dtype, bool vec, const void* q, int64_t q_ld, const void* k, int64_t k_ld, const void* v,
                  int64_t v_ld, const float* mq, const float* mk, float scale, void* out, int64_t out_ld, float* lse, hipStream_t st);
-int resident_bwd(const Shape& s, int hw, int dtype, bool vec, const void* q, int64_t q_ld, const void* k, int64_t k_ld, const void* v,
+int resident_bwd(const Shape& s, int dtype, bool vec, const void* q, int64_t q_ld, const void* k, int64_t k_ld, const void* v,
                  int64_t v_ld, const float* mq, const float* mk, float scale, const void* out, int64_t out_ld, const void* dout,
                  int64_t dout_ld, const float* lse, void* dq, int64_t dq_ld, void* dk, int64_t dk_ld, void* dv, int64_t dv_ld, hipStream_t st);
 

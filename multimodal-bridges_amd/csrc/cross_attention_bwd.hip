@@ -369,8 +369,8 @@ extern "C" int mmb_cross_attention_bwd(int B, int Nq, int Nk, int nheads, int nh
                    chunk_aligned(out, out_ld, es) && chunk_aligned(dout, dout_ld, es) && chunk_aligned(dq, dq_ld, es) &&
                    chunk_aligned(dk, dk_ld, es) && chunk_aligned(dv, dv_ld, es);
   hipStream_t st = as_stream(stream);
-  if (const int hw = resident_heads(a.sh, dtype, true))
-    return resident_bwd(a.sh, hw, dtype, vec, q, q_ld, k, k_ld, v, v_ld, maskf_q, maskf_k, scale, out, out_ld, dout, dout_ld, lse, dq,
+  if (resident_fits(a.sh, dtype, true))
+    return resident_bwd(a.sh, dtype, vec, q, q_ld, k, k_ld, v, v_ld, maskf_q, maskf_k, scale, out, out_ld, dout, dout_ld, lse, dq,
                         dq_ld, dk, dk_ld, dv, dv_ld, st);
   if (dtype == MMB_DT_F32) return vec ? pick_dp<float, true>(a, st) : pick_dp<float, false>(a, st);
   if (dtype == MMB_DT_BF16) return vec ? pick_dp<__bf16, true>(a, st) : pick_dp<__bf16, false>(a, st);

@@ -1,10 +1,12 @@
 // Cross attention of small clouds (jets): the keys of a head fit into LDS whole.
 //
 // With some hundred slots a cloud is a few 32 x 32 tiles a head, and what a call costs is not its products but the chain
-// mask -> kept slots -> rows -> products of every workgroup.  Here a workgroup owns one cloud and as many of its heads as LDS
-// holds: the masks are read and compacted once for all of them, the rows of these heads are read side by side (whole cache
-// lines), and after ONE barrier every wave walks its own (head, 32 rows) items without meeting the others.  The reverse does
-// this twice, with K and V resident for dq and with q and dout resident for dk and dv; delta stays in LDS between the two.
+// mask -> kept slots -> rows -> products of every workgroup.  Here a workgroup owns one key head of one cloud: the masks are
+// read and compacted once, and after ONE barrier every wave walks its own (query head, 32 rows) items without meeting the
+// others.  The reverse does this twice, with K and V resident for dq and with q and dout resident for dk and dv; delta stays in
+// LDS between the two.  What counts is how many workgroups a CU holds at once (their chains hide each other): two or four
+// heads a workgroup, which would share the masks and read longer row segments, need as much more LDS and measured 1.04 to
+// 1.4 times the time; eight waves instead of four 1.1 to 1.3 times.
 #include "cross_attention.h"
 
 namespace mmb {
@@ -24,33 +26,35 @@ struct ResArgs {
   float* lse;
   float scale;
   void *o, *dq, *dk, *dv;
-  int hw, parts;                                  // key heads of a workgroup; workgroups that share a cloud's query tiles (forward)
+  int parts;                                      // workgroups that share a head's query tiles (forward)
   int nkp, nqp;                                   // slots padded to 32
-  GridMap map;                                    // units = clouds, items = head groups * parts
+  GridMap map;                                    // units = clouds, items = key heads * parts
 };
 
-// kept slots of a mask (or all), one wave; returns their number
-__device__ __forceinline__ int keep_list(const float* __restrict__ maskf, int N, int* list) {
-  if (maskf == nullptr) {
-    for (int i = threadIdx.x & 63; i < N; i += 64) list[i] = i;
-    return N;
-  }
-  int c = 0;
-  for (int lo = 0; lo < N; lo += kChunk) c += compact_chunk(maskf, lo, N, list + c);
-  return c;
-}
-
-// rows of `heads` neighbouring heads into LDS: [head][rows, padded to 32 with zeros][DP]
-template <typename T, int DP, bool VEC>
-__device__ __forceinline__ void fill(T* __restrict__ dst, int head_stride, int heads, const T* __restrict__ src, int64_t ld, const int* list, int n, int D) {
+// rows of one head of two matrices into LDS, padded to 32 with zeros; four chunks of each are in flight a thread
+template <typename T, int DP, int NT, bool VEC>
+__device__ __forceinline__ void fill2(T* __restrict__ d0, T* __restrict__ d1, const T* __restrict__ s0, int64_t ld0, const T* __restrict__ s1,
+                                      int64_t ld1, const int* list, int n, int D) {
   using R = ResTile<T, DP>;
-  const int n32 = (n + 31) & ~31, per = heads * R::CH, work = n32 * per;
-#pragma unroll 4
-  for (int it = threadIdx.x; it < work; it += blockDim.x) {
-    const int row = it / per, x = it - row * per, hd = x / R::CH, ch = x % R::CH;
-    const bool ok = row < n;
-    const u32x4 c = load_chunk<T, VEC>(ok ? src + (int64_t)list[row] * ld + (int64_t)hd * D : nullptr, ch * R::E, D, ok);
-    *reinterpret_cast<u32x4*>(dst + hd * head_stride + chunk_at<T, DP>(row, ch)) = c;
+  const int work = ((n + 31) & ~31) * R::CH;
+  for (int it0 = threadIdx.x; it0 < work; it0 += 4 * NT) {
+    u32x4 c0[4], c1[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int it = it0 + j * NT, row = it / R::CH, ch = it % R::CH;
+      const bool ok = row < n;
+      const int64_t slot = ok ? list[row] : 0;
+      c0[j] = load_chunk<T, VEC>(s0 + slot * ld0, ch * R::E, D, ok);
+      c1[j] = load_chunk<T, VEC>(s1 + slot * ld1, ch * R::E, D, ok);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int it = it0 + j * NT;
+      if (it < work) {
+        *reinterpret_cast<u32x4*>(d0 + chunk_at<T, DP>(it / R::CH, it % R::CH)) = c0[j];
+        *reinterpret_cast<u32x4*>(d1 + chunk_at<T, DP>(it / R::CH, it % R::CH)) = c1[j];
+      }
+    }
   }
 }
 
@@ -62,12 +66,11 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 2 : 3) res_fwd_kernel(Res
   const Shape& sh = a.sh;
   int b, item;
   if (!a.map.decode(blockIdx.x, b, item)) return;
-  const int hk0 = item / a.parts * a.hw, part = item % a.parts;
+  const int hk = item / a.parts, part = item - hk * a.parts;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
-  const int head_stride = a.nkp * R::PITCH;
   T* Ks = reinterpret_cast<T*>(lds);
-  T* Vs = Ks + a.hw * head_stride;
-  int* klist = reinterpret_cast<int*>(Vs + a.hw * head_stride + 16);
+  T* Vs = Ks + a.nkp * R::PITCH;
+  int* klist = reinterpret_cast<int*>(Vs + a.nkp * R::PITCH + 16);
   int* qlist = klist + a.nkp;
   int* counts = qlist + a.nqp;
   const float* mq = a.mq ? a.mq + (int64_t)b * sh.Nq : nullptr;
@@ -80,7 +83,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 2 : 3) res_fwd_kernel(Res
     const int c = keep_list(mq, sh.Nq, qlist);
     if (lane == 0) counts[1] = c;
   }
-  const int heads = a.hw * sh.g, h0 = hk0 * sh.g;
+  const int heads = sh.g, h0 = hk * sh.g;
   if (mq && part == 0) {                          // masked queries: zero rows over all heads of the workgroup, no log-sum
     zero_masked_rows<64 * NW, VEC>((T*)a.o + (int64_t)b * sh.Nq * a.out_ld + (int64_t)h0 * sh.D, a.out_ld, mq, 0, sh.Nq, 1, heads * sh.D);
     if (a.lse)
@@ -92,8 +95,6 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 2 : 3) res_fwd_kernel(Res
   __syncthreads();
   const int nk = counts[0], nq = counts[1];
   const int64_t krow = (int64_t)b * sh.Nk;
-  fill<T, DP, VEC>(Ks, head_stride, a.hw, (const T*)a.k + krow * a.k_ld + (int64_t)hk0 * sh.D, a.k_ld, klist, nk, sh.D);
-  fill<T, DP, VEC>(Vs, head_stride, a.hw, (const T*)a.v + krow * a.v_ld + (int64_t)hk0 * sh.D, a.v_ld, klist, nk, sh.D);
   const float c = a.scale * kLog2e;
   const int qt = (nq + 31) >> 5, items = heads * qt, step = NW * a.parts;
   const T* qb = (const T*)a.q + (int64_t)b * sh.Nq * a.q_ld + (int64_t)h0 * sh.D;
@@ -105,6 +106,8 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 2 : 3) res_fwd_kernel(Res
   };
   int it = part * NW + wave;
   if (qt) fetch(it);
+  fill2<T, DP, 64 * NW, VEC>(Ks, Vs, (const T*)a.k + krow * a.k_ld + (int64_t)hk * sh.D, a.k_ld,
+                             (const T*)a.v + krow * a.v_ld + (int64_t)hk * sh.D, a.v_ld, klist, nk, sh.D);
   __syncthreads();
   for (; it < items; it += step) {
     const int hd = it / qt, r = (it - hd * qt) * 32 + col;
@@ -112,13 +115,11 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 2 : 3) res_fwd_kernel(Res
 #pragma unroll
     for (int s = 0; s < S; ++s) qf[s] = nf[s];
     fetch(it + step);
-    const T* kh = Ks + (hd / sh.g) * head_stride;
-    const T* vh = Vs + (hd / sh.g) * head_stride;
     f32x16 acc[R::FT];
 #pragma unroll
     for (int t = 0; t < R::FT; ++t) acc[t] = zero16();
     float m = -INFINITY, l = 0.0f;
-    for (int kt = 0; kt < nk; kt += 32) attend<T, DP, 32>(kh + kt * R::PITCH, vh + kt * R::PITCH, nk - kt, qf, c, m, l, acc);
+    for (int kt = 0; kt < nk; kt += 32) attend<T, DP, 32>(Ks + kt * R::PITCH, Vs + kt * R::PITCH, nk - kt, qf, c, m, l, acc);
     l += __shfl_xor(l, 32);
     if (r < nq) {
       const int n = qlist[r];
@@ -137,9 +138,9 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(Res
   const Shape& sh = a.sh;
   int b, item;
   if (!a.map.decode(blockIdx.x, b, item)) return;
-  const int hk0 = item * a.hw, heads = a.hw * sh.g, h0 = hk0 * sh.g;
+  const int hk = item, heads = sh.g, h0 = hk * sh.g;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
-  const int ks = a.nkp * R::PITCH, qs = a.nqp * R::PITCH, big = max(a.hw * ks, heads * qs);
+  const int qs = a.nqp * R::PITCH, big = max(a.nkp * R::PITCH, heads * qs);
   T* A0 = reinterpret_cast<T*>(lds);              // K, then q
   T* A1 = A0 + big;                               // V, then dout
   float* sl = reinterpret_cast<float*>(A1 + big + 16);                      // [head][nqp] log-sums, then deltas
@@ -160,8 +161,8 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(Res
   const int64_t krow = (int64_t)b * sh.Nk, qrow = (int64_t)b * sh.Nq;
   if (mq) zero_masked_rows<64 * NW, VEC>((T*)a.dq + qrow * a.dq_ld + (int64_t)h0 * sh.D, a.dq_ld, mq, 0, sh.Nq, 1, heads * sh.D);
   if (mk) {
-    zero_masked_rows<64 * NW, VEC>((T*)a.dk + krow * a.dk_ld + (int64_t)hk0 * sh.D, a.dk_ld, mk, 0, sh.Nk, 1, a.hw * sh.D);
-    zero_masked_rows<64 * NW, VEC>((T*)a.dv + krow * a.dv_ld + (int64_t)hk0 * sh.D, a.dv_ld, mk, 0, sh.Nk, 1, a.hw * sh.D);
+    zero_masked_rows<64 * NW, VEC>((T*)a.dk + krow * a.dk_ld + (int64_t)hk * sh.D, a.dk_ld, mk, 0, sh.Nk, 1, sh.D);
+    zero_masked_rows<64 * NW, VEC>((T*)a.dv + krow * a.dv_ld + (int64_t)hk * sh.D, a.dv_ld, mk, 0, sh.Nk, 1, sh.D);
   }
   __syncthreads();
   const int nk = counts[0], nq = counts[1];
@@ -169,12 +170,10 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(Res
   const T* qb = (const T*)a.q + qrow * a.q_ld + (int64_t)h0 * sh.D;
   const T* gb = (const T*)a.dout + qrow * a.dout_ld + (int64_t)h0 * sh.D;
   const T* ob = (const T*)a.out + qrow * a.out_ld + (int64_t)h0 * sh.D;
-  const T* kb = (const T*)a.k + krow * a.k_ld + (int64_t)hk0 * sh.D;
-  const T* vb = (const T*)a.v + krow * a.v_ld + (int64_t)hk0 * sh.D;
+  const T* kb = (const T*)a.k + krow * a.k_ld + (int64_t)hk * sh.D;
+  const T* vb = (const T*)a.v + krow * a.v_ld + (int64_t)hk * sh.D;
 
   // ---- dq: keys resident
-  fill<T, DP, VEC>(A0, ks, a.hw, kb, a.k_ld, klist, nk, sh.D);
-  fill<T, DP, VEC>(A1, ks, a.hw, vb, a.v_ld, klist, nk, sh.D);
   const int qt = (nq + 31) >> 5, kt = (nk + 31) >> 5;
   u32x4 nqf[S], ngf[S], nof[S];
   float nl = INFINITY;
@@ -188,6 +187,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(Res
     nl = ok ? row_stat<T>(a.lse[((int64_t)b * sh.nh + h0 + hd) * sh.Nq + n]) : INFINITY;
   };
   if (qt) fetch_q(wave);
+  fill2<T, DP, 64 * NW, VEC>(A0, A1, kb, a.k_ld, vb, a.v_ld, klist, nk, sh.D);
   __syncthreads();
   for (int it = wave; it < heads * qt; it += NW) {
     const int hd = it / qt, r0 = (it - hd * qt) * 32;
@@ -206,8 +206,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(Res
     }
     delta += __shfl_xor(delta, 32);
     fetch_q(it + NW);
-    const T* kh = A0 + (hd / sh.g) * ks;
-    const T* vh = A1 + (hd / sh.g) * ks;
+    const T *kh = A0, *vh = A1;
     f32x16 acc[R::FT];
 #pragma unroll
     for (int t = 0; t < R::FT; ++t) acc[t] = zero16();
@@ -255,19 +254,19 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(Res
   // ---- dk, dv: queries resident
   u32x4 kf[S], vf[S];
   auto fetch_k = [&](int it) {
-    const int hd = it / kt, r = (it - hd * kt) * 32 + col;
-    const bool ok = it < a.hw * kt && r < nk;
+    const int r = it * 32 + col;
+    const bool ok = r < nk;
     const int64_t n = ok ? klist[r] : 0;
-    load_row<T, DP, VEC>(kf, kb + n * a.k_ld + (int64_t)hd * sh.D, sh.D, ok);
-    load_row<T, DP, VEC>(vf, vb + n * a.v_ld + (int64_t)hd * sh.D, sh.D, ok);
+    load_row<T, DP, VEC>(kf, kb + n * a.k_ld, sh.D, ok);
+    load_row<T, DP, VEC>(vf, vb + n * a.v_ld, sh.D, ok);
   };
-  if (kt) fetch_k(wave);
+  fetch_k(wave);
   __syncthreads();                                // K and V have been read
-  fill<T, DP, VEC>(A0, qs, heads, qb, a.q_ld, qlist, nq, sh.D);
-  fill<T, DP, VEC>(A1, qs, heads, gb, a.dout_ld, qlist, nq, sh.D);
+  for (int gi = 0; gi < heads; ++gi)
+    fill2<T, DP, 64 * NW, VEC>(A0 + gi * qs, A1 + gi * qs, qb + (int64_t)gi * sh.D, a.q_ld, gb + (int64_t)gi * sh.D, a.dout_ld, qlist, nq, sh.D);
   __syncthreads();
-  for (int it = wave; it < a.hw * kt; it += NW) {
-    const int hd = it / kt, r = (it - hd * kt) * 32 + col;
+  for (int it = wave; it < kt; it += NW) {
+    const int r = it * 32 + col;
     if (it != wave) fetch_k(it);
     f32x16 dk[R::FT], dv[R::FT];
 #pragma unroll
@@ -277,10 +276,10 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(Res
     }
     ColScale cs;
     for (int gi = 0; gi < sh.g; ++gi) {
-      const T* qh = A0 + (hd * sh.g + gi) * qs;
-      const T* gh = A1 + (hd * sh.g + gi) * qs;
-      const float* lh = sl + (hd * sh.g + gi) * a.nqp;
-      const float* dh = sd + (hd * sh.g + gi) * a.nqp;
+      const T* qh = A0 + gi * qs;
+      const T* gh = A1 + gi * qs;
+      const float* lh = sl + gi * a.nqp;
+      const float* dh = sd + gi * a.nqp;
       for (int q0 = 0; q0 < nq; q0 += 32) {
         f32x16 s = dot_rows<T, DP>(qh, q0, kf, zero16());
         f32x16 dp = dot_rows<T, DP>(gh, q0, vf, zero16());
@@ -306,33 +305,29 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(Res
     }
     if (r < nk) {
       const int64_t n = krow + klist[r];
-      store_col<T, DP, VEC>((T*)a.dk + n * a.dk_ld + (int64_t)(hk0 + hd) * sh.D, dk, HALF ? a.scale / kHalfP / cs.sc : a.scale, sh.D);
-      store_col<T, DP, VEC>((T*)a.dv + n * a.dv_ld + (int64_t)(hk0 + hd) * sh.D, dv, HALF ? 1.0f / kHalfP : 1.0f, sh.D);
+      store_col<T, DP, VEC>((T*)a.dk + n * a.dk_ld + (int64_t)hk * sh.D, dk, HALF ? a.scale / kHalfP / cs.sc : a.scale, sh.D);
+      store_col<T, DP, VEC>((T*)a.dv + n * a.dv_ld + (int64_t)hk * sh.D, dv, HALF ? 1.0f / kHalfP : 1.0f, sh.D);
     }
   }
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------
-constexpr int kResBudget = 80 * 1024;             // two workgroups on a CU
+constexpr int kResBudget = 53 * 1024;             // three workgroups on a CU
 constexpr int kResWaves = 4;
 
 static int res_width(int D, int dtype) { return dtype == MMB_DT_F32 && D <= 16 ? 16 : pad_width(D); }
-static int64_t res_bytes(const Shape& s, int dtype, int hw, bool bwd) {
+static int64_t res_bytes(const Shape& s, int dtype, bool bwd) {
   const int es = dtype == MMB_DT_F32 ? 4 : 2, dp = res_width(s.D, dtype), pitch = es == 2 ? dp : dp + 4;
   const int64_t nkp = (s.Nk + 31) / 32 * 32, nqp = (s.Nq + 31) / 32 * 32;
-  int64_t rows = hw * nkp;
-  if (bwd && (int64_t)hw * s.g * nqp > rows) rows = (int64_t)hw * s.g * nqp;
-  return 2 * rows * pitch * es + 16 * es + (bwd ? 2 * (int64_t)hw * s.g * nqp * 4 : 0) + (nkp + nqp + 4) * 4;
+  int64_t rows = nkp;
+  if (bwd && s.g * nqp > rows) rows = s.g * nqp;
+  return 2 * rows * pitch * es + 16 * es + (bwd ? 2 * s.g * nqp * 4 : 0) + (nkp + nqp + 4) * 4;
 }
-// Key heads of a workgroup (0: the cloud is not small).  As many as two workgroups on a CU leave room for, of those that
-// divide the heads; at least as many clouds as half the CUs, below which the streaming kernels spread one cloud better; a
-// query tile that is at least half full.
-int resident_heads(const Shape& s, int dtype, bool bwd) {
-  if (s.Nk > 1024 || s.Nq > 1024 || s.Nq < 16 || (int64_t)s.B * s.nkv < 256) return 0;
-  int best = 0;
-  for (int hw = 1; hw <= s.nkv && hw <= 8; ++hw)
-    if (s.nkv % hw == 0 && res_bytes(s, dtype, hw, bwd) <= kResBudget && (hw == 1 || (int64_t)s.B * (s.nkv / hw) >= 512)) best = hw;
-  return best;
+// Whether a cloud is small: its workgroups leave room for two others on a CU (at 150 x 128 slots of 16 floats 243 us a training
+// step against 524 in the streaming kernels; at one workgroup a CU the two are level), there are clouds for every CU -- fewer
+// are spread better by the streaming kernels --, and a query tile is at least half full.
+bool resident_fits(const Shape& s, int dtype, bool bwd) {
+  return s.Nk <= 1024 && s.Nq <= 1024 && s.Nq >= 16 && (int64_t)s.B * s.nkv >= 256 && res_bytes(s, dtype, bwd) <= kResBudget;
 }
 
 template <bool BWD, typename T, int DP, bool VEC>
@@ -341,11 +336,6 @@ static int launch_res(ResArgs& a, int64_t bytes, hipStream_t st) {
   void (*kern)(ResArgs);
   if constexpr (BWD) kern = res_bwd_kernel<T, DP, NW, VEC>;
   else kern = res_fwd_kernel<T, DP, NW, VEC>;
-  static PerDeviceOnce once;
-  if (!once.run([&] { return hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, kResBudget) == hipSuccess; })) {
-    set_error("mmb_cross_attention: the runtime refuses %d bytes of LDS", kResBudget);
-    return MMB_ERR_LAUNCH;
-  }
   kern<<<dim3((unsigned)a.map.blocks()), dim3(64 * NW), (size_t)bytes, st>>>(a);
   return check_launch(BWD ? "mmb_cross_attention_bwd (resident)" : "mmb_cross_attention_fwd (resident)");
 }
@@ -364,31 +354,30 @@ static int run_res(ResArgs& a, int dtype, bool vec, hipStream_t st) {
   const Shape& s = a.sh;
   a.nkp = (s.Nk + 31) / 32 * 32;
   a.nqp = (s.Nq + 31) / 32 * 32;
-  const int groups = s.nkv / a.hw;
-  // forward: a cloud's query tiles over several workgroups while the chip is not full
+  // forward: a head's query tiles over several workgroups while the chip is not full
   a.parts = 1;
   if (!BWD)
-    while ((int64_t)s.B * groups * a.parts < 1024 && a.parts * kResWaves < a.hw * s.g * (a.nqp / 32)) a.parts *= 2;
-  a.map = {s.B, groups * a.parts, s.B % 8 == 0 || s.B >= 64 ? 1 : 0};
+    while ((int64_t)s.B * s.nkv * a.parts < 1024 && a.parts * kResWaves < s.g * (a.nqp / 32)) a.parts *= 2;
+  a.map = {s.B, s.nkv * a.parts, s.B % 8 == 0 || s.B >= 64 ? 1 : 0};
   MMB_REQUIRE(a.map.blocks() <= 0x7fffffffLL, "mmb_cross_attention: %lld workgroups", (long long)a.map.blocks());
-  const int64_t bytes = res_bytes(s, dtype, a.hw, BWD);
+  const int64_t bytes = res_bytes(s, dtype, BWD);
   if (dtype == MMB_DT_F32) return vec ? pick_res<BWD, float, true>(a, dtype, bytes, st) : pick_res<BWD, float, false>(a, dtype, bytes, st);
   if (dtype == MMB_DT_BF16) return vec ? pick_res<BWD, __bf16, true>(a, dtype, bytes, st) : pick_res<BWD, __bf16, false>(a, dtype, bytes, st);
   return vec ? pick_res<BWD, _Float16, true>(a, dtype, bytes, st) : pick_res<BWD, _Float16, false>(a, dtype, bytes, st);
 }
 
-int resident_fwd(const Shape& s, int hw, int dtype, bool vec, const void* q, int64_t q_ld, const void* k, int64_t k_ld, const void* v,
+int resident_fwd(const Shape& s, int dtype, bool vec, const void* q, int64_t q_ld, const void* k, int64_t k_ld, const void* v,
                  int64_t v_ld, const float* mq, const float* mk, float scale, void* out, int64_t out_ld, float* lse, hipStream_t st) {
   ResArgs a = {};
-  a.sh = s; a.hw = hw; a.q = q; a.q_ld = q_ld; a.k = k; a.k_ld = k_ld; a.v = v; a.v_ld = v_ld; a.mq = mq; a.mk = mk; a.scale = scale;
+  a.sh = s; a.q = q; a.q_ld = q_ld; a.k = k; a.k_ld = k_ld; a.v = v; a.v_ld = v_ld; a.mq = mq; a.mk = mk; a.scale = scale;
   a.o = out; a.out_ld = out_ld; a.lse = lse;
   return run_res<false>(a, dtype, vec, st);
 }
-int resident_bwd(const Shape& s, int hw, int dtype, bool vec, const void* q, int64_t q_ld, const void* k, int64_t k_ld, const void* v,
+int resident_bwd(const Shape& s, int dtype, bool vec, const void* q, int64_t q_ld, const void* k, int64_t k_ld, const void* v,
                  int64_t v_ld, const float* mq, const float* mk, float scale, const void* out, int64_t out_ld, const void* dout,
                  int64_t dout_ld, const float* lse, void* dq, int64_t dq_ld, void* dk, int64_t dk_ld, void* dv, int64_t dv_ld, hipStream_t st) {
   ResArgs a = {};
-  a.sh = s; a.hw = hw; a.q = q; a.q_ld = q_ld; a.k = k; a.k_ld = k_ld; a.v = v; a.v_ld = v_ld; a.mq = mq; a.mk = mk; a.scale = scale;
+  a.sh = s; a.q = q; a.q_ld = q_ld; a.k = k; a.k_ld = k_ld; a.v = v; a.v_ld = v_ld; a.mq = mq; a.mk = mk; a.scale = scale;
   a.out = out; a.out_ld = out_ld; a.dout = dout; a.dout_ld = dout_ld; a.lse = const_cast<float*>(lse);
   a.dq = dq; a.dq_ld = dq_ld; a.dk = dk; a.dk_ld = dk_ld; a.dv = dv; a.dv_ld = dv_ld;
   return run_res<true>(a, dtype, vec, st);
