@@ -189,7 +189,7 @@ struct SlotTiles {
 // 16-bit: row-major without padding, the 16-byte chunks of a row permuted by an exclusive-or with a function of the row
 //         that serves both kinds of read: 16 rows at one chunk column (the scores) and four rows of 16 columns (the
 //         transposing read of the second product) each fall on 64 different banks.
-template <int DP> constexpr int feature_tiles() { return DP < 32 ? 1 : DP / 32; }      // 32-row accumulators of DP features
+template <int DP> constexpr int feature_tiles() { return DP / 32; }      // 32-row accumulators of DP features
 template <typename T, int DP> constexpr int row_pitch() { return sizeof(T) == 2 ? DP : DP + 4; }
 template <int DP>
 __device__ __forceinline__ int swizzle(int row) {
@@ -243,8 +243,6 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 // out[t] (features 32t.. x columns) += X^T . w, the contraction over the 32 rows row0.. that w's registers run over.
-// (DP = 16, floats: the upper half of the feature rows multiplies what lies behind a row; it is never stored, the caller
-// keeps 16 elements behind the last row addressable.)
 // 16-bit: X^T by the transposing read: the 16 lanes that hold 16 columns address four rows (lane j: row j >> 2, columns
 // from 4 (j & 3)) and receive four rows of their own column.  float: one element a lane and step.
 template <typename T, int DP>
@@ -487,6 +485,14 @@ int resident_fwd(const Shape& s, int dtype, bool vec, const void* q, int64_t q_l
 int resident_bwd(const Shape& s, int dtype, bool vec, const void* q, int64_t q_ld, const void* k, int64_t k_ld, const void* v,
                  int64_t v_ld, const float* mq, const float* mk, float scale, const void* out, int64_t out_ld, const void* dout,
                  int64_t dout_ld, const float* lse, void* dq, int64_t dq_ld, void* dk, int64_t dk_ld, void* dv, int64_t dv_ld, hipStream_t st);
+
+// the same in floats with narrow heads (cross_attention_jets.hip)
+bool jets_fit(const Shape& s, int dtype, bool bwd);
+int jets_fwd(const Shape& s, bool vec, const float* q, int64_t q_ld, const float* k, int64_t k_ld, const float* v, int64_t v_ld,
+             const float* mq, const float* mk, float scale, float* out, int64_t out_ld, float* lse, hipStream_t st);
+int jets_bwd(const Shape& s, bool vec, const float* q, int64_t q_ld, const float* k, int64_t k_ld, const float* v, int64_t v_ld,
+             const float* mq, const float* mk, float scale, const float* out, int64_t out_ld, const float* dout, int64_t dout_ld,
+             const float* lse, float* dq, int64_t dq_ld, float* dk, int64_t dk_ld, float* dv, int64_t dv_ld, hipStream_t st);
 
 inline int pad_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 int check_shape(const char* who, int B, int Nq, int Nk, int nh, int nkv, int D, int dtype, float scale);

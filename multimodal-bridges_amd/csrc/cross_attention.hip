@@ -310,7 +310,7 @@ extern "C" int mmb_cross_attention_workspace(int B, int Nq, int Nk, int nheads, 
     return MMB_OK;
   }
   const Plan p = fwd_plan(s);
-  *bytes_host = p.nsplit > 1 && !resident_fits(s, dtype, false) ? (int64_t)B * nheads_kv * p.tiles * p.nsplit * 32 * (pad_width(D) + 2) * 4 : 0;
+  *bytes_host = p.nsplit > 1 && !resident_fits(s, dtype, false) && !jets_fit(s, dtype, false) ? (int64_t)B * nheads_kv * p.tiles * p.nsplit * 32 * (pad_width(D) + 2) * 4 : 0;
   return MMB_OK;
 }
 
@@ -327,6 +327,9 @@ extern "C" int mmb_cross_attention_fwd(int B, int Nq, int Nk, int nheads, int nh
   const int es = dtype == MMB_DT_F32 ? 4 : 2;
   const bool vec = D * es % 16 == 0 && chunk_aligned(q, q_ld, es) && chunk_aligned(k, k_ld, es) && chunk_aligned(v, v_ld, es) &&
                    chunk_aligned(out, out_ld, es);
+  if (jets_fit(s, dtype, false))
+    return jets_fwd(s, vec, (const float*)q, q_ld, (const float*)k, k_ld, (const float*)v, v_ld, maskf_q, maskf_k, scale, (float*)out, out_ld,
+                    lse, as_stream(stream));
   if (resident_fits(s, dtype, false))
     return resident_fwd(s, dtype, vec, q, q_ld, k, k_ld, v, v_ld, maskf_q, maskf_k, scale, out, out_ld, lse, as_stream(stream));
   const Plan p = fwd_plan(s);

@@ -369,6 +369,9 @@ extern "C" int mmb_cross_attention_bwd(int B, int Nq, int Nk, int nheads, int nh
                    chunk_aligned(out, out_ld, es) && chunk_aligned(dout, dout_ld, es) && chunk_aligned(dq, dq_ld, es) &&
                    chunk_aligned(dk, dk_ld, es) && chunk_aligned(dv, dv_ld, es);
   hipStream_t st = as_stream(stream);
+  if (jets_fit(a.sh, dtype, true))
+    return jets_bwd(a.sh, vec, (const float*)q, q_ld, (const float*)k, k_ld, (const float*)v, v_ld, maskf_q, maskf_k, scale, (const float*)out,
+                    out_ld, (const float*)dout, dout_ld, lse, (float*)dq, dq_ld, (float*)dk, dk_ld, (float*)dv, dv_ld, st);
   if (resident_fits(a.sh, dtype, true))
     return resident_bwd(a.sh, dtype, vec, q, q_ld, k, k_ld, v, v_ld, maskf_q, maskf_k, scale, out, out_ld, dout, dout_ld, lse, dq,
                         dq_ld, dk, dk_ld, dv, dv_ld, st);

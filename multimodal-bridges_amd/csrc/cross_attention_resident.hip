@@ -12,10 +12,9 @@
 namespace mmb {
 namespace xattn {
 
-// 16-wide heads of floats keep 16-wide rows (half the score products); every other width is padded to 32, 64 or 128
 template <typename T, int DP>
 struct ResTile {
-  static constexpr int E = Traits<T>::EPC, CH = DP / E, PITCH = row_pitch<T, DP>(), FT = DP < 32 ? 1 : DP / 32;
+  static constexpr int E = Traits<T>::EPC, CH = DP / E, PITCH = row_pitch<T, DP>(), FT = DP / 32;
 };
 
 struct ResArgs {
@@ -70,7 +69,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 2 : 3) res_fwd_kernel(Res
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
   T* Ks = reinterpret_cast<T*>(lds);
   T* Vs = Ks + a.nkp * R::PITCH;
-  int* klist = reinterpret_cast<int*>(Vs + a.nkp * R::PITCH + 16);
+  int* klist = reinterpret_cast<int*>(Vs + a.nkp * R::PITCH);
   int* qlist = klist + a.nkp;
   int* counts = qlist + a.nqp;
   const float* mq = a.mq ? a.mq + (int64_t)b * sh.Nq : nullptr;
@@ -143,7 +142,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(Res
   const int qs = a.nqp * R::PITCH, big = max(a.nkp * R::PITCH, heads * qs);
   T* A0 = reinterpret_cast<T*>(lds);              // K, then q
   T* A1 = A0 + big;                               // V, then dout
-  float* sl = reinterpret_cast<float*>(A1 + big + 16);                      // [head][nqp] log-sums, then deltas
+  float* sl = reinterpret_cast<float*>(A1 + big);                      // [head][nqp] log-sums, then deltas
   float* sd = sl + heads * a.nqp;
   int* klist = reinterpret_cast<int*>(sd + heads * a.nqp);
   int* qlist = klist + a.nkp;
@@ -315,16 +314,15 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(Res
 constexpr int kResBudget = 53 * 1024;             // three workgroups on a CU
 constexpr int kResWaves = 4;
 
-static int res_width(int D, int dtype) { return dtype == MMB_DT_F32 && D <= 16 ? 16 : pad_width(D); }
 static int64_t res_bytes(const Shape& s, int dtype, bool bwd) {
-  const int es = dtype == MMB_DT_F32 ? 4 : 2, dp = res_width(s.D, dtype), pitch = es == 2 ? dp : dp + 4;
+  const int es = dtype == MMB_DT_F32 ? 4 : 2, dp = pad_width(s.D), pitch = es == 2 ? dp : dp + 4;
   const int64_t nkp = (s.Nk + 31) / 32 * 32, nqp = (s.Nq + 31) / 32 * 32;
   int64_t rows = nkp;
   if (bwd && s.g * nqp > rows) rows = s.g * nqp;
-  return 2 * rows * pitch * es + 16 * es + (bwd ? 2 * s.g * nqp * 4 : 0) + (nkp + nqp + 4) * 4;
+  return 2 * rows * pitch * es + (bwd ? 2 * s.g * nqp * 4 : 0) + (nkp + nqp + 4) * 4;
 }
-// Whether a cloud is small: its workgroups leave room for two others on a CU (at 150 x 128 slots of 16 floats 243 us a training
-// step against 524 in the streaming kernels; at one workgroup a CU the two are level), there are clouds for every CU -- fewer
+// Whether a cloud is small: its workgroups leave room for two others on a CU (1024 clouds of 150 x 128 slots, 4 heads of 16 floats in
+// 32-wide tiles: 225 us a training step against 524 in the streaming kernels; at one workgroup a CU the two are level), there are clouds for every CU -- fewer
 // are spread better by the streaming kernels --, and a query tile is at least half full.
 bool resident_fits(const Shape& s, int dtype, bool bwd) {
   return s.Nk <= 1024 && s.Nq <= 1024 && s.Nq >= 16 && (int64_t)s.B * s.nkv >= 256 && res_bytes(s, dtype, bwd) <= kResBudget;
@@ -341,9 +339,7 @@ static int launch_res(ResArgs& a, int64_t bytes, hipStream_t st) {
 }
 template <bool BWD, typename T, bool VEC>
 static int pick_res(ResArgs& a, int dtype, int64_t bytes, hipStream_t st) {
-  switch (res_width(a.sh.D, dtype)) {
-    case 16:
-      if constexpr (sizeof(T) == 4) return launch_res<BWD, T, 16, VEC>(a, bytes, st);
+  switch (pad_width(a.sh.D)) {
     case 32: return launch_res<BWD, T, 32, VEC>(a, bytes, st);
     case 64: return launch_res<BWD, T, 64, VEC>(a, bytes, st);
     default: return launch_res<BWD, T, 128, VEC>(a, bytes, st);

@@ -1,6 +1,8 @@
 """Tensor-level wrappers over the C ABI: validate device/dtype/contiguity, allocate outputs
 with torch (plumbing only), enqueue on torch's current HIP stream.  No host syncs."""
+import contextlib
 import ctypes as C
+import functools
 import os
 
 import torch
@@ -729,10 +731,26 @@ def _xattn_args(q, k, v, B, nheads, nheads_kv, scale):
     return nkv, D, q.shape[0] // B, k.shape[0] // B, scale, qp + kp + vp
 
 
-def _workspace(name, *args, device):
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(name, *args):
     n = C.c_int64(0)
     call(name, *args, C.byref(n))
-    return (torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None), n.value
+    return n.value
+
+
+def _workspace(name, *args, device):
+    """(tensor | None, address | None, bytes): allocated on the current stream, for this call alone"""
+    n = _workspace_bytes(name, *args)
+    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    return ws, (ws.data_ptr() if n else None), n
+
+
+def _on(device):
+    """Makes the tensors' device current for the launch (nothing to do when it is)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def cross_attention_fwd(q, k, v, B, nheads, nheads_kv=None, mq=None, mk=None, scale=None, want_lse=False, out=None):
@@ -743,15 +761,15 @@ def cross_attention_fwd(q, k, v, B, nheads, nheads_kv=None, mq=None, mk=None, sc
     key.  scale: D ** -0.5 by default.  Returns out (B*Nq, nheads*D), with want_lse (out, lse (B, nheads, Nq) float32)."""
     nkv, D, Nq, Nk, scale, ptrs = _xattn_args(q, k, v, B, nheads, nheads_kv, scale)
     dev = q.device
-    with torch.cuda.device(dev):
+    with _on(dev):
         if out is None:
             out = torch.empty(B * Nq, nheads * D, dtype=q.dtype, device=dev)
         op = _rows(out, "out", q.dtype, B * Nq, nheads * D, dev)
         lse = torch.empty(B, nheads, Nq, dtype=torch.float32, device=dev) if want_lse else None
         shape = (B, Nq, Nk, nheads, nkv, D, DT[q.dtype])
-        ws, n = _workspace("mmb_cross_attention_workspace", *shape, 0, device=dev)
+        ws, wp, n = _workspace("mmb_cross_attention_workspace", *shape, 0, device=dev)
         call("mmb_cross_attention_fwd", *shape, *ptrs, _key_mask(mq, "mq", B, Nq, dev), _key_mask(mk, "mk", B, Nk, dev), _fl(scale),
-             *op, f32(lse), None if ws is None else ws.data_ptr(), n, stream())
+             *op, f32(lse), wp, n, stream())
     return (out, lse) if want_lse else out
 
 
@@ -761,16 +779,16 @@ def cross_attention_bwd(q, k, v, out, dout, lse, B, nheads, nheads_kv=None, mq=N
     are overwritten (dq, dk, dv given: rows that may be column slices), zero for padded slots.  Equal inputs, equal bits."""
     nkv, D, Nq, Nk, scale, ptrs = _xattn_args(q, k, v, B, nheads, nheads_kv, scale)
     dev = q.device
-    with torch.cuda.device(dev):
+    with _on(dev):
         dq = torch.empty(B * Nq, nheads * D, dtype=q.dtype, device=dev) if dq is None else dq
         dk = torch.empty(B * Nk, nkv * D, dtype=q.dtype, device=dev) if dk is None else dk
         dv = torch.empty(B * Nk, nkv * D, dtype=q.dtype, device=dev) if dv is None else dv
         o = [_rows(t, name, q.dtype, B * n, h * D, dev) for t, name, n, h in
              ((out, "out", Nq, nheads), (dout, "dout", Nq, nheads), (dq, "dq", Nq, nheads), (dk, "dk", Nk, nkv), (dv, "dv", Nk, nkv))]
         shape = (B, Nq, Nk, nheads, nkv, D, DT[q.dtype])
-        ws, n = _workspace("mmb_cross_attention_workspace", *shape, 1, device=dev)
+        ws, wp, n = _workspace("mmb_cross_attention_workspace", *shape, 1, device=dev)
         call("mmb_cross_attention_bwd", *shape, *ptrs, _key_mask(mq, "mq", B, Nq, dev), _key_mask(mk, "mk", B, Nk, dev), _fl(scale),
-             *o[0], *o[1], _vec(lse, "lse", B * nheads * Nq, dev), *o[2], *o[3], *o[4], ws.data_ptr(), n, stream())
+             *o[0], *o[1], _vec(lse, "lse", B * nheads * Nq, dev), *o[2], *o[3], *o[4], wp, n, stream())
     return dq, dk, dv
 
 
@@ -804,7 +822,7 @@ def head_norm_rotate_fwd(x, nheads, weight=None, nheads2=0, weight2=None, eps=1e
     pos[row, p // (pairs // axes)] * freq[p]; layout "half" pairs (p, p + pairs), "interleaved" (2p, 2p + 1).  The
     particles' own (eta, phi) as positions make scores depend on distances in that plane.  out may be x."""
     D, args, xp, tail = _head_args(x, nheads, weight, nheads2, weight2, eps, pos, freq, layout)
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
         op = _rows(out, "out", x.dtype, x.shape[0], x.shape[1], x.device)
         call("mmb_head_norm_rotate_fwd", *args, *xp, *tail, *op, stream())
@@ -819,7 +837,7 @@ def head_norm_rotate_bwd(x, dy, nheads, weight=None, nheads2=0, weight2=None, ep
     dx may be dy.  No gradient reaches pos and freq."""
     D, args, xp, tail = _head_args(x, nheads, weight, nheads2, weight2, eps, pos, freq, layout)
     dev = x.device
-    with torch.cuda.device(dev):
+    with _on(dev):
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if dx is None else dx
         gp = _rows(dy, "dy", x.dtype, x.shape[0], x.shape[1], dev)
         op = _rows(dx, "dx", x.dtype, x.shape[0], x.shape[1], dev)
@@ -861,7 +879,7 @@ def checkpoint_rows(x):
         raise MMBError("checkpoint_rows: no rows")
     M, K = x.shape
     nb = (K + 31) // 32
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         q8 = Q8Rows(torch.empty(M, 32 * nb, dtype=torch.int8, device=x.device),
                     torch.empty(M, nb, dtype=torch.uint8, device=x.device), K)
         _, _, cp, sp = q8.args()
@@ -872,7 +890,7 @@ def checkpoint_rows(x):
 def restore_rows(q8, dtype=torch.float32, out=None):
     """The (M, K) rows that a Q8Rows stands for."""
     M, K, cp, sp = q8.args()
-    with torch.cuda.device(q8.device):
+    with _on(q8.device):
         if out is None:
             if dtype not in DT:
                 raise MMBError(f"restore_rows: dtype {dtype} is not float32, bfloat16 or float16")
@@ -893,14 +911,14 @@ def grad_weight_rows_q8(q8, dZ, dW=None, db=None, accumulate=False, want_db=True
     if accumulate and dW is None:
         raise MMBError("grad_weight_rows_q8: accumulate needs dW")
     dev = q8.device
-    with torch.cuda.device(dev):
+    with _on(dev):
         if dW is None:
             dW = torch.empty(N, K, dtype=torch.float32, device=dev)
             db = torch.empty(N, dtype=torch.float32, device=dev) if db is None and want_db else db
         wp = _rows(dW, "dW", torch.float32, N, K, dev)
-        ws, n = _workspace("mmb_grad_weight_rows_q8_workspace", M, N, K, device=dev)
+        ws, ws_p, n = _workspace("mmb_grad_weight_rows_q8_workspace", M, N, K, device=dev)
         call("mmb_grad_weight_rows_q8", M, K, N, DT[dZ.dtype], cp, sp, *zp, *wp, _vec(db, "db", N, dev), int(bool(accumulate)),
-             ws.data_ptr(), n, stream())
+             ws_p, n, stream())
     return dW, db
 
 
