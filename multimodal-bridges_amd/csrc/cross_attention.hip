@@ -103,10 +103,12 @@ __global__ void __launch_bounds__(64 * NW, 2) fwd_kernel(FwdArgs a) {
     T* Vs = Ks + TILE_E;
     kr.store(tid, Ks);
     vr.store(tid, Vs);
-    const int nn = keys.next(TK);                 // the next tile's rows come in while this one is worked on
+    const int nn = keys.next(TK);
+    SlotTiles<TEAM>::sync();                      // (team: whoever passes here has read the other buffer)
+    // the next tile's rows come in while this one is worked on; issued behind the barrier, where finding their addresses
+    // overlaps with this tile's products
     kr.template load<VEC>(tid, nn, sh.D, [&](int i) { return kb + (int64_t)keys.slot(i) * a.k_ld; });
     vr.template load<VEC>(tid, nn, sh.D, [&](int i) { return vb + (int64_t)keys.slot(i) * a.v_ld; });
-    SlotTiles<TEAM>::sync();                      // (team: whoever passes here has read the other buffer)
     attend<T, DP, TK>(Ks, Vs, nk, qf, c, m, l, acc);
     nk = nn;
   }

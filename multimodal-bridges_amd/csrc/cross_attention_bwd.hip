@@ -98,9 +98,9 @@ __device__ __forceinline__ void dq_body(const BwdArgs& a, int64_t id, char* lds)
     kr.store(threadIdx.x, Ks);
     vr.store(threadIdx.x, Vs);
     const int nn = keys.next(TK);
+    SlotTiles<NW>::sync();
     kr.template load<VEC>(threadIdx.x, nn, sh.D, [&](int i) { return kb + (int64_t)keys.slot(i) * a.k_ld; });
     vr.template load<VEC>(threadIdx.x, nn, sh.D, [&](int i) { return vb + (int64_t)keys.slot(i) * a.v_ld; });
-    SlotTiles<NW>::sync();
     if (a.few_keys) {                             // at most 32 keys, all of them here: p normalised by its own sum
       f32x16 s = dot_rows<T, DP>(Ks, 0, qf, zero16());
       const f32x16 dp = dot_rows<T, DP>(Vs, 0, gf, zero16());
@@ -195,13 +195,11 @@ __device__ __forceinline__ void dkv_body(const BwdArgs& a, int64_t id, char* lds
     auto fetch = [&](int n) {
       qr.template load<VEC>(threadIdx.x, n, sh.D, [&](int i) { return qb + (int64_t)rows.slot(i) * a.q_ld; });
       gr.template load<VEC>(threadIdx.x, n, sh.D, [&](int i) { return gb + (int64_t)rows.slot(i) * a.dout_ld; });
-      st_l = INFINITY;                            // rows past the end, and rows without a key: p = 0
-      st_d = 0.0f;
-      if (threadIdx.x < TQ && threadIdx.x < n) {
+      st_l = -INFINITY;
+      if (threadIdx.x < TQ && threadIdx.x < n) {  // (both loads at once; looked at when the tile is stored)
         const int s = rows.slot(threadIdx.x);
-        st_l = row_stat<T>(a.lse[stat + s]);
-        if (st_l < INFINITY) st_d = a.delta[stat + s];
-        if (__is_same(T, _Float16)) st_l -= kHalfLog;
+        st_l = a.lse[stat + s];
+        st_d = a.delta[stat + s];
       }
     };
     fetch(nq);
@@ -212,12 +210,13 @@ __device__ __forceinline__ void dkv_body(const BwdArgs& a, int64_t id, char* lds
       qr.store(threadIdx.x, Qs);
       gr.store(threadIdx.x, Gs);
       if (threadIdx.x < TQ) {
-        sl[threadIdx.x] = st_l;
-        sl[TQ + threadIdx.x] = st_d;
+        const float x = row_stat<T>(st_l);        // rows past the end, and rows without a key: p = 0
+        sl[threadIdx.x] = __is_same(T, _Float16) ? x - kHalfLog : x;
+        sl[TQ + threadIdx.x] = x < INFINITY ? st_d : 0.0f;
       }
       const int nn = rows.next(TQ);
-      fetch(nn);
       SlotTiles<NW>::sync();
+      fetch(nn);
 #pragma unroll
       for (int sub = 0; sub < TQ; sub += 32) {
         f32x16 s = dot_rows<T, DP>(Qs, sub, kf, zero16());
