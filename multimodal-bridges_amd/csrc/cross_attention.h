@@ -88,6 +88,10 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// First statement of a branch that is rarely taken: keeps the compiler from executing the branch's arithmetic always and
+// selecting afterwards (it does so for the tail of the keys and for rescaling, at three instructions an element).
+__device__ __forceinline__ void rarely() { asm volatile(""); }
+
 constexpr int kChunk = 512;                       // raw slots one compaction step looks at
 
 // Appends the slots n in [lo, min(lo + kChunk, hi)) with maskf[n] != 0 to list[], in order; returns how many.
@@ -293,24 +297,30 @@ __device__ __forceinline__ T round_to(float x) {
 // what the column has summed; values 2^-38 below the largest are lost, which is below the sum's own rounding.
 struct ColScale {
   float sc = 0x1p60f;                              // (products of halves stay below 2^52: no overflow in 32 bits)
-  // w already carries sc
-  __device__ __forceinline__ void fit(f32x16& w, f32x16* acc, int n_acc) {
+  // N tiles of values that already carry sc; true: the scale has changed
+  template <int N>
+  __device__ __forceinline__ bool fit(f32x16* w, f32x16* acc, int n_acc) {
     float top = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(w[r]));
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(w[u][r]));
     top = fmaxf(top, __shfl_xor(top, 32));
-    if (__any(top >= 0x1p14f)) {
-      const int ex = (int)(__float_as_uint(top) >> 23);                       // 2^(ex - 127) <= top
-      const float f = top >= 0x1p14f ? __uint_as_float((uint32_t)max(266 - ex, 12) << 23) : 1.0f;      // top * f in [2^12, 2^13)
+    if (!__any(top >= 0x1p14f)) return false;
+    rarely();
+    const int ex = (int)(__float_as_uint(top) >> 23);                         // 2^(ex - 127) <= top
+    const float f = top >= 0x1p14f ? __uint_as_float((uint32_t)max(266 - ex, 12) << 23) : 1.0f;        // top * f in [2^12, 2^13)
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-        if (t < n_acc)
+    for (int t = 0; t < 4; ++t)
+      if (t < n_acc)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[t][r] *= f;
+        for (int r = 0; r < 16; ++r) acc[t][r] *= f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) w[r] *= f;
-      sc *= f;
-    }
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) w[u][r] *= f;
+    sc *= f;
+    return true;
   }
 };
 

@@ -115,25 +115,30 @@ __device__ __forceinline__ void dq_body(const BwdArgs& a, int64_t id, char* lds)
       for (int r = 0; r < 16; ++r) delta = fmaf(sum == 0.0f ? 0.0f : s[r] / sum, dp[r], delta);
       delta += __shfl_xor(delta, 32);
     }
+    // all score tiles, then all second products: the matrix work of one tile beside the element work of another
+    constexpr int SUBS = TK / 32;
+    f32x16 s[SUBS];
 #pragma unroll
-    for (int sub = 0; sub < TK; sub += 32) {
-      f32x16 s = dot_rows<T, DP>(Ks, sub, qf, zero16());
-      const f32x16 dp = dot_rows<T, DP>(Vs, sub, gf, zero16());
-      // ds is rounded to the inputs' type for the product, like p in the forward; the sum over keys stays in 32 bits
+    for (int u = 0; u < SUBS; ++u) {
+      s[u] = dot_rows<T, DP>(Ks, 32 * u, qf, zero16());
+      const f32x16 dp = dot_rows<T, DP>(Vs, 32 * u, gf, zero16());
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = prob<T>(s[r], a.scale, c, st) * (dp[r] - delta);
-      if (sub + 32 > nk) {
+      for (int r = 0; r < 16; ++r) s[u][r] = prob<T>(s[u][r], a.scale, c, st) * (dp[r] - delta);
+    }
+    if (nk < TK) {
+      rarely();
+#pragma unroll
+      for (int u = 0; u < SUBS; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (sub + crow(r, h) >= nk) s[r] = 0.0f;
-      }
-      if constexpr (__is_same(T, _Float16)) {
-        const float before = cs.sc;
-        cs.fit(s, acc, DP / 32);
-        if (__any(cs.sc != before)) st = lse - log2_pow2(cs.sc);
-      }
-      dot_cols<T, DP>(Ks, sub, s, acc);
+          if (32 * u + crow(r, h) >= nk) s[u][r] = 0.0f;
     }
+    if constexpr (__is_same(T, _Float16)) {
+      if (cs.fit<SUBS>(s, acc, DP / 32)) st = lse - log2_pow2(cs.sc);
+    }
+    // ds is rounded to the inputs' type for the product, like p in the forward; the sum over keys stays in 32 bits
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u) dot_cols<T, DP>(Ks, 32 * u, s[u], acc);
     nk = nn;
   }
   if (!live) return;
@@ -217,28 +222,30 @@ __device__ __forceinline__ void dkv_body(const BwdArgs& a, int64_t id, char* lds
       const int nn = rows.next(TQ);
       SlotTiles<NW>::sync();
       fetch(nn);
+      constexpr int SUBS = TQ / 32;
+      f32x16 s[SUBS], dp[SUBS];
 #pragma unroll
-      for (int sub = 0; sub < TQ; sub += 32) {
-        f32x16 s = dot_rows<T, DP>(Qs, sub, kf, zero16());
-        f32x16 dp = dot_rows<T, DP>(Gs, sub, vf, zero16());
+      for (int u = 0; u < SUBS; ++u) {
+        s[u] = dot_rows<T, DP>(Qs, 32 * u, kf, zero16());
+        dp[u] = dot_rows<T, DP>(Gs, 32 * u, vf, zero16());
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4) {
-          const f32x4 ls = *reinterpret_cast<const f32x4*>(sl + sub + 8 * g4 + 4 * h);
-          const f32x4 dl = *reinterpret_cast<const f32x4*>(sl + TQ + sub + 8 * g4 + 4 * h);
+          const f32x4 ls = *reinterpret_cast<const f32x4*>(sl + 32 * u + 8 * g4 + 4 * h);
+          const f32x4 dl = *reinterpret_cast<const f32x4*>(sl + TQ + 32 * u + 8 * g4 + 4 * h);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int r = 4 * g4 + i;
-            s[r] = prob<T>(s[r], a.scale, c, ls[i]);
-            dp[r] = s[r] * (dp[r] - dl[i]);
+            s[u][r] = prob<T>(s[u][r], a.scale, c, ls[i]);
+            dp[u][r] = s[u][r] * (dp[u][r] - dl[i]);
+            if constexpr (__is_same(T, _Float16)) dp[u][r] *= cs.sc;
           }
         }
-        if constexpr (__is_same(T, _Float16)) {
+      }
+      if constexpr (__is_same(T, _Float16)) cs.fit<SUBS>(dp, dk, DP / 32);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) dp[r] *= cs.sc;
-          cs.fit(dp, dk, DP / 32);
-        }
-        dot_cols<T, DP>(Gs, sub, s, dv);
-        dot_cols<T, DP>(Qs, sub, dp, dk);
+      for (int u = 0; u < SUBS; ++u) {
+        dot_cols<T, DP>(Gs, 32 * u, s[u], dv);
+        dot_cols<T, DP>(Qs, 32 * u, dp[u], dk);
       }
       nq = nn;
     }

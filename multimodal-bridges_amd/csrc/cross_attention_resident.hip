@@ -236,14 +236,13 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(Res
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = prob<T>(s[r], a.scale, c, st) * (dp[r] - delta);
       if (kt0 + 32 > nk) {
+        rarely();
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (kt0 + crow(r, h) >= nk) s[r] = 0.0f;
       }
       if constexpr (HALF) {
-        const float before = cs.sc;
-        cs.fit(s, acc, R::FT);
-        if (__any(cs.sc != before)) st = lse - log2_pow2(cs.sc);
+        if (cs.fit<1>(&s, acc, R::FT)) st = lse - log2_pow2(cs.sc);
       }
       dot_cols<T, DP>(kh, kt0, s, acc);
     }
@@ -296,7 +295,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(Res
         if constexpr (HALF) {
 #pragma unroll
           for (int r2 = 0; r2 < 16; ++r2) dp[r2] *= cs.sc;
-          cs.fit(dp, dk, R::FT);
+          cs.fit<1>(&dp, dk, R::FT);
         }
         dot_cols<T, DP>(gh, q0, s, dv);
         dot_cols<T, DP>(qh, q0, dp, dk);
