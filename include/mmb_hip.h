@@ -502,8 +502,9 @@ int mmb_head_norm_rotate_bwd(int64_t M, int nheads, int nheads2, int D, int dtyp
 /* Activations kept for the reverse pass in 8 bits.  32 consecutive features of a row share a step 2^e, e the smallest
  * exponent >= -127 with 127 * 2^e >= max |x|; codes (M, 32*ceil(K/32)) int8 = round(x / 2^e), ties to even, features past K
  * zero; steps (M, ceil(K/32)) uint8 = e + 127, 255 for a block that holds an infinity or NaN (it is restored as NaN).
- * |restored - x| <= 2^(e-1).  x: M rows of K, dtype MMB_DT_*.  codes 16-byte aligned. */
-int mmb_checkpoint_rows(int64_t M, int K, int dtype, const void* x, int64_t x_ld, void* codes, void* steps, void* stream);
+ * |restored - x| <= 2^(e-1).  keep_nonzero != 0: values other than 0 get code +-1 at least (ReLU outputs: the gate is the same
+ * from the checkpoint; |restored - x| < 2^e).  x: M rows of K, dtype MMB_DT_*.  codes 16-byte aligned. */
+int mmb_checkpoint_rows(int64_t M, int K, int dtype, int keep_nonzero, const void* x, int64_t x_ld, void* codes, void* steps, void* stream);
 /* y (M, K) = code * 2^e, rounded to dtype (exact in float and bf16) */
 int mmb_restore_rows(int64_t M, int K, int dtype, const void* codes, const void* steps, void* y, int64_t y_ld, void* stream);
 /* Weight gradient of a Linear straight from its input's checkpoint: dW (N, K) = dZ^T Xhat, db (N) | NULL = column sums of

@@ -5,6 +5,8 @@
 // rounding but its own, and a value stands for at most half a step off: |xhat - x| <= 2^(e-1) <= max|x| / 127.  An integer
 // grid over a shared step holds a block of like-sized activations about four times closer than an 8-bit float would (whose
 // three mantissa bits spend the range on small values).
+// With keep_nonzero a value that would round to code 0 takes code +-1 (a step off at most, not half): what is told from the
+// sign of an activation -- whether a ReLU passes the gradient -- is then told the same from its checkpoint.
 // step byte = e + 127; 255 marks a block that held an infinity or a NaN: it comes back as NaN, never as a finite value.
 //
 // A code is an integer of 7 bits: code * 2^e is EXACT in bf16.  The weight gradient dW = dZ^T Xhat therefore needs ONE bf16
@@ -53,7 +55,8 @@ __device__ __forceinline__ void load8(const T* __restrict__ p, int k, int K, flo
 // a thread owns 8 features, four neighbouring lanes one block of 32
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-encode_kernel(int64_t M, int K, int nb, const T* __restrict__ x, int64_t x_ld, int8_t* __restrict__ codes, uint8_t* __restrict__ steps) {
+encode_kernel(int64_t M, int K, int nb, int keep_nonzero, const T* __restrict__ x, int64_t x_ld, int8_t* __restrict__ codes,
+              uint8_t* __restrict__ steps) {
   const int64_t n = M * nb * 4;
   for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
     const int64_t blk = t >> 2, row = blk / nb;
@@ -75,7 +78,10 @@ encode_kernel(int64_t M, int K, int nb, const T* __restrict__ x, int64_t x_ld, i
       const float lim = s >= 249u ? 63.0f : 127.0f;                     // (64 * 2^122 would leave the range of a float)
       int q[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = (int)fminf(fmaxf(rintf(v[i] * inv), -lim), lim);
+      for (int i = 0; i < 8; ++i) {
+        q[i] = (int)fminf(fmaxf(rintf(v[i] * inv), -lim), lim);
+        if (keep_nonzero && q[i] == 0 && v[i] != 0.0f) q[i] = v[i] > 0.0f ? 1 : -1;
+      }
       packed.x = (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | (uint32_t)q[3] << 24;
       packed.y = (q[4] & 255) | (q[5] & 255) << 8 | (q[6] & 255) << 16 | (uint32_t)q[7] << 24;
     }
@@ -393,11 +399,11 @@ static int check_q8(const char* who, int64_t M, int K, const void* codes, const 
 }
 
 template <typename T>
-static int encode(int64_t M, int K, const void* x, int64_t x_ld, void* codes, void* steps, hipStream_t st) {
+static int encode(int64_t M, int K, int keep_nonzero, const void* x, int64_t x_ld, void* codes, void* steps, hipStream_t st) {
   const int nb = (K + 31) / 32, grid = stream_grid(M * nb * 4, 256);
   const bool vec = K % 8 == 0 && ((uintptr_t)x & 15) == 0 && x_ld * (int64_t)sizeof(T) % 16 == 0;
-  if (vec) encode_kernel<T, true><<<grid, 256, 0, st>>>(M, K, nb, (const T*)x, x_ld, (int8_t*)codes, (uint8_t*)steps);
-  else encode_kernel<T, false><<<grid, 256, 0, st>>>(M, K, nb, (const T*)x, x_ld, (int8_t*)codes, (uint8_t*)steps);
+  if (vec) encode_kernel<T, true><<<grid, 256, 0, st>>>(M, K, nb, keep_nonzero, (const T*)x, x_ld, (int8_t*)codes, (uint8_t*)steps);
+  else encode_kernel<T, false><<<grid, 256, 0, st>>>(M, K, nb, keep_nonzero, (const T*)x, x_ld, (int8_t*)codes, (uint8_t*)steps);
   return check_launch("mmb_checkpoint_rows");
 }
 template <typename T>
@@ -441,13 +447,14 @@ static int grad_weight(GwArgs& a, int bk, float* dW, int64_t dw_ld, float* db, i
 using namespace mmb;
 using namespace mmb::ckpt;
 
-extern "C" int mmb_checkpoint_rows(int64_t M, int K, int dtype, const void* x, int64_t x_ld, void* codes, void* steps, void* stream) {
+extern "C" int mmb_checkpoint_rows(int64_t M, int K, int dtype, int keep_nonzero, const void* x, int64_t x_ld, void* codes, void* steps,
+                                   void* stream) {
   if (int rc = check_q8("mmb_checkpoint_rows", M, K, codes, steps)) return rc;
   MMB_REQUIRE(x && x_ld >= K, "mmb_checkpoint_rows: x is NULL or its leading dimension smaller than its row");
   hipStream_t st = as_stream(stream);
-  if (dtype == MMB_DT_F32) return encode<float>(M, K, x, x_ld, codes, steps, st);
-  if (dtype == MMB_DT_BF16) return encode<__bf16>(M, K, x, x_ld, codes, steps, st);
-  if (dtype == MMB_DT_F16) return encode<_Float16>(M, K, x, x_ld, codes, steps, st);
+  if (dtype == MMB_DT_F32) return encode<float>(M, K, keep_nonzero != 0, x, x_ld, codes, steps, st);
+  if (dtype == MMB_DT_BF16) return encode<__bf16>(M, K, keep_nonzero != 0, x, x_ld, codes, steps, st);
+  if (dtype == MMB_DT_F16) return encode<_Float16>(M, K, keep_nonzero != 0, x, x_ld, codes, steps, st);
   set_error("mmb_checkpoint_rows: unknown dtype %d", dtype);
   return MMB_ERR_INVALID_ARG;
 }

@@ -21,6 +21,7 @@ import torch
 
 from mmb_hip import ops
 from mmb_hip.ops import SEG_ROW, SEG_JET, SEG_JET_MASK
+from encoders.checkpoint8 import Keep8, storage_id
 
 
 GW_REPLICAS = 8
@@ -30,14 +31,14 @@ class GradStore:
     def __init__(self):
         self.bufs = {}
         self.relu_gates, self.gated = {}, set()         # (see _relu_gates)
+        self.kept = Keep8()                             # activations that the forward left in 8 bits
 
-    @staticmethod
-    def _key(t):
-        return t.untyped_storage().data_ptr()
+    _key = staticmethod(storage_id)
 
     @staticmethod
     def _owns_storage(t):
-        return t.is_contiguous() and t.storage_offset() == 0 and t.untyped_storage().nbytes() == t.numel() * 4
+        n = t.untyped_storage().nbytes()                # (0: the storage of a whole tensor, kept in 8 bits)
+        return t.is_contiguous() and t.storage_offset() == 0 and (n == t.numel() * 4 or n == 0)
 
     def seed(self, t, g):
         """Gradient of a tensor that owns its whole storage."""
@@ -46,7 +47,7 @@ class GradStore:
     def view(self, t):
         key = self._key(t)
         if key not in self.bufs:
-            n = t.untyped_storage().nbytes() // 4
+            n = t.untyped_storage().nbytes() // 4 or t.numel()
             self.bufs[key] = (torch.zeros(n, dtype=torch.float32, device=t.device), t)
         return self.bufs[key][0].as_strided(t.shape, t.stride(), t.storage_offset())
 
@@ -76,6 +77,14 @@ class GradStore:
             self.bufs[key] = (g.reshape(-1), t)
         else:
             self.view(t).add_(g)
+
+    def done(self, *tensors):
+        """The gradients of these activations are not needed any more.  Only where the forward kept its activations in 8
+        bits: there the gradients, not the tape, would be what the reverse pass holds most of."""
+        if self.kept:
+            for t in tensors:
+                if t is not None and self._owns_storage(t):
+                    self.bufs.pop(self._key(t), None)
 
 
 class Arena:
@@ -219,12 +228,22 @@ def param_grads(layer, segs, dZ, S, Sm, arena, touched):
     return W
 
 
-def plain_param_grads(spec, segs, dZ, S, Sm, arena):
+def plain_param_grads(spec, segs, dZ, S, Sm, arena, kept=None):
     """The same for a PlainLinear (encoders/particle_transformer.py): dW of the concatenated weight through the
     row-streaming kernel, replicas folded by mmb_sum_replicas, then split over the nn.Linear parameters (an
     identity part has none).  Returns the effective (concatenated) weight."""
     M, Nout = dZ.shape
     W = spec.weight()
+    q8 = kept.rows(segs[0][0]) if kept and len(segs) == 1 and len(spec.parts) == len(spec.biases) == 1 else None
+    if q8 is not None:                                  # the input was kept in 8 bits: dW, db straight from the codes
+        w, b = spec.parts[0][0], spec.biases[0]
+        if w.grad is not None and b.grad is not None and w.grad.is_contiguous() and b.grad.is_contiguous():
+            ops.grad_weight_rows_q8(q8, dZ, dW=w.grad, db=b.grad, accumulate=True)
+        else:
+            dW, db = ops.grad_weight_rows_q8(q8, dZ)
+            _acc_param(w, dW)
+            _acc_param(b, db)
+        return W
     R = GW_REPLICAS if M >= 16384 else 1
     Kall = W.shape[1]
     dWr = arena.take((R, Nout * Kall))
@@ -288,8 +307,12 @@ def _linear_bwd(e, store, produced, mi, seed, arena, touched):
         dZ = gY1                        # its consumer's GEMM already applied relu' (mmb_linear_cat_gate)
     elif y1 is None and y2 is not None and GradStore._key(y2) in store.gated:
         dZ = gY2                        # ... and, for relu + dropout, the keep factor with it
+    elif store.kept and act is None and post is None:
+        # dropout alone: the values (kept in 8 bits) do not matter, only a matrix of their shape does
+        dZ = ops.act_bwd(M, Nout, gY1, gY2, gY2, None, None, None, act, post, p, seed, off)
     else:
-        dZ = ops.act_bwd(M, Nout, gY1, gY2, y1, y2, res2, pre, act, post, p, seed, off)
+        with store.kept.restored(y1, y2, res2, pre):
+            dZ = ops.act_bwd(M, Nout, gY1, gY2, y1, y2, res2, pre, act, post, p, seed, off)
     if res2 is not None and gY2 is not None and GradStore._key(res2) in produced:
         store.add(res2, gY2)            # y2's gradient is final here: nothing reads it after its producer
     if res1 is not None and GradStore._key(res1) in produced:
@@ -304,7 +327,7 @@ def _linear_bwd(e, store, produced, mi, seed, arena, touched):
     S = ops.jet_sum(dZ, B, N) if SEG_JET in kinds else None
     Sm = ops.jet_sum(dZ, B, N, maskf=maskf) if SEG_JET_MASK in kinds else None
     if kind_ == "plinear":
-        W = plain_param_grads(layer, segs, dZ, S, Sm, arena)
+        W = plain_param_grads(layer, segs, dZ, S, Sm, arena, store.kept)
     else:
         W = param_grads(layer, segs, dZ, S, Sm, arena, touched)
     # ---- inputs
@@ -322,7 +345,8 @@ def _linear_bwd(e, store, produced, mi, seed, arena, touched):
             if kind == SEG_ROW and fresh and GradStore._key(t) in store.relu_gates:
                 g_act, g_ref, g_scale = store.relu_gates[GradStore._key(t)]
                 Wg = Wseg if g_scale == 1.0 else (Wseg * g_scale).contiguous()         # (a d x ff matrix: one tiny launch)
-                ops.linear_cat_gate([(dZ, SEG_ROW)], Wg, N, g_ref, gx, act=g_act)      # dZ of the activated layer
+                with store.kept.restored(g_ref):
+                    ops.linear_cat_gate([(dZ, SEG_ROW)], Wg, N, g_ref, gx, act=g_act)  # dZ of the activated layer
                 store.gated.add(GradStore._key(t))
             elif kind == SEG_ROW:
                 ops.linear_cat([(dZ, SEG_ROW)], Wseg, None, N, residual=res, out=gx)
@@ -337,7 +361,14 @@ def _attn_bwd(e, store, mi, seed=0):
     p, off = (e[5], e[6]) if len(e) > 5 else (0.0, 0)
     bits = e[7] if len(e) > 7 else None
     g = store.get(a)
-    if g is not None:
+    if g is not None and lse is None:
+        # qkv was kept in 8 bits: attention of the decoded rows once more, so that out and log-sum are those of the values the
+        # gradient is taken at (with the exact rows' log-sum the decoded probabilities would not sum to one)
+        with store.kept.restored(qkv):
+            r = ops.attention_fwd(qkv, mi, nheads, valid_is_zero=True, want_lse=True, drop_p=p, seed=seed, offset=off)
+            store.add(qkv, ops.attention_bwd(qkv, mi, nheads, r[0], g, r[1], valid_is_zero=True, drop_p=p, seed=seed,
+                                             offset=off, keep_bits=r[2] if len(r) > 2 else None))
+    elif g is not None:
         store.add(qkv, ops.attention_bwd(qkv, mi, nheads, a, g, lse, valid_is_zero=True, drop_p=p, seed=seed, offset=off,
                                          keep_bits=bits))
 
@@ -357,8 +388,9 @@ def _ln_bwd(e, store, produced, arena):
     if GradStore._key(x) in produced:
         gx, fresh = store.target(x)
     else:
-        gx, fresh = torch.empty_like(x), True
-    ops.layernorm_bwd(x, norm.weight.detach(), stats, g, gx, not fresh, dgamma, dbeta)
+        gx, fresh = torch.empty(x.shape, dtype=torch.float32, device=x.device), True
+    with store.kept.restored(x):
+        ops.layernorm_bwd(x, norm.weight.detach(), stats, g, gx, not fresh, dgamma, dbeta)
     if not direct:
         _acc_param(norm.weight, dgamma, shared=True)
         _acc_param(norm.bias, dbeta, shared=True)
@@ -414,6 +446,7 @@ def run_backward(model, tape, heads, d_hc, d_hd, d_s=None, scale=None):
         store.seed(heads.discrete, d_hd.reshape(-1, d_hd.shape[-1]))
     produced = _produced(tape)
     store.relu_gates, store.gated = _relu_gates(tape), set()
+    store.kept = next((e[1] for e in tape if e[0] == "kept8"), None) or Keep8()
     mi = next(e[3] if e[0] == "embed" else e[2] for e in tape if e[0] in ("embed", "toyin"))
     seed = model.seed
     n_acc = sum(GW_REPLICAS * (e[1].weight_v.numel() + e[1].weight_v.shape[0] + 8) for e in tape if e[0] == "linear")
@@ -425,10 +458,13 @@ def run_backward(model, tape, heads, d_hc, d_hd, d_s=None, scale=None):
         kind = e[0]
         if kind in ("linear", "plinear"):
             _linear_bwd(e, store, produced, mi, seed, arena, touched)
+            store.done(e[9], e[10])
         elif kind == "attn":
             _attn_bwd(e, store, mi, seed)
+            store.done(e[2])
         elif kind == "ln":
             _ln_bwd(e, store, produced, arena)
+            store.done(e[2])
         elif kind == "pool":
             gP = store.get(e[2])
             if gP is not None and GradStore._key(e[1]) in produced:

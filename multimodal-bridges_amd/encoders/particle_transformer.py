@@ -24,6 +24,9 @@ Dropout (training mode, encoder.dropout > 0) sits where nn.TransformerEncoderLay
 probabilities (mmb_attention_dropout_fwd), after out_proj (dropout1), after the FFN's ReLU, after linear2 (dropout2);
 Philox masks keyed by (model seed, per-call offset), regenerated by the reverse pass.  Same law as torch's, another
 random stream: checked statistically and, with the masks extracted, exactly (tests/test_hip_transformer.py).
+
+encoder.checkpoint_bits: 8 keeps the activations of the layers in 8 bits between forward and reverse pass (checkpoint8.py):
+a quarter of the tape; the attention runs once more in the reverse pass, on the decoded rows.
 """
 import os
 from types import SimpleNamespace
@@ -38,6 +41,7 @@ from encoders.multimodal_epic import _unpack, _Head
 from mmb_hip import ops
 from mmb_hip import fused as fused_epic
 from mmb_hip.ops import SEG_ROW
+from encoders.checkpoint8 import Keep8, activations
 
 
 class PlainLinear:
@@ -190,22 +194,30 @@ class TransformerEncoderBlock(nn.Module):
                 out.copy_(h)
                 h = out
             return h
+        kept = getattr(ctx, "kept", None) if ctx.recording else None
         for i, (in_proj, out_proj, lin1, lin2, norm1, norm2) in enumerate(layers):
+            mark = len(ctx.tape) if kept is not None else 0
             qkv = in_proj.run(ctx, [(h, SEG_ROW)])
             rec = ctx.recording
+            lse = rec and kept is None                     # (kept in 8 bits: the reverse pass runs the attention again)
             off = ctx.next_offset() if p > 0.0 else 0
             if attn is not None:
                 r = attn(qkv)
             else:
-                r = ops.attention_fwd(qkv, ctx.mi, self.n_heads, valid_is_zero=True, want_lse=rec,  # quirk Q4
+                r = ops.attention_fwd(qkv, ctx.mi, self.n_heads, valid_is_zero=True, want_lse=lse,  # quirk Q4
                                       drop_p=p, seed=ctx.seed, offset=off)
-            a = r[0] if rec else r
+            a = r[0] if lse else r
             if rec:
-                ctx.tape.append(("attn", qkv, a, r[1], self.n_heads, p, off, r[2] if len(r) > 2 else None))
+                ctx.tape.append(("attn", qkv, a, r[1] if lse else None, self.n_heads, p, off,
+                                 r[2] if lse and len(r) > 2 else None))
             # x = norm1(x + dropout1(out_proj(attn)));  x = norm2(x + dropout2(linear2(dropout(relu(linear1(x))))))
             h1 = out_proj.run(ctx, [(a, SEG_ROW)], res1=h, norm=norm1, dropout=True)
             f = lin1.run(ctx, [(h1, SEG_ROW)], act="relu", dropout=True)
             h = lin2.run(ctx, [(f, SEG_ROW)], res1=h1, norm=norm2, out=out if i == len(layers) - 1 else None, dropout=True)
+            if kept is not None:                           # all that this layer's entries hold, but its output
+                for t, gate in activations(ctx.tape[mark:]):
+                    if t is not h:
+                        kept.keep(t, gate)
         if not layers and out is not None:
             out.copy_(h)
             h = out
@@ -222,11 +234,13 @@ class TransformerEncoderBlock(nn.Module):
 class MultiModalParticleTransformer(nn.Module):
     """Two branch transformers (continuous / discrete features), an optional fusion transformer over cat[h1,h2]
     and two GELU MLP heads on cat[t, h_i, f_i] (particle_transformer.py:52-167)."""
+    checkpoint_bits_choices = (None, 8)
 
     def __init__(self, config):
         super().__init__()
         self.config = config
         e, d = config.encoder, config.data
+        self.checkpoint_bits = getattr(e, "checkpoint_bits", None)
         Et = e.dim_emb_time
         dim_cont, dim_disc = e.dim_emb_continuous, e.dim_emb_discrete * d.dim_discrete
         H0, H1 = e.dim_hidden_local[0], e.dim_hidden_local[1]
@@ -325,6 +339,9 @@ class MultiModalParticleTransformer(nn.Module):
         glob = state_global if state_global is not None else TensorMultiModal(time=state_local.time)
         ctx, time, cont, disc, _ = _unpack(state_local, glob, self.training, self.config.encoder.dropout, tape, seed,
                                            offset0)
+        if ctx.recording and self.checkpoint_bits:
+            ctx.kept = Keep8()
+            tape.append(("kept8", ctx.kept))
         cp = self._compaction(state_local, ctx, time)
         if cp is not None:
             hc, hd = self.run_compact(ctx, time, cont, disc, cp)

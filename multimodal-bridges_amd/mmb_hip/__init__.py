@@ -134,7 +134,7 @@ SIGNATURES = {
     "mmb_head_norm_rotate_bwd": [C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
                                  c_f32p, c_f32p, C.c_float, c_f32p, C.c_int64, C.c_int, c_f32p, C.c_int, C.c_int, C.c_void_p,
                                  C.c_int64, c_f32p, c_f32p, c_f32p, c_stream],
-    "mmb_checkpoint_rows": [C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, c_stream],
+    "mmb_checkpoint_rows": [C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, c_stream],
     "mmb_restore_rows": [C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, c_stream],
     "mmb_grad_weight_rows_q8": [C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, c_f32p,
                                 C.c_int64, c_f32p, C.c_int, C.c_void_p, C.c_int64, c_stream],

@@ -872,8 +872,8 @@ class Q8Rows:
         return self.codes.shape[0], self.K, _chk(self.codes, torch.int8, "codes"), _chk(self.steps, torch.uint8, "steps")
 
 
-def checkpoint_rows(x):
-    """x (M, K) float32 / bfloat16 / float16 rows -> Q8Rows"""
+def checkpoint_rows(x, keep_nonzero=False):
+    """x (M, K) float32 / bfloat16 / float16 rows -> Q8Rows.  keep_nonzero: no value but 0 gets code 0 (ReLU outputs)."""
     xp = _rows(x, "x")
     if x.numel() == 0:
         raise MMBError("checkpoint_rows: no rows")
@@ -883,7 +883,7 @@ def checkpoint_rows(x):
         q8 = Q8Rows(torch.empty(M, 32 * nb, dtype=torch.int8, device=x.device),
                     torch.empty(M, nb, dtype=torch.uint8, device=x.device), K)
         _, _, cp, sp = q8.args()
-        call("mmb_checkpoint_rows", M, K, DT[x.dtype], *xp, cp, sp, stream())
+        call("mmb_checkpoint_rows", M, K, DT[x.dtype], int(bool(keep_nonzero)), *xp, cp, sp, stream())
     return q8
 
 

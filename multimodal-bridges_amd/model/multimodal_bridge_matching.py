@@ -80,6 +80,10 @@ class MultiModalBridgeMatching(nn.Module):
         self.config = config
         # an encoder class with `raw_state = True` (the toy MultiModalMLP) takes the bridge state as it is: no embedder
         self.raw_state = bool(getattr(Encoder[config.encoder.name], "raw_state", False))
+        bits = getattr(config.encoder, "checkpoint_bits", None)
+        choices = getattr(Encoder[config.encoder.name], "checkpoint_bits_choices", (None,))
+        if bits not in choices:
+            raise ValueError(f"encoder.checkpoint_bits = {bits!r}: {config.encoder.name} takes one of {choices}")
         if not self.raw_state:
             self.embedder = MultiModalEmbedder(config)
         self.encoder = Encoder[config.encoder.name](config)

@@ -65,6 +65,7 @@ class EncoderConfig:
     dim_emb_discrete: Optional[int] = 0
     dim_emb_context_continuous: Optional[int] = 0
     dim_emb_context_discrete: Optional[int] = 0
+    checkpoint_bits: Optional[int] = None      # 8: activations kept in 8 bits for the reverse pass (particle transformer)
 
 
 @dataclass

@@ -455,6 +455,23 @@ def test_checkpoint_rows(dtype, M, K):
     assert torch.equal(back[:, 1:1 + K].cpu(), val.float()) and bool((back[:, 0] == 9).all()) and bool((back[:, 1 + K:] == 9).all())
 
 
+def test_checkpoint_keeps_nonzero_values():
+    """keep_nonzero: the sign of every value survives, whatever its size beside the block's largest; all else is the same."""
+    from mmb_hip import ops
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(60, 96, generator=g) * torch.exp2(torch.randint(-40, 4, (60, 96), generator=g).float())
+    x[:, ::7] = 0
+    x[0, :32], x[1, 32:64] = 0, 2.0 ** -149
+    plain, kept = ops.checkpoint_rows(x.cuda()), ops.checkpoint_rows(x.cuda(), keep_nonzero=True)
+    assert torch.equal(plain.steps, kept.steps)
+    y = ops.restore_rows(kept).cpu()
+    assert torch.equal(kept.codes.cpu().sign().float(), x.sign())
+    zero = plain.codes == 0
+    assert bool(zero.any()) and torch.equal(plain.codes[~zero], kept.codes[~zero])
+    step = torch.exp2(kept.steps.double().cpu() - 127).repeat_interleave(32, 1)
+    assert bool(((y.double() - x.double()).abs() < step).all())
+
+
 def test_checkpoint_extremes():
     from mmb_hip import ops
     big = torch.finfo(torch.float32).max

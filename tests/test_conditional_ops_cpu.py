@@ -83,10 +83,10 @@ def test_head_norm_bwd_refuses():
 
 
 @pytest.mark.parametrize("name,args,word", [
-    ("mmb_checkpoint_rows", (0, 8, 0, P, 8, P, P, None), b"positive"), ("mmb_checkpoint_rows", (4, 0, 0, P, 8, P, P, None), b"positive"),
-    ("mmb_checkpoint_rows", (4, 8, 5, P, 8, P, P, None), b"dtype"), ("mmb_checkpoint_rows", (4, 8, 0, None, 8, P, P, None), b"x is NULL"),
-    ("mmb_checkpoint_rows", (4, 8, 0, P, 7, P, P, None), b"leading"), ("mmb_checkpoint_rows", (4, 8, 0, P, 8, None, P, None), b"NULL"),
-    ("mmb_checkpoint_rows", (4, 8, 0, P, 8, P + 1, P, None), b"aligned"), ("mmb_restore_rows", (4, 8, 0, P, None, P, 8, None), b"NULL"),
+    ("mmb_checkpoint_rows", (0, 8, 0, 0, P, 8, P, P, None), b"positive"), ("mmb_checkpoint_rows", (4, 0, 0, 0, P, 8, P, P, None), b"positive"),
+    ("mmb_checkpoint_rows", (4, 8, 5, 0, P, 8, P, P, None), b"dtype"), ("mmb_checkpoint_rows", (4, 8, 0, 0, None, 8, P, P, None), b"x is NULL"),
+    ("mmb_checkpoint_rows", (4, 8, 0, 0, P, 7, P, P, None), b"leading"), ("mmb_checkpoint_rows", (4, 8, 0, 0, P, 8, None, P, None), b"NULL"),
+    ("mmb_checkpoint_rows", (4, 8, 0, 0, P, 8, P + 1, P, None), b"aligned"), ("mmb_restore_rows", (4, 8, 0, P, None, P, 8, None), b"NULL"),
     ("mmb_restore_rows", (4, 8, 0, P, P, None, 8, None), b"NULL"), ("mmb_restore_rows", (4, 8, 0, P, P, P, 7, None), b"leading"),
     ("mmb_restore_rows", (4, 8, 7, P, P, P, 8, None), b"dtype"),
     ("mmb_grad_weight_rows_q8", (4, 8, 0, 0, P, P, P, 8, P, 8, P, 0, P, 1 << 20, None), b"N in"),
