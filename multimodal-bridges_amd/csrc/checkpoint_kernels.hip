@@ -129,14 +129,15 @@ decode_kernel(int64_t M, int K, int nb, const int8_t* __restrict__ codes, const 
 }
 
 // ---- dW (N, K) = dZ^T (N, M) . Xhat (M, K), db (N) = column sums of dZ -------------------------------------------
-// A workgroup owns a 128 x BK tile of dW (BK = 128 or 256) over a range of rows and walks the range 32 rows at a time; four
-// waves compute 64 x BK/2 each.  dZ (in bf16 planes) and Xhat lie in LDS as they come, row by row; the matrix operands want
+// A workgroup owns a BN x BK tile of dW (128 x 128, 128 x 256 with four waves, 256 x 256 with eight) over a range of rows and
+// walks the range 32 rows at a time; a wave computes 64 x BK/2.  What a wave has to decode and move beside its products falls
+// with the tile's size.  dZ (in bf16 planes) and Xhat lie in LDS as they come, row by row; the matrix operands want
 // eight consecutive ROWS of one column, which the transposing LDS read supplies (four rows of 16 columns per 16 lanes), so
 // nothing is transposed in registers.  Row pitch 16 banks past a multiple of 64: the four rows of such a read do not meet.
 // Two buffers, one barrier a step; the rows of the step after next are in registers meanwhile.
 // The rows are split over workgroups to fill the chip; partial tiles are summed by a second launch in a fixed order (no
 // atomics: equal inputs give equal bits).
-constexpr int BN = 128, MS = 32;
+constexpr int MS = 32;
 constexpr int pitch_of(int cols) { return cols + 32; }
 
 template <typename T> struct Planes;
@@ -166,12 +167,13 @@ __device__ __forceinline__ u32x4 read_cols(const uint16_t* p, int pitch) {
   return r.v;
 }
 
-template <typename T, int BK>
+template <typename T, int BN, int BK>
 constexpr int gw_lds() { return 2 * MS * (Planes<T>::n * pitch_of(BN) + pitch_of(BK)) * 2; }
 
-template <typename T, int BK, bool VEC>
-__global__ void __launch_bounds__(256, 2) gw_kernel(GwArgs a) {
-  constexpr int PL = Planes<T>::n, PA = pitch_of(BN), PB = pitch_of(BK), NJ = BK / 64, XC = MS * BK / 16 / 256;
+template <typename T, int BN, int BK, bool VEC>
+__global__ void __launch_bounds__(2 * BN, 2) gw_kernel(GwArgs a) {
+  constexpr int NT = 2 * BN, NWN = BN / 64;
+  constexpr int PL = Planes<T>::n, PA = pitch_of(BN), PB = pitch_of(BK), NJ = BK / 64, XC = MS * BK / 16 / NT;
   extern __shared__ __attribute__((aligned(16))) uint16_t gw_sm[];
   constexpr int BUF = MS * (PL * PA + PB);
   const int tiles = a.nt * a.kt;
@@ -183,11 +185,11 @@ __global__ void __launch_bounds__(256, 2) gw_kernel(GwArgs a) {
   const bool sums = tile / a.nt == 0;              // the tiles of the first K window also sum dZ's columns
   const int64_t m0 = (int64_t)split * a.rows, m1 = min(a.M, m0 + a.rows);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
-  const int wn = (wave & 1) * 64, wk = (wave >> 1) * (BK / 2);
+  const int wn = wave % NWN * 64, wk = wave / NWN * (BK / 2);
   // transposing reads: lane j of 16 addresses row j >> 2, four columns from 4 (j & 3)
   const int tr_row = 8 * h + ((lane & 15) >> 2), tr_col = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-  // loads: dZ rows (tid >> 4) and + 16, eight columns; Xhat 16 codes a chunk
-  const int zr = threadIdx.x >> 4, zc = (threadIdx.x & 15) * 8;
+  // loads: dZ rows zr and zr + 16, eight columns; Xhat 16 codes a chunk
+  const int zr = threadIdx.x / (BN / 8), zc = threadIdx.x % (BN / 8) * 8;
   f32x16 acc[2][NJ];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(256, 2) gw_kernel(GwArgs a) {
     }
 #pragma unroll
     for (int j = 0; j < XC; ++j) {
-      const int it = threadIdx.x + 256 * j, c = (it % (BK / 16)) * 16;
+      const int it = threadIdx.x + NT * j, c = (it % (BK / 16)) * 16;
       const int64_t row = m + it / (BK / 16);
       cw[j] = u32x4{0u, 0u, 0u, 0u};
       sw[j] = 0u;
@@ -273,7 +275,7 @@ __global__ void __launch_bounds__(256, 2) gw_kernel(GwArgs a) {
     }
 #pragma unroll
     for (int j = 0; j < XC; ++j) {
-      const int it = threadIdx.x + 256 * j;
+      const int it = threadIdx.x + NT * j;
       uint16_t* dst = buf + MS * PL * PA + (it / (BK / 16)) * PB + (it % (BK / 16)) * 16;
       // code * step with the code as an unsigned byte, offset by 128: (u - 128) step, exact in one fused step
       const float st = step_of(sw[j]), off = -128.0f * st;
@@ -328,7 +330,7 @@ __global__ void __launch_bounds__(256, 2) gw_kernel(GwArgs a) {
         if (n < a.N && k < a.K) pw[(int64_t)n * a.K + k] = acc[i][j][r];
       }
   if (sums) {
-    float* red = reinterpret_cast<float*>(gw_sm);  // 16 row groups x 128 columns
+    float* red = reinterpret_cast<float*>(gw_sm);  // 16 row groups x BN columns
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) red[zr * BN + zc + i] = db[i];
@@ -369,19 +371,21 @@ gw_fold_kernel(int splits, int64_t nw, int N, int K, const float* __restrict__ p
   }
 }
 
-// Row ranges: enough workgroups for two on every CU, no range shorter than 8 steps, and no more partial sums than a quarter
-// of what the operands themselves hold (they are written and read once more).
+// Tile: 256 x 256 where both sides have more than 128 columns and it wastes little more than 128-wide tiles would.
+// Row ranges: enough workgroups for eight waves on every CU, no range shorter than 8 steps, and no more partial sums than a
+// quarter of what the operands themselves hold (they are written and read once more).
 struct GwPlan {
-  int bk, nt, kt, splits;
+  int bn, bk, nt, kt, splits;
   int64_t rows;
 };
 static GwPlan gw_plan(int64_t M, int N, int K) {
   GwPlan p;
   p.bk = K > 128 ? 256 : 128;
-  p.nt = (N + BN - 1) / BN;
+  p.bn = p.bk == 256 && N > 128 && (int64_t)(N + 255) / 256 * 256 * 4 <= (int64_t)(N + 127) / 128 * 128 * 5 ? 256 : 128;
+  p.nt = (N + p.bn - 1) / p.bn;
   p.kt = (K + p.bk - 1) / p.bk;
-  const int64_t tiles = (int64_t)p.nt * p.kt;
-  int64_t s = (512 + tiles - 1) / tiles;
+  const int64_t tiles = (int64_t)p.nt * p.kt, groups = p.bn == 256 ? 256 : 512;
+  int64_t s = (groups + tiles - 1) / tiles;
   const int64_t most = (M + 8 * MS - 1) / (8 * MS), fit = M * ((int64_t)K + 4 * N) / (32 * (int64_t)N * K) + 1;
   if (s > most) s = most;
   if (s > fit) s = fit;
@@ -414,10 +418,11 @@ static int decode(int64_t M, int K, const void* codes, const void* steps, void* 
   else decode_kernel<T, false><<<grid, 256, 0, st>>>(M, K, nb, (const int8_t*)codes, (const uint8_t*)steps, (T*)y, y_ld);
   return check_launch("mmb_restore_rows");
 }
-template <typename T, int BK, bool VEC>
+template <typename T, int BN, int BK, bool VEC>
 static int launch_gw(const GwArgs& a, hipStream_t st) {
-  constexpr int bytes = gw_lds<T, BK>();
-  auto kern = gw_kernel<T, BK, VEC>;
+  constexpr int bytes = gw_lds<T, BN, BK>();
+  static_assert(bytes <= 160 * 1024, "LDS");
+  auto kern = gw_kernel<T, BN, BK, VEC>;
   static PerDeviceOnce once;
   if (bytes > 64 * 1024 &&
       !once.run([&] { return hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess; })) {
@@ -426,16 +431,20 @@ static int launch_gw(const GwArgs& a, hipStream_t st) {
   }
   const int64_t blocks = (int64_t)(a.splits + 7) / 8 * 8 * a.nt * a.kt;
   MMB_REQUIRE(blocks <= 0x7fffffffLL, "mmb_grad_weight_rows_q8: %lld workgroups", (long long)blocks);
-  kern<<<(unsigned)blocks, 256, bytes, st>>>(a);
+  kern<<<(unsigned)blocks, 2 * BN, bytes, st>>>(a);
   return check_launch("mmb_grad_weight_rows_q8");
 }
+template <typename T, bool VEC>
+static int pick_tile(const GwArgs& a, const GwPlan& p, hipStream_t st) {
+  if (p.bn == 256) return launch_gw<T, 256, 256, VEC>(a, st);
+  return p.bk == 256 ? launch_gw<T, 128, 256, VEC>(a, st) : launch_gw<T, 128, 128, VEC>(a, st);
+}
 template <typename T>
-static int grad_weight(GwArgs& a, int bk, float* dW, int64_t dw_ld, float* db, int accumulate, hipStream_t st) {
+static int grad_weight(GwArgs& a, const GwPlan& p, float* dW, int64_t dw_ld, float* db, int accumulate, hipStream_t st) {
   const bool vec = a.N % 8 == 0 && ((uintptr_t)a.dz & 15) == 0 && a.dz_ld * (int64_t)sizeof(T) % 16 == 0;
   const int64_t nw = (int64_t)a.N * a.K, fold = (nw + a.N + 31) / 32;
   MMB_REQUIRE(fold <= 0x7fffffffLL, "mmb_grad_weight_rows_q8: dW of %lld values", (long long)nw);
-  int rc = bk == 256 ? (vec ? launch_gw<T, 256, true>(a, st) : launch_gw<T, 256, false>(a, st))
-                     : (vec ? launch_gw<T, 128, true>(a, st) : launch_gw<T, 128, false>(a, st));
+  int rc = vec ? pick_tile<T, true>(a, p, st) : pick_tile<T, false>(a, p, st);
   if (rc != MMB_OK) return rc;
   gw_fold_kernel<<<(unsigned)fold, 256, 0, st>>>(a.splits, nw, a.N, a.K, a.pw, a.pb, dW, dw_ld, db, accumulate);
   return check_launch("mmb_grad_weight_rows_q8 (fold)");
@@ -490,9 +499,9 @@ extern "C" int mmb_grad_weight_rows_q8(int64_t M, int K, int N, int dtype, const
   a.pw = (float*)workspace;
   a.pb = a.pw + (int64_t)a.splits * N * K;
   hipStream_t st = as_stream(stream);
-  if (dtype == MMB_DT_F32) return grad_weight<float>(a, p.bk, dW, dw_ld, db, accumulate, st);
-  if (dtype == MMB_DT_BF16) return grad_weight<__bf16>(a, p.bk, dW, dw_ld, db, accumulate, st);
-  if (dtype == MMB_DT_F16) return grad_weight<_Float16>(a, p.bk, dW, dw_ld, db, accumulate, st);
+  if (dtype == MMB_DT_F32) return grad_weight<float>(a, p, dW, dw_ld, db, accumulate, st);
+  if (dtype == MMB_DT_BF16) return grad_weight<__bf16>(a, p, dW, dw_ld, db, accumulate, st);
+  if (dtype == MMB_DT_F16) return grad_weight<_Float16>(a, p, dW, dw_ld, db, accumulate, st);
   set_error("mmb_grad_weight_rows_q8: unknown dtype %d", dtype);
   return MMB_ERR_INVALID_ARG;
 }
