@@ -134,10 +134,10 @@ decode_kernel(int64_t M, int K, int nb, const int8_t* __restrict__ codes, const 
 // with the tile's size.  dZ (in bf16 planes) and Xhat lie in LDS as they come, row by row; the matrix operands want
 // eight consecutive ROWS of one column, which the transposing LDS read supplies (four rows of 16 columns per 16 lanes), so
 // nothing is transposed in registers.  Row pitch 16 banks past a multiple of 64: the four rows of such a read do not meet.
-// Two buffers, one barrier a step; the rows of the step after next are in registers meanwhile.
+// Two buffers, one barrier a step; the rows of the two steps behind are on their way to registers meanwhile.
 // The rows are split over workgroups to fill the chip; partial tiles are summed by a second launch in a fixed order (no
 // atomics: equal inputs give equal bits).
-constexpr int MS = 32;
+constexpr int MS = 32;                            // rows of a step
 constexpr int pitch_of(int cols) { return cols + 32; }
 
 template <typename T> struct Planes;
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(2 * BN, 2) gw_kernel(GwArgs a) {
   const int wn = wave % NWN * 64, wk = wave / NWN * (BK / 2);
   // transposing reads: lane j of 16 addresses row j >> 2, four columns from 4 (j & 3)
   const int tr_row = 8 * h + ((lane & 15) >> 2), tr_col = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-  // loads: dZ rows zr and zr + 16, eight columns; Xhat 16 codes a chunk
+  // loads: dZ rows zr, zr + 16 .., eight columns; Xhat 16 codes a chunk
   const int zr = threadIdx.x / (BN / 8), zc = threadIdx.x % (BN / 8) * 8;
   f32x16 acc[2][NJ];
 #pragma unroll
@@ -199,63 +199,86 @@ __global__ void __launch_bounds__(2 * BN, 2) gw_kernel(GwArgs a) {
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
   float db[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   constexpr int ZW = sizeof(T) == 4 ? 8 : 4;       // words of eight elements
-  uint32_t zw[2][ZW];
-  u32x4 cw[XC];
-  uint32_t sw[XC];
-  auto fetch = [&](int64_t m) {
+  struct Step {                                    // one step's rows on their way from memory to LDS
+    uint32_t zw[MS / 16][ZW];
+    u32x4 cw[XC];
+    uint32_t sw[XC];
+  } steps[2];
+  // addresses: a uniform part that moves with the rows, and 32-bit offsets that stay.  Columns past the matrix read column 0
+  // instead: what they multiply into is not stored.
+  const int zcol = n0 + zc < a.N ? zc : 0;
+  const uint32_t zoff = (uint32_t)(zr * a.dz_ld + zcol) * (uint32_t)sizeof(T);
+  uint32_t coff[XC], soff[XC];
+  int crow_[XC];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int64_t row = m + zr + 16 * j;
-      const T* p = (const T*)a.dz + row * a.dz_ld + n0 + zc;
+  for (int j = 0; j < XC; ++j) {
+    const int it = threadIdx.x + NT * j, c = (it % (BK / 16)) * 16, cc = k0 + c < a.nb * 32 ? k0 + c : 0;
+    crow_[j] = it / (BK / 16);
+    coff[j] = (uint32_t)crow_[j] * (uint32_t)(a.nb * 32) + cc;
+    soff[j] = (uint32_t)crow_[j] * (uint32_t)a.nb + cc / 32;
+  }
+  auto fetch = [&](Step& st, int64_t m) {
+    auto &zw = st.zw;
+    auto &cw = st.cw;
+    auto &sw = st.sw;
+    const int left = (int)min((int64_t)MS, m1 - m);                         // rows of this step: fewer than MS in the last only
+    const char* zb = reinterpret_cast<const char*>((const T*)a.dz + m * a.dz_ld + n0);
+    const int8_t* cb = a.codes + m * (a.nb * 32);
+    const uint8_t* sb = a.steps + m * a.nb;
 #pragma unroll
-      for (int w = 0; w < ZW; ++w) zw[j][w] = 0u;
-      if (row < m1) {
-        if constexpr (VEC) {
-          if (n0 + zc < a.N) {
+    for (int j = 0; j < MS / 16; ++j) {
+      const bool in = left == MS || zr + 16 * j < left;
+      if constexpr (VEC) {
+        const char* p = zb + (int64_t)j * 16 * a.dz_ld * (int64_t)sizeof(T);
 #pragma unroll
-            for (int w = 0; w < ZW / 4; ++w) {
-              const u32x4 t = *reinterpret_cast<const u32x4*>(p + w * 4);
+        for (int w = 0; w < ZW / 4; ++w) {
+          const u32x4 t = in ? *reinterpret_cast<const u32x4*>(p + zoff + 16 * w) : u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-              for (int i = 0; i < 4; ++i) zw[j][4 * w + i] = t[i];
-            }
-          }
-        } else {
-          T t[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) t[i] = n0 + zc + i < a.N ? p[i] : (T)0.0f;
-          __builtin_memcpy(zw[j], t, sizeof(t));
+          for (int i = 0; i < 4; ++i) zw[j][4 * w + i] = t[i];
         }
+      } else {
+        const T* p = (const T*)a.dz + (m + zr + 16 * j) * a.dz_ld + n0 + zc;
+        T t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = in && n0 + zc + i < a.N ? p[i] : (T)0.0f;
+        __builtin_memcpy(zw[j], t, sizeof(t));
       }
     }
 #pragma unroll
     for (int j = 0; j < XC; ++j) {
-      const int it = threadIdx.x + NT * j, c = (it % (BK / 16)) * 16;
-      const int64_t row = m + it / (BK / 16);
-      cw[j] = u32x4{0u, 0u, 0u, 0u};
-      sw[j] = 0u;
-      if (row < m1 && k0 + c < a.nb * 32) {
-        cw[j] = *reinterpret_cast<const u32x4*>(a.codes + row * (a.nb * 32) + k0 + c);
-        sw[j] = a.steps[row * a.nb + (k0 + c) / 32];
-      }
+      const bool in = left == MS || crow_[j] < left;
+      cw[j] = in ? *reinterpret_cast<const u32x4*>(cb + coff[j]) : u32x4{0u, 0u, 0u, 0u};
+      sw[j] = in ? sb[soff[j]] : 0u;
     }
   };
-  auto put = [&](uint16_t* buf) {
+  auto put = [&](const Step& step, uint16_t* buf) {
+    const auto &zw = step.zw;
+    const auto &cw = step.cw;
+    const auto &sw = step.sw;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < MS / 16; ++j) {
       uint16_t* dst = buf + (zr + 16 * j) * PA + zc;
       float f[8];
-      if constexpr (sizeof(T) == 4) {
+      if (PL > 1 || sums) {
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(zw[j][i]);
-      } else {
-        T t[8];
-        __builtin_memcpy(t, zw[j], 16);
+          for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(zw[j][i]);
+        } else if constexpr (PL > 1) {
+          T t[8];
+          __builtin_memcpy(t, zw[j], 16);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = (float)t[i];
-      }
-      if (sums) {
+          for (int i = 0; i < 8; ++i) f[i] = (float)t[i];
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) db[i] += f[i];
+          for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(zw[j][i] << 16);
+            f[2 * i + 1] = __uint_as_float(zw[j][i] & 0xffff0000u);
+          }
+        }
+        if (sums) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) db[i] += f[i];
+        }
       }
       if constexpr (PL == 1) {
         *reinterpret_cast<u32x4*>(dst) = u32x4{zw[j][0], zw[j][1], zw[j][2], zw[j][3]};
@@ -277,30 +300,32 @@ __global__ void __launch_bounds__(2 * BN, 2) gw_kernel(GwArgs a) {
     for (int j = 0; j < XC; ++j) {
       const int it = threadIdx.x + NT * j;
       uint16_t* dst = buf + MS * PL * PA + (it / (BK / 16)) * PB + (it % (BK / 16)) * 16;
-      // code * step with the code as an unsigned byte, offset by 128: (u - 128) step, exact in one fused step
-      const float st = step_of(sw[j]), off = -128.0f * st;
+      const float st = step_of(sw[j]);
+      // code * step with the code as an unsigned byte, offset by 128: (u - 128) step, exact in one fused step -- unless
+      // 128 step leaves the range of a float
+      const bool huge = __any(sw[j] >= 248u);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        u32x4 w;
+        float x[8];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t u = cw[j][2 * q + i] ^ 0x80808080u;
-          const float x0 = fmaf((float)(u & 255u), st, off), x1 = fmaf((float)((u >> 8) & 255u), st, off),
-                      x2 = fmaf((float)((u >> 16) & 255u), st, off), x3 = fmaf((float)(u >> 24), st, off);
-          w[2 * i] = __builtin_amdgcn_perm(__float_as_uint(x1), __float_as_uint(x0), 0x07060302u);
-          w[2 * i + 1] = __builtin_amdgcn_perm(__float_as_uint(x3), __float_as_uint(x2), 0x07060302u);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[4 * i + k] = fmaf((float)((u >> (8 * k)) & 255u), st, -128.0f * st);
         }
+        if (huge) {
+          asm volatile("");                        // (a branch: not computed beside the above)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = (float)(int8_t)(cw[j][2 * q + (i >> 2)] >> (8 * (i & 3))) * st;
+        }
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(__float_as_uint(x[2 * i + 1]), __float_as_uint(x[2 * i]), 0x07060302u);
         *reinterpret_cast<u32x4*>(dst + 8 * q) = w;
       }
     }
   };
-  fetch(m0);
-  int p = 0;
-  for (int64_t m = m0; m < m1; m += MS, p ^= 1) {
-    uint16_t* buf = gw_sm + p * BUF;
-    put(buf);
-    if (m + MS < m1) fetch(m + MS);
-    __syncthreads();                               // (the other buffer's readers passed here after their products)
+  auto products = [&](const uint16_t* buf) {
     const uint16_t* As = buf + tr_row * PA + wn + tr_col;
     const uint16_t* Bs = buf + MS * PL * PA + tr_row * PB + wk + tr_col;
 #pragma unroll
@@ -317,6 +342,20 @@ __global__ void __launch_bounds__(2 * BN, 2) gw_kernel(GwArgs a) {
           for (int j = 0; j < NJ; ++j)
             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af, __builtin_bit_cast(bf16x8, bf[j]), acc[i][j], 0, 0, 0);
         }
+    }
+  };
+  // two steps' rows are on their way while one is worked on; of the two LDS buffers one is written while the other is read
+  fetch(steps[0], m0);
+  if (m0 + MS < m1) fetch(steps[1], m0 + MS);
+  for (int64_t m = m0; m < m1; m += 2 * MS) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int64_t at = m + p * MS;
+      if (at >= m1) break;
+      put(steps[p], gw_sm + p * BUF);
+      if (at + 2 * MS < m1) fetch(steps[p], at + 2 * MS);
+      __syncthreads();                             // (the other buffer's readers passed here after their products)
+      products(gw_sm + p * BUF);
     }
   }
   float* pw = a.pw + (int64_t)split * a.N * a.K;
@@ -441,7 +480,7 @@ static int pick_tile(const GwArgs& a, const GwPlan& p, hipStream_t st) {
 }
 template <typename T>
 static int grad_weight(GwArgs& a, const GwPlan& p, float* dW, int64_t dw_ld, float* db, int accumulate, hipStream_t st) {
-  const bool vec = a.N % 8 == 0 && ((uintptr_t)a.dz & 15) == 0 && a.dz_ld * (int64_t)sizeof(T) % 16 == 0;
+  const bool vec = a.N % 8 == 0 && ((uintptr_t)a.dz & 15) == 0 && a.dz_ld * (int64_t)sizeof(T) % 16 == 0 && a.dz_ld < (1 << 24);
   const int64_t nw = (int64_t)a.N * a.K, fold = (nw + a.N + 31) / 32;
   MMB_REQUIRE(fold <= 0x7fffffffLL, "mmb_grad_weight_rows_q8: dW of %lld values", (long long)nw);
   int rc = vec ? pick_tile<T, true>(a, p, st) : pick_tile<T, false>(a, p, st);

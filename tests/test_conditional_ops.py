@@ -516,6 +516,21 @@ def test_grad_weight_rows_q8(dtype, M, K, N):
     assert none is None and torch.equal(only, dW)
 
 
+def test_grad_weight_rows_q8_extremes():
+    """Codes of the largest floats and of subnormals; a block that was not finite spoils its own columns of dW and no others."""
+    from mmb_hip import ops
+    x = torch.zeros(40, 96)
+    x[:, 0], x[:, 1], x[:, 33] = torch.finfo(torch.float32).max, -1.0e38, 2.0 ** -140
+    dz = torch.full((40, 8), 2.0 ** -20)
+    q8 = ops.checkpoint_rows(x.cuda())
+    dW, _ = ops.grad_weight_rows_q8(q8, dz.cuda())
+    v = ops.restore_rows(q8).double().cpu()
+    within(dW, dz.double().t() @ v, 44 * E * (dz.double().abs().t() @ v.abs()) + 2.0 ** -149, "dW")
+    x[7, 70] = math.nan
+    dW, _ = ops.grad_weight_rows_q8(ops.checkpoint_rows(x.cuda()), dz.cuda())
+    assert dW[:, 64:96].isnan().all() and dW[:, :64].isfinite().all()
+
+
 # ------------------------------------------------------------------------------------------------ together
 class Layer:
     """One conditional attention layer as a training step runs it: project, norm and rotate q and k, attend, project; the
