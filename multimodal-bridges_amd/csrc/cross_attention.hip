@@ -71,6 +71,7 @@ __global__ void __launch_bounds__(64 * NW, 2) fwd_kernel(FwdArgs a) {
   const int row = r0 + (SPLIT ? 0 : wave * 32) + col;
   int n = -1, gi = 0;
   const bool live = row < R && rt.locate(row, sh.Nq, mq != nullptr, n, gi);
+  const bool wave_live = __any(live);
   const int head = hk * sh.g + gi;
 
   u32x4 qf[DP / (2 * Traits<T>::EPC)];
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(64 * NW, 2) fwd_kernel(FwdArgs a) {
     // overlaps with this tile's products
     kr.template load<VEC>(tid, nn, sh.D, [&](int i) { return kb + (int64_t)keys.slot(i) * a.k_ld; });
     vr.template load<VEC>(tid, nn, sh.D, [&](int i) { return vb + (int64_t)keys.slot(i) * a.v_ld; });
-    attend<T, DP, TK>(Ks, Vs, nk, qf, c, m, l, acc);
+    if (wave_live) attend<T, DP, TK>(Ks, Vs, nk, qf, c, m, l, acc);         // (a wave without rows only helps to load)
     nk = nn;
   }
   l += __shfl_xor(l, 32);

@@ -44,7 +44,11 @@ def i32(t, name="tensor"):
 
 
 def stream():
-    return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(torch.cuda.current_device())
+
+
+# the address of a device's current stream, without a Stream object around it where torch offers that (2 us of every call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _fl(v):
@@ -683,18 +687,21 @@ def _rows(t, name, dtype=None, rows=None, width=None, device=None):
         raise MMBError(f"{name}: expected a 2-D tensor of rows")
     if not t.is_cuda:
         raise MMBError(f"{name}: tensor lives on {t.device}; the HIP path has no CPU fallback")
-    if t.dtype not in DT or (dtype is not None and t.dtype != dtype):
+    if t.dtype != dtype if dtype is not None else t.dtype not in DT:
         raise MMBError(f"{name}: expected dtype {dtype or 'float32, bfloat16 or float16'}, got {t.dtype}")
     if device is not None and t.device != device:
         raise MMBError(f"{name}: tensor lives on {t.device}, the call's other tensors on {device}")
-    if (rows is not None and t.shape[0] != rows) or (width is not None and t.shape[1] != width):
+    m, n = t.shape
+    if (rows is not None and m != rows) or (width is not None and n != width):
         raise MMBError(f"{name}: expected {rows if rows is not None else '(any)'} rows of "
-                       f"{width if width is not None else '(any)'}, got {tuple(t.shape)}")
-    if t.stride(1) != 1 and t.shape[1] > 1:
+                       f"{width if width is not None else '(any)'}, got {(m, n)}")
+    ld, inner = t.stride()
+    if inner != 1 and n > 1:
         raise MMBError(f"{name}: unit inner stride required")
-    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    if ld < t.shape[1]:
-        raise MMBError(f"{name}: rows overlap (row stride {ld}, width {t.shape[1]})")
+    if m <= 1:
+        ld = n
+    elif ld < n:
+        raise MMBError(f"{name}: rows overlap (row stride {ld}, width {n})")
     return t.data_ptr(), ld
 
 

@@ -127,6 +127,9 @@ SHAPES = [  # B, Nq, Nk, nh, nkv, D, masked
     (8, 100, 96, 2, 1, 33, True),                               # odd head width: scalar loads
     (2, 130, 70, 3, 3, 1, False),
     (4, 5, 600, 4, 4, 8, True),
+    (5, 2, 300, 15, 3, 16, True),                               # few queries: the heads of a group share tiles
+    (3, 9, 130, 20, 2, 32, True),
+    (2, 1, 100, 70, 1, 8, False),
     (64, 150, 128, 4, 4, 16, True),                             # many small clouds: their keys stay in LDS
     (70, 40, 50, 8, 4, 32, True),
     (128, 16, 20, 4, 2, 64, True),
