@@ -223,12 +223,14 @@ struct Plan {
   bool split;
   int nw, tiles, nsplit, chunk;
 };
-// Team form: 32 rows a wave, as many waves (1, 2, 4) as a cloud's rows fill.  Split form when the team form would put
+// Team form: 32 rows a wave, as many waves (1, 2, 4) as a cloud's rows fill, eight where those still give every CU two
+// workgroups: the more waves share a tile, the less of it each has to load (4096 x 5000 slots, bf16: 373 us with eight, 424
+// with four; 2047 x 4099, where eight would leave CUs idle: 325 against 298).  Split form when the team form would put
 // fewer than one workgroup on each of the 256 CUs, or one 32-row tile holds all rows, and there are keys to split.
 static Plan fwd_plan(const Shape& s) {
   const int64_t R = (int64_t)s.g * s.Nq, pairs = (int64_t)s.B * s.nkv;
   Plan p;
-  p.nw = R > 64 ? 4 : R > 32 ? 2 : 1;
+  p.nw = R > 128 && pairs * ((R + 255) / 256) >= 512 ? 8 : R > 64 ? 4 : R > 32 ? 2 : 1;
   p.tiles = (int)((R + 32 * p.nw - 1) / (32 * p.nw));
   p.nsplit = 1;
   p.chunk = s.Nk;
@@ -274,6 +276,7 @@ static int pick_nw(const Plan& p, const FwdArgs& a, hipStream_t st) {
   // keys per tile: 64 in 16 bits (two K and V tiles of a 128-wide head: 64 KB), 32 in float (68 KB)
   constexpr int TK = sizeof(T) == 2 ? 64 : 32;
   if (p.split) return launch_fwd<T, DP, 4, 32, true, VEC>(a, st);
+  if (p.nw == 8) return launch_fwd<T, DP, 8, TK, false, VEC>(a, st);
   if (p.nw == 4) return launch_fwd<T, DP, 4, TK, false, VEC>(a, st);
   if (p.nw == 2) return launch_fwd<T, DP, 2, TK, false, VEC>(a, st);
   return launch_fwd<T, DP, 1, 32, false, VEC>(a, st);

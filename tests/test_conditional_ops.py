@@ -137,6 +137,7 @@ SHAPES = [  # B, Nq, Nk, nh, nkv, D, masked
     (256, 20, 40, 1, 1, 128, False),
     (66, 17, 200, 4, 4, 21, True),
     (500, 18, 1, 2, 2, 8, False),
+    (256, 130, 150, 2, 2, 128, True),                           # eight waves share a tile
 ]
 
 
