@@ -7,7 +7,8 @@
 // so a single token with g heads reads its keys once.
 //
 // Two forms of one kernel body:
-//   team    NW waves of one workgroup share every key tile through LDS, each owns 32 rows;
+//   team    NW waves of one workgroup share every key tile through LDS, each owns 32 rows; many keys of few clouds go in two
+//           ranges to two workgroups, whose results a second launch joins;
 //   split   every wave walks its own range of keys with its own LDS tiles (no workgroup barrier while it runs); the
 //           four partial sums of a workgroup are joined in LDS, those of several workgroups by a second launch.  For a
 //           few rows against many keys, where the team form would leave most of the chip idle.
@@ -25,8 +26,9 @@ struct FwdArgs {
   float scale;
   void* out;
   float* lse;
-  float* part;                                    // split form with several workgroups per tile: partial results
-  int tiles, nsplit, chunk;                       // row tiles per (cloud, key head); key splits; keys per wave (split form)
+  float* part;                                    // key splits: partial results of every 32 rows
+  bool vec;
+  int tiles, nsplit, chunk;                       // row tiles per (cloud, key head); key splits; keys of one (split form: of one wave)
   GridMap map;
 };
 
@@ -83,8 +85,8 @@ __global__ void __launch_bounds__(64 * NW, 2) fwd_kernel(FwdArgs a) {
   const float c = a.scale * kLog2e;
 
   int lo = 0, hi = sh.Nk;
-  if constexpr (SPLIT) {
-    lo = (int)min((int64_t)sh.Nk, (int64_t)(split * NW + wave) * a.chunk);
+  if (SPLIT || a.nsplit > 1) {
+    lo = (int)min((int64_t)sh.Nk, (int64_t)(SPLIT ? split * NW + wave : split) * a.chunk);
     hi = (int)min((int64_t)sh.Nk, (int64_t)lo + a.chunk);
   }
   T* tiles = reinterpret_cast<T*>(lds + team * TILE);
@@ -170,13 +172,27 @@ __global__ void __launch_bounds__(64 * NW, 2) fwd_kernel(FwdArgs a) {
     if (a.lse && threadIdx.x < 32)
       a.lse[((int64_t)b * sh.nh + head2) * sh.Nq + n2] = L == 0.0f ? -INFINITY : M * a.scale + logf(L);
   } else {
+    if (a.nsplit > 1) {                           // this range's sums of the wave's 32 rows
+      if (!wave_live) return;
+      float* p = a.part + ((int64_t)((pair * a.tiles + tile) * NW + wave) * a.nsplit + split) * (32 * (DP + 2));
+      if (h == 0) {
+        p[col] = m;
+        p[32 + col] = l;
+      }
+#pragma unroll
+      for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[64 + (32 * t + crow(r, h)) * 32 + col] = acc[t][r];
+      return;
+    }
     if (!live) return;
     store_col<T, DP, VEC>((T*)a.out + ((int64_t)b * sh.Nq + n) * a.out_ld + (int64_t)head * sh.D, acc, l == 0.0f ? 0.0f : 1.0f / l, sh.D);
     if (a.lse && h == 0) a.lse[((int64_t)b * sh.nh + head) * sh.Nq + n] = l == 0.0f ? -INFINITY : m * a.scale + logf(l);
   }
 }
 
-// joins the key splits of one row tile; workgroup = (pair, tile), 32 rows x 8 features at a time
+// joins the key splits of 32 rows; workgroup = (pair, 32-row tile), a thread has an eighth of a row's features.  a.tiles: 32-row
+// tiles.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) fwd_join_kernel(FwdArgs a) {
   __shared__ int qlist[34];
@@ -197,6 +213,7 @@ __global__ void __launch_bounds__(256) fwd_join_kernel(FwdArgs a) {
   float M = -INFINITY;
   for (int s = 0; s < a.nsplit; ++s) M = fmaxf(M, p[(int64_t)s * 32 * (DP + 2) + rr]);
   const float Ms = M == -INFINITY ? 0.0f : M;
+  const int d0 = (threadIdx.x >> 5) * (DP / 8);
   float L = 0.0f, o[DP / 8];
 #pragma unroll
   for (int i = 0; i < DP / 8; ++i) o[i] = 0.0f;
@@ -205,14 +222,22 @@ __global__ void __launch_bounds__(256) fwd_join_kernel(FwdArgs a) {
     const float f = __builtin_amdgcn_exp2f((ps[rr] - Ms) * c);
     L += f * ps[32 + rr];
 #pragma unroll
-    for (int i = 0; i < DP / 8; ++i) o[i] += f * ps[64 + (i * 8 + (threadIdx.x >> 5)) * 32 + rr];
+    for (int i = 0; i < DP / 8; ++i) o[i] += f * ps[64 + (d0 + i) * 32 + rr];
   }
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   T* op = (T*)a.out + ((int64_t)b * sh.Nq + n) * a.out_ld + (int64_t)head * sh.D;
+  T v[DP / 8];
 #pragma unroll
-  for (int i = 0; i < DP / 8; ++i) {
-    const int d = i * 8 + (threadIdx.x >> 5);
-    if (d < sh.D) op[d] = round_to<T>(o[i] * inv);
+  for (int i = 0; i < DP / 8; ++i) v[i] = round_to<T>(o[i] * inv);
+  if (a.vec) {                                    // (rows 16-byte aligned, D a multiple of a chunk)
+    constexpr int W = 4;                          // four elements at a time: every DP / 8 is a multiple
+#pragma unroll
+    for (int i = 0; i < DP / 8; i += W)
+      if (d0 + i < sh.D) __builtin_memcpy(__builtin_assume_aligned(op + d0 + i, W * sizeof(T)), v + i, W * sizeof(T));
+  } else {
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i)
+      if (d0 + i < sh.D) op[d0 + i] = v[i];
   }
   if (a.lse && threadIdx.x < 32)
     a.lse[((int64_t)b * sh.nh + head) * sh.Nq + n] = L == 0.0f ? -INFINITY : M * a.scale + logf(L);
@@ -222,6 +247,9 @@ __global__ void __launch_bounds__(256) fwd_join_kernel(FwdArgs a) {
 struct Plan {
   bool split;
   int nw, tiles, nsplit, chunk;
+  int64_t part_bytes(const Shape& s) const {      // partial sums of every 32 rows and key range
+    return nsplit > 1 ? (int64_t)s.B * s.nkv * tiles * (split ? 1 : nw) * nsplit * 32 * (pad_width(s.D) + 2) * 4 : 0;
+  }
 };
 // Team form: 32 rows a wave, as many waves (1, 2, 4) as a cloud's rows fill, eight where those still give every CU two
 // workgroups: the more waves share a tile, the less of it each has to load (4096 x 5000 slots, bf16: 373 us with eight, 424
@@ -244,6 +272,12 @@ static Plan fwd_plan(const Shape& s) {
     if (p.nsplit < 1) p.nsplit = 1;
     p.chunk = (s.Nk + p.nsplit * 4 - 1) / (p.nsplit * 4);
     p.chunk = (p.chunk + 31) / 32 * 32;
+  } else if (p.nw == 4 && s.Nk >= 2560 && pairs * p.tiles < 512) {
+    // the team form alone leaves CUs with one workgroup, whose four waves do not hide each other's latencies: the keys in two
+    // ranges and a second launch that joins them (2047 x 4099 slots, 16 heads on 8, fp16, D = 64: 79 us with two ranges, 93
+    // with one; masked 57, 72; bf16, D = 128: 115, 157; 2048 keys: 50, 47; two such clouds, masked: the same within 3 %)
+    p.nsplit = 2;
+    p.chunk = ((s.Nk + 1) / 2 + 63) / 64 * 64;
   }
   return p;
 }
@@ -264,8 +298,10 @@ static int launch_fwd(const FwdArgs& a, hipStream_t st) {
   }
   kern<<<dim3((unsigned)a.map.blocks()), dim3(64 * NW), bytes, st>>>(a);
   int rc = check_launch("mmb_cross_attention_fwd");
-  if (rc == MMB_OK && SPLIT && a.nsplit > 1) {
-    fwd_join_kernel<T, DP><<<dim3((unsigned)(a.sh.B * a.sh.nkv * a.tiles)), dim3(256), 0, st>>>(a);
+  if (rc == MMB_OK && a.nsplit > 1) {
+    FwdArgs j = a;
+    j.tiles = a.tiles * (SPLIT ? 1 : NW);
+    fwd_join_kernel<T, DP><<<dim3((unsigned)(j.sh.B * j.sh.nkv * j.tiles)), dim3(256), 0, st>>>(j);
     rc = check_launch("mmb_cross_attention_fwd (join)");
   }
   return rc;
@@ -315,8 +351,7 @@ extern "C" int mmb_cross_attention_workspace(int B, int Nq, int Nk, int nheads, 
     *bytes_host = (int64_t)B * nheads * Nq * 4;
     return MMB_OK;
   }
-  const Plan p = fwd_plan(s);
-  *bytes_host = p.nsplit > 1 && !resident_fits(s, dtype, false) && !jets_fit(s, dtype, false) ? (int64_t)B * nheads_kv * p.tiles * p.nsplit * 32 * (pad_width(D) + 2) * 4 : 0;
+  *bytes_host = resident_fits(s, dtype, false) || jets_fit(s, dtype, false) ? 0 : fwd_plan(s).part_bytes(s);
   return MMB_OK;
 }
 
@@ -339,10 +374,10 @@ extern "C" int mmb_cross_attention_fwd(int B, int Nq, int Nk, int nheads, int nh
   if (resident_fits(s, dtype, false))
     return resident_fwd(s, dtype, vec, q, q_ld, k, k_ld, v, v_ld, maskf_q, maskf_k, scale, out, out_ld, lse, as_stream(stream));
   const Plan p = fwd_plan(s);
-  const int64_t need = p.nsplit > 1 ? (int64_t)B * nheads_kv * p.tiles * p.nsplit * 32 * (pad_width(D) + 2) * 4 : 0;
+  const int64_t need = p.part_bytes(s);
   MMB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "mmb_cross_attention_fwd: workspace of %lld bytes needed, got %lld",
               (long long)need, (long long)(workspace ? workspace_bytes : 0));
-  FwdArgs a = {s, q, k, v, q_ld, k_ld, v_ld, out_ld, maskf_q, maskf_k, scale, out, lse, (float*)workspace, p.tiles, p.nsplit, p.chunk,
+  FwdArgs a = {s, q, k, v, q_ld, k_ld, v_ld, out_ld, maskf_q, maskf_k, scale, out, lse, (float*)workspace, vec, p.tiles, p.nsplit, p.chunk,
                grid_map(B, nheads_kv, p.tiles * p.nsplit)};
   MMB_REQUIRE(a.map.blocks() <= 0x7fffffffLL, "mmb_cross_attention_fwd: %lld workgroups", (long long)a.map.blocks());
   hipStream_t st = as_stream(stream);

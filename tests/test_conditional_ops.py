@@ -138,6 +138,8 @@ SHAPES = [  # B, Nq, Nk, nh, nkv, D, masked
     (66, 17, 200, 4, 4, 21, True),
     (500, 18, 1, 2, 2, 8, False),
     (256, 130, 150, 2, 2, 128, True),                           # eight waves share a tile
+    (65, 66, 2562, 4, 4, 16, True),                             # keys in two ranges
+    (65, 33, 2561, 8, 4, 40, False),
 ]
 
 
