@@ -336,6 +336,14 @@ int check_shape(const char* who, int B, int Nq, int Nk, int nh, int nkv, int D, 
   return MMB_OK;
 }
 
+int check_outputs(const char* who, const void* const* outs, int no, const void* const* ins, int ni) {
+  for (int i = 0; i < no; ++i) {
+    for (int j = 0; j < ni; ++j) MMB_REQUIRE(outs[i] != ins[j], "%s: an output is the same memory as an input", who);
+    for (int j = 0; j < i; ++j) MMB_REQUIRE(outs[i] != outs[j], "%s: two outputs are the same memory", who);
+  }
+  return MMB_OK;
+}
+
 }  // namespace xattn
 }  // namespace mmb
 
@@ -368,15 +376,18 @@ extern "C" int mmb_cross_attention_fwd(int B, int Nq, int Nk, int nheads, int nh
   const int es = dtype == MMB_DT_F32 ? 4 : 2;
   const bool vec = D * es % 16 == 0 && chunk_aligned(q, q_ld, es) && chunk_aligned(k, k_ld, es) && chunk_aligned(v, v_ld, es) &&
                    chunk_aligned(out, out_ld, es);
-  if (jets_fit(s, dtype, false))
-    return jets_fwd(s, vec, (const float*)q, q_ld, (const float*)k, k_ld, (const float*)v, v_ld, maskf_q, maskf_k, scale, (float*)out, out_ld,
-                    lse, as_stream(stream));
-  if (resident_fits(s, dtype, false))
-    return resident_fwd(s, dtype, vec, q, q_ld, k, k_ld, v, v_ld, maskf_q, maskf_k, scale, out, out_ld, lse, as_stream(stream));
+  const bool jets = jets_fit(s, dtype, false), resident = resident_fits(s, dtype, false);
   const Plan p = fwd_plan(s);
-  const int64_t need = p.part_bytes(s);
+  const int64_t need = jets || resident ? 0 : p.part_bytes(s);
   MMB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "mmb_cross_attention_fwd: workspace of %lld bytes needed, got %lld",
               (long long)need, (long long)(workspace ? workspace_bytes : 0));
+  const void *outs[] = {out}, *ins[] = {q, k, v};
+  if (int rc = check_outputs("mmb_cross_attention_fwd", outs, 1, ins, 3)) return rc;
+  if (jets)
+    return jets_fwd(s, vec, (const float*)q, q_ld, (const float*)k, k_ld, (const float*)v, v_ld, maskf_q, maskf_k, scale, (float*)out, out_ld,
+                    lse, as_stream(stream));
+  if (resident)
+    return resident_fwd(s, dtype, vec, q, q_ld, k, k_ld, v, v_ld, maskf_q, maskf_k, scale, out, out_ld, lse, as_stream(stream));
   FwdArgs a = {s, q, k, v, q_ld, k_ld, v_ld, out_ld, maskf_q, maskf_k, scale, out, lse, (float*)workspace, vec, p.tiles, p.nsplit, p.chunk,
                grid_map(B, nheads_kv, p.tiles * p.nsplit)};
   MMB_REQUIRE(a.map.blocks() <= 0x7fffffffLL, "mmb_cross_attention_fwd: %lld workgroups", (long long)a.map.blocks());

@@ -391,6 +391,8 @@ extern "C" int mmb_cross_attention_bwd(int B, int Nq, int Nk, int nheads, int nh
   const int64_t need = (int64_t)B * nheads * Nq * 4;
   MMB_REQUIRE(workspace && workspace_bytes >= need, "mmb_cross_attention_bwd: workspace of %lld bytes needed, got %lld",
               (long long)need, (long long)(workspace ? workspace_bytes : 0));
+  const void *outs[] = {dq, dk, dv}, *ins[] = {q, k, v, out, dout};
+  if (int rc = check_outputs("mmb_cross_attention_bwd", outs, 3, ins, 5)) return rc;
   BwdArgs a = {{B, Nq, Nk, nheads, nheads_kv, D, nheads / nheads_kv}, q, k, v, out, dout, q_ld, k_ld, v_ld, out_ld, dout_ld,
                dq_ld, dk_ld, dv_ld, maskf_q, maskf_k, lse, scale, dq, dk, dv, (float*)workspace, false, false, 0, 0, {}, {}, 0};
   const int es = dtype == MMB_DT_F32 ? 4 : 2;

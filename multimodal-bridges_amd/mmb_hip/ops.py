@@ -695,6 +695,8 @@ def _rows(t, name, dtype=None, rows=None, width=None, device=None):
     if (rows is not None and m != rows) or (width is not None and n != width):
         raise MMBError(f"{name}: expected {rows if rows is not None else '(any)'} rows of "
                        f"{width if width is not None else '(any)'}, got {(m, n)}")
+    if n >= 2 ** 31:
+        raise MMBError(f"{name}: rows of {n} elements, must stay below 2^31")
     ld, inner = t.stride()
     if inner != 1 and n > 1:
         raise MMBError(f"{name}: unit inner stride required")
@@ -734,6 +736,8 @@ def _xattn_args(q, k, v, B, nheads, nheads_kv, scale):
     vp = _rows(v, "v", q.dtype, k.shape[0], nkv * D, q.device)
     if k.shape[0] % B or k.shape[0] == 0:
         raise MMBError(f"cross_attention: {k.shape[0]} key rows are not {B} clouds")
+    if max(B, q.shape[0] // B, k.shape[0] // B) >= 2 ** 31:
+        raise MMBError(f"cross_attention: {B} clouds of {q.shape[0] // B} and {k.shape[0] // B} slots: counts must stay below 2^31")
     scale = D ** -0.5 if scale is None else float(scale)
     return nkv, D, q.shape[0] // B, k.shape[0] // B, scale, qp + kp + vp
 
@@ -765,7 +769,7 @@ def cross_attention_fwd(q, k, v, B, nheads, nheads_kv=None, mq=None, mk=None, sc
     q (B*Nq, nheads*D); k, v (B*Nk, nheads_kv*D), e.g. column slices of one projection's rows; float32, bfloat16 or float16.
     nheads_kv divides nheads: groups of query heads share a key head.  mq, mk: MaskInfo of the query / key slots (None: all
     real); padded keys take no part, padded queries get zero rows (whatever the padded rows hold), as does a query without a
-    key.  scale: D ** -0.5 by default.  Returns out (B*Nq, nheads*D), with want_lse (out, lse (B, nheads, Nq) float32)."""
+    key.  scale: D ** -0.5 by default.  out shares no memory with q, k, v.  Returns out (B*Nq, nheads*D), with want_lse (out, lse (B, nheads, Nq) float32)."""
     nkv, D, Nq, Nk, scale, ptrs = _xattn_args(q, k, v, B, nheads, nheads_kv, scale)
     dev = q.device
     with _on(dev):
@@ -783,7 +787,8 @@ def cross_attention_fwd(q, k, v, B, nheads, nheads_kv=None, mq=None, mk=None, sc
 def cross_attention_bwd(q, k, v, out, dout, lse, B, nheads, nheads_kv=None, mq=None, mk=None, scale=None, dq=None, dk=None,
                         dv=None):
     """(dq, dk, dv) of cross_attention_fwd from its out, lse and dout = d loss / d out; the arguments as there.  Gradients
-    are overwritten (dq, dk, dv given: rows that may be column slices), zero for padded slots.  Equal inputs, equal bits."""
+    are overwritten (dq, dk, dv given: rows that may be column slices, of memory that no input and no other gradient shares),
+    zero for padded slots.  Equal inputs, equal bits."""
     nkv, D, Nq, Nk, scale, ptrs = _xattn_args(q, k, v, B, nheads, nheads_kv, scale)
     dev = q.device
     with _on(dev):

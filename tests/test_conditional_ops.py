@@ -680,3 +680,13 @@ def test_two_calls_at_once():
     torch.cuda.synchronize()
     for g, w in zip(got, want):
         assert all(torch.equal(g[n], w[n]) for n in w)
+
+
+def test_counts_beyond_32_bits_are_refused():
+    from mmb_hip import ops, MMBError
+    x, kv = torch.empty(2 ** 32 + 4, 1, dtype=torch.bfloat16, device="cuda"), torch.zeros(4, 1, dtype=torch.bfloat16, device="cuda")
+    for q, k in ((x, kv), (kv, x)):
+        with pytest.raises(MMBError, match="2\\^31"):
+            ops.cross_attention_fwd(q, k, k, 1, 1)
+    with pytest.raises(MMBError, match="2\\^31"):
+        ops.checkpoint_rows(x.view(1, -1))

@@ -117,3 +117,20 @@ def test_tensor_layer_refuses_host_tensors_and_wrong_shapes():
         ops.Q8Rows(torch.zeros(2, 32, dtype=torch.int8), torch.zeros(3, 1, dtype=torch.uint8), 32)
     with pytest.raises(MMBError, match="multiple"):
         ops.cross_attention_fwd(x, x, x, 2, 3, 2)
+
+
+def test_cross_attention_refuses_outputs_over_inputs():
+    at = [0x10000 * (i + 1) for i in range(9)]
+    for i in range(3):
+        rc, msg = fwd(q=at[0], k=at[1], v=at[2], out=at[i])
+        assert rc == -1 and b"an output is the same memory as an input" in msg
+    names = ("q", "k", "v", "out", "dout", "dq", "dk", "dv")
+    def bwd(over):
+        p = dict(zip(names, at), **over)
+        return rc_of("mmb_cross_attention_bwd", 1, 4, 8, 2, 1, 16, 1, p["q"], 32, p["k"], 16, p["v"], 16, None, None, 0.25, p["out"], 32,
+                     p["dout"], 32, at[8], p["dq"], 32, p["dk"], 16, p["dv"], 16, P, 1 << 20, None)
+    for g in names[5:]:
+        for i, other in enumerate(names):
+            if other != g:
+                rc, msg = bwd({g: at[i]})
+                assert rc == -1 and b"same memory" in msg, (g, other, msg)
