@@ -332,6 +332,9 @@ int check_shape(const char* who, int B, int Nq, int Nk, int nh, int nkv, int D, 
   MMB_REQUIRE(D > 0 && D <= 128, "%s: head width must be 1..128 (got %d)", who, D);
   MMB_REQUIRE(dtype == MMB_DT_F32 || dtype == MMB_DT_BF16 || dtype == MMB_DT_F16, "%s: unknown dtype %d", who, dtype);
   MMB_REQUIRE(scale > 0.0f && std::isfinite(scale), "%s: scale must be positive and finite", who);
+  // 32-bit slot counters run a compaction step past the last slot, and the plan's divisions round up
+  constexpr int most = 0x7fffffff - 4096;
+  MMB_REQUIRE(Nk <= most, "%s: Nk must not exceed 2^31 - 4097 (got %d)", who, Nk);
   MMB_REQUIRE((int64_t)nh * Nq <= (1 << 30) && (int64_t)B * nh <= (1 << 30), "%s: nheads * Nq and B * nheads must stay below 2^30", who);
   return MMB_OK;
 }

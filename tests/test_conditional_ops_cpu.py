@@ -134,3 +134,16 @@ def test_cross_attention_refuses_outputs_over_inputs():
             if other != g:
                 rc, msg = bwd({g: at[i]})
                 assert rc == -1 and b"same memory" in msg, (g, other, msg)
+
+
+def test_cross_attention_refuses_more_keys_than_its_counters_hold():
+    """The kernels count slots in 32 bits and look a step past the last: the largest key counts would wrap around."""
+    n, most = C.c_int64(-1), 2 ** 31 - 4097
+    for backward in (0, 1):
+        assert rc_of("mmb_cross_attention_workspace", 1, 1, most, 1, 1, 1, 2, backward, C.byref(n))[0] == 0 and n.value > 0
+    for Nk in (most + 1, 2 ** 31 - 513, 2 ** 31 - 1):
+        for backward in (0, 1):
+            rc, msg = rc_of("mmb_cross_attention_workspace", 1, 1, Nk, 1, 1, 1, 2, backward, C.byref(n))
+            assert rc == -1 and b"Nk must not exceed" in msg, msg
+        rc, msg = fwd(Nq=1, Nk=Nk, nh=1, nkv=1, D=1, dt=2, mk=P)
+        assert rc == -1 and b"Nk must not exceed" in msg, msg
