@@ -440,14 +440,14 @@ int mmb_attention_dropout_mask(int B, int N, int nheads, const float* maskf, int
  * not read (whatever they hold), a masked query gets a zero row and lse -inf, as does a query without a kept key.
  * lse (B,nheads,Nq) | NULL.  scale > 0.  workspace: device memory of the size mmb_cross_attention_workspace gives for the
  * same arguments (0: none), owned by this call until it has run: two calls that may overlap (streams, captured graphs)
- * need one each.  out overlaps no input. */
+ * need one each.  out, lse and workspace overlap no input and not each other (column slices of the same rows do not overlap). */
 int mmb_cross_attention_fwd(int B, int Nq, int Nk, int nheads, int nheads_kv, int D, int dtype, const void* q, int64_t q_ld,
                             const void* k, int64_t k_ld, const void* v, int64_t v_ld, const float* maskf_q,
                             const float* maskf_k, float scale, void* out, int64_t out_ld, float* lse, void* workspace,
                             int64_t workspace_bytes, void* stream);
 /* its reverse: dq, dk, dv (rows and types as q, k, v) are OVERWRITTEN; masked slots get zero rows.  out, lse: what the
  * forward returned for the same inputs; dout = d loss / d out.  Sums run in a fixed order: equal inputs, equal bits.
- * dq, dk, dv overlap no input and not each other. */
+ * dq, dk, dv and workspace overlap no input and not each other. */
 int mmb_cross_attention_bwd(int B, int Nq, int Nk, int nheads, int nheads_kv, int D, int dtype, const void* q, int64_t q_ld,
                             const void* k, int64_t k_ld, const void* v, int64_t v_ld, const float* maskf_q,
                             const float* maskf_k, float scale, const void* out, int64_t out_ld, const void* dout,

@@ -506,8 +506,6 @@ int jets_bwd(const Shape& s, bool vec, const float* q, int64_t q_ld, const float
 
 inline int pad_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 int check_shape(const char* who, int B, int Nq, int Nk, int nh, int nkv, int D, int dtype, float scale);
-// an output may not be the memory of an input (other workgroups still read it) or of another output
-int check_outputs(const char* who, const void* const* outs, int no, const void* const* ins, int ni);
 inline bool chunk_aligned(const void* p, int64_t ld, int es) { return ((uintptr_t)p & 15) == 0 && ld * es % 16 == 0; }
 
 }  // namespace xattn

@@ -13,6 +13,7 @@
 //           four partial sums of a workgroup are joined in LDS, those of several workgroups by a second launch.  For a
 //           few rows against many keys, where the team form would leave most of the chip idle.
 #include "cross_attention.h"
+#include "regions.h"
 #include <cmath>
 
 namespace mmb {
@@ -339,14 +340,6 @@ int check_shape(const char* who, int B, int Nq, int Nk, int nh, int nkv, int D, 
   return MMB_OK;
 }
 
-int check_outputs(const char* who, const void* const* outs, int no, const void* const* ins, int ni) {
-  for (int i = 0; i < no; ++i) {
-    for (int j = 0; j < ni; ++j) MMB_REQUIRE(outs[i] != ins[j], "%s: an output is the same memory as an input", who);
-    for (int j = 0; j < i; ++j) MMB_REQUIRE(outs[i] != outs[j], "%s: two outputs are the same memory", who);
-  }
-  return MMB_OK;
-}
-
 }  // namespace xattn
 }  // namespace mmb
 
@@ -384,8 +377,11 @@ extern "C" int mmb_cross_attention_fwd(int B, int Nq, int Nk, int nheads, int nh
   const int64_t need = jets || resident ? 0 : p.part_bytes(s);
   MMB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "mmb_cross_attention_fwd: workspace of %lld bytes needed, got %lld",
               (long long)need, (long long)(workspace ? workspace_bytes : 0));
-  const void *outs[] = {out}, *ins[] = {q, k, v};
-  if (int rc = check_outputs("mmb_cross_attention_fwd", outs, 1, ins, 3)) return rc;
+  const int64_t rq = (int64_t)B * Nq, rk = (int64_t)B * Nk, wq = (int64_t)nheads * D, wk = (int64_t)nheads_kv * D;
+  const Region outs[] = {row_region(out, rq, wq, out_ld, es), flat_region(lse, rq * nheads * 4), flat_region(workspace, need)};
+  const Region ins[] = {row_region(q, rq, wq, q_ld, es), row_region(k, rk, wk, k_ld, es), row_region(v, rk, wk, v_ld, es),
+                        flat_region(maskf_q, rq * 4), flat_region(maskf_k, rk * 4)};
+  if (int rc = check_apart("mmb_cross_attention_fwd", outs, 3, ins, 5)) return rc;
   if (jets)
     return jets_fwd(s, vec, (const float*)q, q_ld, (const float*)k, k_ld, (const float*)v, v_ld, maskf_q, maskf_k, scale, (float*)out, out_ld,
                     lse, as_stream(stream));

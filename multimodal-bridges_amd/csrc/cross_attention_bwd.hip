@@ -11,6 +11,7 @@
 // waves of one kind alone are too few to cover each other's latencies); with so few keys that a row is in registers at once,
 // the dq workgroups run first and take delta from p and dp themselves, free of the rounding of out.
 #include "cross_attention.h"
+#include "regions.h"
 
 namespace mmb {
 namespace xattn {
@@ -391,11 +392,16 @@ extern "C" int mmb_cross_attention_bwd(int B, int Nq, int Nk, int nheads, int nh
   const int64_t need = (int64_t)B * nheads * Nq * 4;
   MMB_REQUIRE(workspace && workspace_bytes >= need, "mmb_cross_attention_bwd: workspace of %lld bytes needed, got %lld",
               (long long)need, (long long)(workspace ? workspace_bytes : 0));
-  const void *outs[] = {dq, dk, dv}, *ins[] = {q, k, v, out, dout};
-  if (int rc = check_outputs("mmb_cross_attention_bwd", outs, 3, ins, 5)) return rc;
+  const int es = dtype == MMB_DT_F32 ? 4 : 2;
+  const int64_t rq = (int64_t)B * Nq, rk = (int64_t)B * Nk;
+  const Region outs[] = {row_region(dq, rq, wq, dq_ld, es), row_region(dk, rk, wk, dk_ld, es), row_region(dv, rk, wk, dv_ld, es),
+                         flat_region(workspace, need)};
+  const Region ins[] = {row_region(q, rq, wq, q_ld, es), row_region(k, rk, wk, k_ld, es), row_region(v, rk, wk, v_ld, es),
+                        row_region(out, rq, wq, out_ld, es), row_region(dout, rq, wq, dout_ld, es), flat_region(lse, need),
+                        flat_region(maskf_q, rq * 4), flat_region(maskf_k, rk * 4)};
+  if (int rc = check_apart("mmb_cross_attention_bwd", outs, 4, ins, 8)) return rc;
   BwdArgs a = {{B, Nq, Nk, nheads, nheads_kv, D, nheads / nheads_kv}, q, k, v, out, dout, q_ld, k_ld, v_ld, out_ld, dout_ld,
                dq_ld, dk_ld, dv_ld, maskf_q, maskf_k, lse, scale, dq, dk, dv, (float*)workspace, false, false, 0, 0, {}, {}, 0};
-  const int es = dtype == MMB_DT_F32 ? 4 : 2;
   const bool vec = D * es % 16 == 0 && chunk_aligned(q, q_ld, es) && chunk_aligned(k, k_ld, es) && chunk_aligned(v, v_ld, es) &&
                    chunk_aligned(out, out_ld, es) && chunk_aligned(dout, dout_ld, es) && chunk_aligned(dq, dq_ld, es) &&
                    chunk_aligned(dk, dk_ld, es) && chunk_aligned(dv, dv_ld, es);

@@ -251,6 +251,24 @@ def test_cross_attention_strides_and_what_lies_around(dtype, off):
         assert bool((rest == 7.0).all()), n
 
 
+def test_cross_attention_all_in_the_columns_of_one_matrix():
+    """Inputs, output and gradients side by side in the same rows share no memory: the call is taken and gives the same bits."""
+    from mmb_hip import ops
+    B, N, nh, D = 2, 70, 2, 16
+    q, k, v, do, mq, mk = make(B, N, N, nh, nh, D, torch.float32, 51, True)
+    want = run_attention(q, k, v, do, mq, mk, B, nh, nh, 0.25)
+    w = torch.full((B * N, 8 * 32 + 5), 3.0, device="cuda")
+    c = [w[:, 32 * i:32 * i + 32] for i in range(8)]
+    for t, x in zip(c, (q, k, v, do)):
+        t.copy_(x)
+    kw = dict(mq=ops.mask_prepare(mq.cuda()), mk=ops.mask_prepare(mk.cuda()), scale=0.25)
+    _, lse = ops.cross_attention_fwd(*c[:3], B, nh, want_lse=True, out=c[4], **kw)
+    ops.cross_attention_bwd(*c[:3], c[4], c[3], lse, B, nh, dq=c[5], dk=c[6], dv=c[7], **kw)
+    for t, n in zip(c[4:], ("out", "dq", "dk", "dv")):
+        assert torch.equal(t, want[n]), n
+    assert all(torch.equal(t.cpu(), x) for t, x in zip(c, (q, k, v, do))) and bool((w[:, 256:] == 3.0).all())
+
+
 def test_cross_attention_equal_bits_and_clouds_alone():
     """The same call twice, and each cloud in a call of its own, give equal bits."""
     args = make(3, 90, 400, 4, 2, 64, torch.bfloat16, 31, True)

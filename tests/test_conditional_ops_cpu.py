@@ -147,3 +147,43 @@ def test_cross_attention_refuses_more_keys_than_its_counters_hold():
             assert rc == -1 and b"Nk must not exceed" in msg, msg
         rc, msg = fwd(Nq=1, Nk=Nk, nh=1, nkv=1, D=1, dt=2, mk=P)
         assert rc == -1 and b"Nk must not exceed" in msg, msg
+
+
+class Box:
+    """Byte addresses of column slices in rows of 256 floats, two of them at the same place."""
+    base, ld = 0x100000, 256
+
+    def __call__(self, col, row=0):
+        return self.base + 4 * (row * self.ld + col)
+
+
+def fwd_in_box(**kw):
+    """B = 2, Nq = 4, Nk = 8, 2 heads on 1 of 16 floats: q, out 8 rows of 32; k, v 16 rows of 16, all slices of rows of 256"""
+    at = Box()
+    a = dict(B=2, Nq=4, Nk=8, nh=2, nkv=1, D=16, dt=0, q=at(0), q_ld=256, k=at(64), k_ld=256, v=at(96), v_ld=256, mq=0x10000, mk=0x20000,
+             scale=0.25, out=at(128), out_ld=256, lse=0x30000, ws=None, n=0, stream=None)
+    a.update(kw)
+    return rc_of("mmb_cross_attention_fwd", *a.values())
+
+
+@pytest.mark.parametrize("kw", [
+    dict(out=Box()(16)), dict(out=Box()(31)), dict(out=Box()(0, 1)), dict(out=Box()(0, 7)), dict(out=Box()(240)),
+    dict(out=Box()(48)), dict(out=Box()(79, 3)), dict(out=Box()(100)), dict(out=Box()(250, 2)), dict(out=Box()(0), out_ld=512),
+    dict(out=Box()(224), out_ld=288), dict(lse=Box()(0, 3)), dict(lse=0x10000), dict(lse=0x2003c), dict(out=0x30000), dict(out=0x10010, out_ld=32),
+])
+def test_cross_attention_fwd_refuses_partial_overlaps(kw):
+    rc, msg = fwd_in_box(**kw)
+    assert rc == -1 and b"overlap" in msg, msg
+
+
+def test_cross_attention_bwd_refuses_partial_overlaps():
+    at = Box()
+    ok = dict(q=at(0), k=at(32), v=at(48), out=at(64), dout=at(96), lse=0x30000, dq=at(128), dk=at(160), dv=at(176), ws=0x40000)
+    def bwd(**kw):
+        p = dict(ok, **kw)
+        return rc_of("mmb_cross_attention_bwd", 2, 4, 8, 2, 1, 16, 0, p["q"], 256, p["k"], 256, p["v"], 256, 0x10000, 0x20000, 0.25, p["out"],
+                     256, p["dout"], 256, p["lse"], p["dq"], 256, p["dk"], 256, p["dv"], 256, p["ws"], 1 << 20, None)
+    for kw in (dict(dq=at(100)), dict(dk=at(150)), dict(dv=at(160, 5)), dict(dk=at(8, 2)), dict(dv=at(64)), dict(dq=at(240, 1)),
+               dict(ws=0x30000), dict(ws=0x10000), dict(ws=0x20004), dict(ws=at(130, 2)), dict(dq=0x30004), dict(ws=0x30000 + 60)):
+        rc, msg = bwd(**kw)
+        assert rc == -1 and b"overlap" in msg, (kw, msg)
