@@ -481,7 +481,8 @@ int mmb_layernorm_bwd(int64_t M, int D, const float* x, int64_t x_ld, const floa
                       const float* dy, int64_t dy_ld, float* dx, int64_t dx_ld, int accumulate, float* dgamma,
                       float* dbeta, void* stream);
 /* Norm of every query and key head together with the rotation by the rows' positions, in one pass.
- * x, y: M rows of (nheads + nheads2) heads of D features (leading dimensions in elements; y may be x).  Per head
+ * x, y: M rows of (nheads + nheads2) heads of D features (leading dimensions in elements; y may be x, at the
+ * same leading dimension, and else overlaps no input).  Per head
  *   u = x / sqrt(mean x^2 + eps) * w      w = weight (D) for the first nheads heads, weight2 (D) for the others, NULL: ones
  *   pair p < n_pairs of u's first 2 n_pairs features is turned by the angle pos[row][p / (n_pairs / n_axes)] * freq[p]:
  *   (a, b) -> (a cos - b sin, a sin + b cos); pairs (p, p + n_pairs) when interleaved = 0, (2p, 2p + 1) when 1.
@@ -492,9 +493,9 @@ int mmb_head_norm_rotate_fwd(int64_t M, int nheads, int nheads2, int D, int dtyp
                              const float* weight, const float* weight2, float eps, const float* pos, int64_t pos_ld, int n_axes,
                              const float* freq, int n_pairs, int interleaved, void* y, int64_t y_ld, void* stream);
 #define MMB_HEAD_NORM_MAX_BLOCKS 1024
-/* its reverse from the SAME x (before the norm) and dy: dx (type and rows as x; may be dy), dweight, dweight2 (D) | NULL,
- * both OVERWRITTEN.  partials: workspace of 2 * D * MMB_HEAD_NORM_MAX_BLOCKS floats.  No gradient reaches pos and freq.
- * Sums run in a fixed order. */
+/* its reverse from the SAME x (before the norm) and dy: dx (type and rows as x; may be dy or x, at the same leading
+ * dimension), dweight, dweight2 (D) | NULL, both OVERWRITTEN; otherwise outputs and partials overlap nothing.  partials:
+ * workspace of 2 * D * MMB_HEAD_NORM_MAX_BLOCKS floats.  No gradient reaches pos and freq.  Sums run in a fixed order. */
 int mmb_head_norm_rotate_bwd(int64_t M, int nheads, int nheads2, int D, int dtype, const void* x, int64_t x_ld, const void* dy,
                              int64_t dy_ld, const float* weight, const float* weight2, float eps, const float* pos,
                              int64_t pos_ld, int n_axes, const float* freq, int n_pairs, int interleaved, void* dx,
@@ -504,7 +505,8 @@ int mmb_head_norm_rotate_bwd(int64_t M, int nheads, int nheads2, int D, int dtyp
  * exponent >= -127 with 127 * 2^e >= max |x|; codes (M, 32*ceil(K/32)) int8 = round(x / 2^e), ties to even, features past K
  * zero; steps (M, ceil(K/32)) uint8 = e + 127, 255 for a block that holds an infinity or NaN (it is restored as NaN).
  * |restored - x| <= 2^(e-1).  keep_nonzero != 0: values other than 0 get code +-1 at least (ReLU outputs: the gate is the same
- * from the checkpoint; |restored - x| < 2^e).  x: M rows of K, dtype MMB_DT_*.  codes 16-byte aligned. */
+ * from the checkpoint; |restored - x| < 2^e).  x: M rows of K, dtype MMB_DT_*.  codes 16-byte aligned.  Outputs of
+ * these calls overlap no input and not each other. */
 int mmb_checkpoint_rows(int64_t M, int K, int dtype, int keep_nonzero, const void* x, int64_t x_ld, void* codes, void* steps, void* stream);
 /* y (M, K) = code * 2^e, rounded to dtype (exact in float and bf16) */
 int mmb_restore_rows(int64_t M, int K, int dtype, const void* codes, const void* steps, void* y, int64_t y_ld, void* stream);

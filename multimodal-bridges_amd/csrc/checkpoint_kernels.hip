@@ -12,7 +12,7 @@
 // A code is an integer of 7 bits: code * 2^e is EXACT in bf16.  The weight gradient dW = dZ^T Xhat therefore needs ONE bf16
 // plane for Xhat and three for a float dZ (exact split, truncated 8 + 8 + 8 bits; two for fp16, one for bf16): three matrix
 // products where float activations need six, and a quarter of the bytes.
-#include "common.h"
+#include "regions.h"
 
 namespace mmb {
 namespace ckpt {
@@ -440,6 +440,9 @@ static int check_q8(const char* who, int64_t M, int K, const void* codes, const 
   MMB_REQUIRE(((uintptr_t)codes & 15) == 0, "%s: codes must be 16-byte aligned", who);
   return MMB_OK;
 }
+static int elem_bytes(int dtype) { return dtype == MMB_DT_F32 ? 4 : dtype == MMB_DT_BF16 || dtype == MMB_DT_F16 ? 2 : 0; }
+static Region code_region(const void* codes, int64_t M, int K) { return flat_region(codes, M * ((K + 31) / 32 * 32)); }
+static Region step_region(const void* steps, int64_t M, int K) { return flat_region(steps, M * ((K + 31) / 32)); }
 
 template <typename T>
 static int encode(int64_t M, int K, int keep_nonzero, const void* x, int64_t x_ld, void* codes, void* steps, hipStream_t st) {
@@ -499,23 +502,27 @@ extern "C" int mmb_checkpoint_rows(int64_t M, int K, int dtype, int keep_nonzero
                                    void* stream) {
   if (int rc = check_q8("mmb_checkpoint_rows", M, K, codes, steps)) return rc;
   MMB_REQUIRE(x && x_ld >= K, "mmb_checkpoint_rows: x is NULL or its leading dimension smaller than its row");
+  const int es = elem_bytes(dtype);
+  MMB_REQUIRE(es, "mmb_checkpoint_rows: unknown dtype %d", dtype);
+  const Region outs[] = {code_region(codes, M, K), step_region(steps, M, K)}, in = row_region(x, M, K, x_ld, es);
+  if (int rc = check_apart("mmb_checkpoint_rows", outs, 2, &in, 1)) return rc;
   hipStream_t st = as_stream(stream);
   if (dtype == MMB_DT_F32) return encode<float>(M, K, keep_nonzero != 0, x, x_ld, codes, steps, st);
   if (dtype == MMB_DT_BF16) return encode<__bf16>(M, K, keep_nonzero != 0, x, x_ld, codes, steps, st);
-  if (dtype == MMB_DT_F16) return encode<_Float16>(M, K, keep_nonzero != 0, x, x_ld, codes, steps, st);
-  set_error("mmb_checkpoint_rows: unknown dtype %d", dtype);
-  return MMB_ERR_INVALID_ARG;
+  return encode<_Float16>(M, K, keep_nonzero != 0, x, x_ld, codes, steps, st);
 }
 
 extern "C" int mmb_restore_rows(int64_t M, int K, int dtype, const void* codes, const void* steps, void* y, int64_t y_ld, void* stream) {
   if (int rc = check_q8("mmb_restore_rows", M, K, codes, steps)) return rc;
   MMB_REQUIRE(y && y_ld >= K, "mmb_restore_rows: y is NULL or its leading dimension smaller than its row");
+  const int es = elem_bytes(dtype);
+  MMB_REQUIRE(es, "mmb_restore_rows: unknown dtype %d", dtype);
+  const Region out = row_region(y, M, K, y_ld, es), ins[] = {code_region(codes, M, K), step_region(steps, M, K)};
+  if (int rc = check_apart("mmb_restore_rows", &out, 1, ins, 2)) return rc;
   hipStream_t st = as_stream(stream);
   if (dtype == MMB_DT_F32) return decode<float>(M, K, codes, steps, y, y_ld, st);
   if (dtype == MMB_DT_BF16) return decode<__bf16>(M, K, codes, steps, y, y_ld, st);
-  if (dtype == MMB_DT_F16) return decode<_Float16>(M, K, codes, steps, y, y_ld, st);
-  set_error("mmb_restore_rows: unknown dtype %d", dtype);
-  return MMB_ERR_INVALID_ARG;
+  return decode<_Float16>(M, K, codes, steps, y, y_ld, st);
 }
 
 extern "C" int mmb_grad_weight_rows_q8_workspace(int64_t M, int N, int K, int64_t* bytes_host) {
@@ -535,12 +542,15 @@ extern "C" int mmb_grad_weight_rows_q8(int64_t M, int K, int N, int dtype, const
   const int64_t need = (int64_t)a.splits * ((int64_t)N * K + N) * 4;
   MMB_REQUIRE(workspace && workspace_bytes >= need, "mmb_grad_weight_rows_q8: workspace of %lld bytes needed, got %lld", (long long)need,
               (long long)(workspace ? workspace_bytes : 0));
+  const int es = elem_bytes(dtype);
+  MMB_REQUIRE(es, "mmb_grad_weight_rows_q8: unknown dtype %d", dtype);
+  const Region outs[] = {row_region(dW, N, K, dw_ld, 4), flat_region(db, 4 * (int64_t)N), flat_region(workspace, need)};
+  const Region ins[] = {code_region(codes, M, K), step_region(steps, M, K), row_region(dZ, M, N, dz_ld, es)};
+  if (int rc = check_apart("mmb_grad_weight_rows_q8", outs, 3, ins, 3)) return rc;
   a.pw = (float*)workspace;
   a.pb = a.pw + (int64_t)a.splits * N * K;
   hipStream_t st = as_stream(stream);
   if (dtype == MMB_DT_F32) return grad_weight<float>(a, p, dW, dw_ld, db, accumulate, st);
   if (dtype == MMB_DT_BF16) return grad_weight<__bf16>(a, p, dW, dw_ld, db, accumulate, st);
-  if (dtype == MMB_DT_F16) return grad_weight<_Float16>(a, p, dW, dw_ld, db, accumulate, st);
-  set_error("mmb_grad_weight_rows_q8: unknown dtype %d", dtype);
-  return MMB_ERR_INVALID_ARG;
+  return grad_weight<_Float16>(a, p, dW, dw_ld, db, accumulate, st);
 }

@@ -9,7 +9,7 @@
 // that row, so its angles -- the same for every head -- are computed once.  The angle is formed in 64 bits (the product of
 // two floats is exact there) and reduced to a fraction of a turn before the 32-bit sine: positions far down a list keep
 // full accuracy.  Statistics and products are in 32 bits, one rounding when a value is stored.
-#include "common.h"
+#include "regions.h"
 
 namespace mmb {
 namespace headnorm {
@@ -356,6 +356,11 @@ static int check(const char* who, int64_t M, int nh1, int nh2, int D, int dtype,
   return MMB_OK;
 }
 
+// y over x (dx over x or dy) row by row is fine: a head is read whole before it is written.  Shifted by anything it is not.
+static Region other_than(const Region& r, const Region& y) {
+  return r.at == y.at && (r.ld == y.ld || r.rows == 1) ? Region{} : r;
+}
+
 }  // namespace headnorm
 }  // namespace mmb
 
@@ -373,6 +378,12 @@ extern "C" int mmb_head_norm_rotate_fwd(int64_t M, int nheads, int nheads2, int 
             x_ld, 0, pos_ld, y_ld, eps, y, nullptr, 0, 0};
   hipStream_t st = as_stream(stream);
   const char* who = "mmb_head_norm_rotate_fwd";
+  const int es = dtype == MMB_DT_F32 ? 4 : 2;
+  const int64_t w = (int64_t)(nheads + nheads2) * D;
+  const Region ry = row_region(y, M, w, y_ld, es);
+  const Region ins[] = {other_than(row_region(x, M, w, x_ld, es), ry), flat_region(weight, 4 * D), flat_region(weight2, 4 * D),
+                        row_region(n_pairs ? pos : nullptr, M, n_axes, pos_ld, 4), flat_region(n_pairs ? freq : nullptr, 4 * n_pairs)};
+  if (int rc = check_apart(who, &ry, 1, ins, 5)) return rc;
   if (dtype == MMB_DT_F32) return launch<float, false>(a, nullptr, nullptr, st, who);
   if (dtype == MMB_DT_BF16) return launch<__bf16, false>(a, nullptr, nullptr, st, who);
   return launch<_Float16, false>(a, nullptr, nullptr, st, who);
@@ -390,6 +401,17 @@ extern "C" int mmb_head_norm_rotate_bwd(int64_t M, int nheads, int nheads2, int 
   Args a = {M, nheads, nheads2, D, n_pairs, n_pairs ? n_pairs / n_axes : 1, interleaved, x, dy, weight, weight2, pos, freq,
             x_ld, dy_ld, pos_ld, dx_ld, eps, dx, partials, 0, 0};
   hipStream_t st = as_stream(stream);
+  const int es = dtype == MMB_DT_F32 ? 4 : 2;
+  const int64_t w = (int64_t)(nheads + nheads2) * D;
+  const Region outs[] = {row_region(dx, M, w, dx_ld, es), flat_region(dweight, 4 * D), flat_region(dweight2, 4 * D),
+                         flat_region(partials, (int64_t)2 * D * kMaxBlocks * 4)};
+  const Region rx = row_region(x, M, w, x_ld, es), rdy = row_region(dy, M, w, dy_ld, es);
+  const Region fixed[] = {flat_region(weight, 4 * D), flat_region(weight2, 4 * D), row_region(n_pairs ? pos : nullptr, M, n_axes, pos_ld, 4),
+                          flat_region(n_pairs ? freq : nullptr, 4 * n_pairs)};
+  const Region of_dx[] = {other_than(rx, outs[0]), other_than(rdy, outs[0])}, of_sums[] = {rx, rdy};
+  if (int rc = check_apart(who, outs, 4, fixed, 4)) return rc;
+  if (int rc = check_apart(who, outs, 1, of_dx, 2)) return rc;
+  if (int rc = check_apart(who, outs + 1, 3, of_sums, 2)) return rc;
   if (dtype == MMB_DT_F32) return launch<float, true>(a, dweight, dweight2, st, who);
   if (dtype == MMB_DT_BF16) return launch<__bf16, true>(a, dweight, dweight2, st, who);
   return launch<_Float16, true>(a, dweight, dweight2, st, who);

@@ -846,7 +846,7 @@ HEAD_NORM_MAX_BLOCKS = 1024
 
 def head_norm_rotate_bwd(x, dy, nheads, weight=None, nheads2=0, weight2=None, eps=1e-6, pos=None, freq=None, layout="half", dx=None):
     """(dx, dweight, dweight2) of head_norm_rotate_fwd from its INPUT x and dy; a weight that was None has gradient None.
-    dx may be dy.  No gradient reaches pos and freq."""
+    dx may be dy or x.  No gradient reaches pos and freq."""
     D, args, xp, tail = _head_args(x, nheads, weight, nheads2, weight2, eps, pos, freq, layout)
     dev = x.device
     with _on(dev):

@@ -413,6 +413,19 @@ def test_head_norm_rotate(case, dtype):
     within(ops.head_norm_rotate_fwd(xd, nh, None, **kw), *ref_head_norm(x, dy, nh, None, nh2, None, eps, pos, freq, layout, dt)["y"], "no weight")
 
 
+@pytest.mark.parametrize("D", [32, 33])
+def test_head_norm_rotate_reverse_over_its_input(D):
+    """dx may be x: every head is read whole before its gradient is written."""
+    from mmb_hip import ops
+    g = torch.Generator().manual_seed(D)
+    x, dy, w = torch.randn(300, 3 * D, generator=g).cuda(), torch.randn(300, 3 * D, generator=g).cuda(), torch.rand(D, generator=g).cuda()
+    kw = dict(pos=torch.randn(300, 1, generator=g).cuda(), freq=torch.rand(16, generator=g).cuda())
+    dx, dw, _ = ops.head_norm_rotate_bwd(x, dy, 3, w, **kw)
+    z = x.clone()
+    got, dw2, _ = ops.head_norm_rotate_bwd(z, dy, 3, w, dx=z, **kw)
+    assert got is z and torch.equal(z, dx) and torch.equal(dw2, dw)
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("off", [0, 1])
 def test_head_norm_rotate_slices(dtype, off):

@@ -187,3 +187,39 @@ def test_cross_attention_bwd_refuses_partial_overlaps():
                dict(ws=0x30000), dict(ws=0x10000), dict(ws=0x20004), dict(ws=at(130, 2)), dict(dq=0x30004), dict(ws=0x30000 + 60)):
         rc, msg = bwd(**kw)
         assert rc == -1 and b"overlap" in msg, (kw, msg)
+
+
+def test_head_norm_refuses_overlaps():
+    """Over x itself (dx over dy or x) is fine, row for row; shifted, at another stride or over the small inputs it is not."""
+    ok = dict(M=4, nh=2, nh2=1, D=16, dt=0, x=0x100000, x_ld=64, w=0x10000, w2=0x11000, eps=1e-6, pos=0x12000, pos_ld=2, axes=2, freq=0x13000,
+              pairs=8, layout=0, y=0x200000, y_ld=64, stream=None)
+    for kw in (dict(y=0x100000, y_ld=48), dict(y=0x100000 + 4), dict(y=0x100000 + 64 * 4), dict(y=0x100000 - 4 * 40), dict(y=0x10020),
+               dict(y=0x11000), dict(y=0x12010), dict(y=0x13000)):
+        a = dict(ok, **kw)
+        rc, msg = rc_of("mmb_head_norm_rotate_fwd", *a.values())
+        assert rc == -1 and b"overlap" in msg, (kw, msg)
+        for dy in (0x300000, a["y"]):                                # (dx over dy does not excuse dx over x)
+            b = list(a.values())
+            rc, msg = rc_of("mmb_head_norm_rotate_bwd", *b[:7], dy, a["y_ld"], *b[7:18], None, None, 0x400000, None)
+            assert rc == -1 and b"overlap" in msg, (kw, msg)
+    b = list(ok.values())
+    for dy, dy_ld, d1, d2, part in ((0x200000, 48, None, None, 0x400000), (0x200004, 64, None, None, 0x400000), (0x300000, 64, 0x200000, None, 0x400000),
+                                    (0x300000, 64, 0x100010, None, 0x400000), (0x300000, 64, 0x500000, 0x500020, 0x400000),
+                                    (0x300000, 64, 0x400000, None, 0x400000), (0x300000, 64, None, None, 0x100000 - 64), (0x300000, 64, 0x10000, None, 0x400000)):
+        rc, msg = rc_of("mmb_head_norm_rotate_bwd", *b[:7], dy, dy_ld, *b[7:18], d1, d2, part, None)
+        assert rc == -1 and b"overlap" in msg, msg
+
+
+@pytest.mark.parametrize("name,args", [
+    ("mmb_checkpoint_rows", (4, 40, 0, 0, 0x1000, 40, 0x1010, 0x9000, None)), ("mmb_checkpoint_rows", (4, 40, 0, 0, 0x1000, 40, 0x8000, 0x1100, None)),
+    ("mmb_checkpoint_rows", (4, 40, 1, 0, 0x1000, 40, 0x8000, 0x8040, None)),
+    ("mmb_restore_rows", (4, 40, 0, 0x8000, 0x9000, 0x80f0, 40, None)), ("mmb_restore_rows", (4, 40, 2, 0x8000, 0x9000, 0x8fff, 40, None)),
+    ("mmb_grad_weight_rows_q8", (4, 8, 6, 0, 0x1000, 0x2000, 0x3000, 6, 0x3040, 8, None, 0, 0x8000, 1 << 20, None)),
+    ("mmb_grad_weight_rows_q8", (4, 8, 6, 0, 0x1000, 0x2000, 0x3000, 6, 0x4000, 8, 0x3000, 0, 0x8000, 1 << 20, None)),
+    ("mmb_grad_weight_rows_q8", (4, 8, 6, 0, 0x1000, 0x2000, 0x3000, 6, 0x4000, 8, 0x4010, 0, 0x8000, 1 << 20, None)),
+    ("mmb_grad_weight_rows_q8", (4, 8, 6, 0, 0x1000, 0x2000, 0x3000, 6, 0x4000, 8, 0x5000, 0, 0x1040, 1 << 20, None)),
+    ("mmb_grad_weight_rows_q8", (4, 8, 6, 0, 0x1000, 0x2000, 0x3000, 6, 0x8010, 8, 0x5000, 0, 0x8000, 1 << 20, None)),
+])
+def test_checkpoints_refuse_overlaps(name, args):
+    rc, msg = rc_of(name, *args)
+    assert rc == -1 and b"overlap" in msg, msg
