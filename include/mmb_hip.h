@@ -435,8 +435,9 @@ int mmb_attention_dropout_mask(int B, int N, int nheads, const float* maskf, int
  *   s_ij = scale q_i . k_j over the kept keys j;  out_i = sum_j softmax_j(s_ij) v_j;  lse_i = log sum_j exp s_ij
  * q, out: B*Nq rows of nheads*D; k, v: B*Nk rows of nheads_kv*D (column slices of wider rows are fine: *_ld in elements).
  * nheads_kv divides nheads: query heads h*g .. h*g+g-1 share key head h (g = nheads / nheads_kv).  1 <= D <= 128,
- * Nk <= 2^31 - 4097, nheads * Nq and B * nheads <= 2^30; dtype MMB_DT_*: q, k, v, out (sums, softmax and lse in 32 bits; with 16-bit types the probabilities are rounded
- * to the type for the product with v).  maskf_q (B,Nq), maskf_k (B,Nk) | NULL: slots with 0 take no part -- their rows are
+ * Nk <= 2^31 - 4097, nheads * Nq and B * nheads <= 2^30, fewer than 2^32 threads in a launch (some 2^24 clouds x key heads);
+ * dtype MMB_DT_*: q, k, v, out (sums, softmax and lse in 32 bits; with 16-bit types the probabilities are rounded to the type
+ * for the product with v).  maskf_q (B,Nq), maskf_k (B,Nk) | NULL: slots with 0 take no part -- their rows are
  * not read (whatever they hold), a masked query gets a zero row and lse -inf, as does a query without a kept key.
  * lse (B,nheads,Nq) | NULL.  scale > 0.  workspace: device memory of the size mmb_cross_attention_workspace gives for the
  * same arguments (0: none), owned by this call until it has run: two calls that may overlap (streams, captured graphs)

@@ -389,24 +389,27 @@ gw_fold_kernel(int splits, int64_t nw, int N, int K, const float* __restrict__ p
                int64_t dw_ld, float* __restrict__ db, int accumulate) {
   __shared__ float red[8][33];
   const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int64_t i = (int64_t)blockIdx.x * 32 + c;
-  float s = 0.0f;
-  if (i < nw) {
+  for (int64_t i0 = (int64_t)blockIdx.x * 32; i0 < nw + N; i0 += (int64_t)gridDim.x * 32) {
+    const int64_t i = i0 + c;
+    float s = 0.0f;
+    if (i < nw) {
 #pragma unroll 4
-    for (int p = g; p < splits; p += 8) s += pw[(int64_t)p * nw + i];
-  } else if (i < nw + N) {
-    for (int p = g; p < splits; p += 8) s += pb[(int64_t)p * N + (i - nw)];
-  }
-  red[g][c] = s;
-  __syncthreads();
-  if (g != 0 || i >= nw + N) return;
+      for (int p = g; p < splits; p += 8) s += pw[(int64_t)p * nw + i];
+    } else if (i < nw + N) {
+      for (int p = g; p < splits; p += 8) s += pb[(int64_t)p * N + (i - nw)];
+    }
+    __syncthreads();                               // (the sums of the turn before have been read)
+    red[g][c] = s;
+    __syncthreads();
+    if (g != 0 || i >= nw + N) continue;
 #pragma unroll
-  for (int q = 1; q < 8; ++q) s += red[q][c];
-  if (i < nw) {
-    float* d = dW + i / K * dw_ld + i % K;
-    *d = accumulate ? *d + s : s;
-  } else if (db) {
-    db[i - nw] = accumulate ? db[i - nw] + s : s;
+    for (int q = 1; q < 8; ++q) s += red[q][c];
+    if (i < nw) {
+      float* d = dW + i / K * dw_ld + i % K;
+      *d = accumulate ? *d + s : s;
+    } else if (db) {
+      db[i - nw] = accumulate ? db[i - nw] + s : s;
+    }
   }
 }
 
@@ -464,6 +467,8 @@ template <typename T, int BN, int BK, bool VEC>
 static int launch_gw(const GwArgs& a, hipStream_t st) {
   constexpr int bytes = gw_lds<T, BN, BK>();
   static_assert(bytes <= 160 * 1024, "LDS");
+  const int64_t blocks = (int64_t)(a.splits + 7) / 8 * 8 * a.nt * a.kt;
+  MMB_REQUIRE(grid_fits(blocks, 2 * BN), "mmb_grad_weight_rows_q8: %lld workgroups are more than a launch takes", (long long)blocks);
   auto kern = gw_kernel<T, BN, BK, VEC>;
   static PerDeviceOnce once;
   if (bytes > 64 * 1024 &&
@@ -471,8 +476,6 @@ static int launch_gw(const GwArgs& a, hipStream_t st) {
     set_error("mmb_grad_weight_rows_q8: the runtime refuses %d bytes of LDS", bytes);
     return MMB_ERR_LAUNCH;
   }
-  const int64_t blocks = (int64_t)(a.splits + 7) / 8 * 8 * a.nt * a.kt;
-  MMB_REQUIRE(blocks <= 0x7fffffffLL, "mmb_grad_weight_rows_q8: %lld workgroups", (long long)blocks);
   kern<<<(unsigned)blocks, 2 * BN, bytes, st>>>(a);
   return check_launch("mmb_grad_weight_rows_q8");
 }
@@ -484,11 +487,10 @@ static int pick_tile(const GwArgs& a, const GwPlan& p, hipStream_t st) {
 template <typename T>
 static int grad_weight(GwArgs& a, const GwPlan& p, float* dW, int64_t dw_ld, float* db, int accumulate, hipStream_t st) {
   const bool vec = a.N % 8 == 0 && ((uintptr_t)a.dz & 15) == 0 && a.dz_ld * (int64_t)sizeof(T) % 16 == 0 && a.dz_ld < (1 << 24);
-  const int64_t nw = (int64_t)a.N * a.K, fold = (nw + a.N + 31) / 32;
-  MMB_REQUIRE(fold <= 0x7fffffffLL, "mmb_grad_weight_rows_q8: dW of %lld values", (long long)nw);
+  const int64_t nw = (int64_t)a.N * a.K, fold = (nw + a.N + 31) / 32, most = 1 << 23;
   int rc = vec ? pick_tile<T, true>(a, p, st) : pick_tile<T, false>(a, p, st);
   if (rc != MMB_OK) return rc;
-  gw_fold_kernel<<<(unsigned)fold, 256, 0, st>>>(a.splits, nw, a.N, a.K, a.pw, a.pb, dW, dw_ld, db, accumulate);
+  gw_fold_kernel<<<(unsigned)(fold < most ? fold : most), 256, 0, st>>>(a.splits, nw, a.N, a.K, a.pw, a.pb, dW, dw_ld, db, accumulate);
   return check_launch("mmb_grad_weight_rows_q8 (fold)");
 }
 

@@ -49,6 +49,9 @@ struct PerDeviceOnce {
   }
 };
 
+// HIP launches fewer than 2^32 threads in a dimension
+inline bool grid_fits(int64_t blocks, int threads) { return blocks <= 0xffffffffLL / threads; }
+
 // grid for a memory-bound grid-stride kernel: enough blocks to fill 256 CUs x 8, capped
 inline int stream_grid(int64_t work_items, int block) {
   int64_t g = (work_items + block - 1) / block;

@@ -438,6 +438,7 @@ struct GridMap {
 };
 inline GridMap grid_map(int B, int nkv, int per_head) {
   GridMap g;
+  if ((int64_t)nkv * per_head > 0x7fffffff) return {0x7fffffff, 0x7fffffff, 0};       // (more than any launch takes)
   if (B % 8 == 0 || B >= 64) g = {B, nkv * per_head, 1};
   else if ((int64_t)B * nkv >= 64 || (B * nkv) % 8 == 0) g = {B * nkv, per_head, 1};
   else g = {B * nkv, per_head, 0};

@@ -389,7 +389,7 @@ extern "C" int mmb_cross_attention_fwd(int B, int Nq, int Nk, int nheads, int nh
     return resident_fwd(s, dtype, vec, q, q_ld, k, k_ld, v, v_ld, maskf_q, maskf_k, scale, out, out_ld, lse, as_stream(stream));
   FwdArgs a = {s, q, k, v, q_ld, k_ld, v_ld, out_ld, maskf_q, maskf_k, scale, out, lse, (float*)workspace, vec, p.tiles, p.nsplit, p.chunk,
                grid_map(B, nheads_kv, p.tiles * p.nsplit)};
-  MMB_REQUIRE(a.map.blocks() <= 0x7fffffffLL, "mmb_cross_attention_fwd: %lld workgroups", (long long)a.map.blocks());
+  MMB_REQUIRE(grid_fits(a.map.blocks(), 64 * p.nw), "mmb_cross_attention_fwd: %lld workgroups are more than a launch takes", (long long)a.map.blocks());
   hipStream_t st = as_stream(stream);
   if (dtype == MMB_DT_F32) return vec ? pick_dp<float, true>(p, a, st) : pick_dp<float, false>(p, a, st);
   if (dtype == MMB_DT_BF16) return vec ? pick_dp<__bf16, true>(p, a, st) : pick_dp<__bf16, false>(p, a, st);

@@ -321,6 +321,13 @@ template <typename T, int DP, int NW, bool VEC>
 static int run_bwd(BwdArgs& a, hipStream_t st) {
   constexpr int bytes = bwd_lds<T, DP, NW>();
   static_assert(bytes <= 160 * 1024, "LDS");
+  const Shape& s = a.sh;
+  a.tiles_q = (int)(((int64_t)s.g * s.Nq + 32 * NW - 1) / (32 * NW));
+  a.tiles_k = (int)(((int64_t)s.Nk + 32 * NW - 1) / (32 * NW));
+  a.map_q = grid_map(s.B, s.nkv, a.tiles_q);
+  a.map_k = grid_map(s.B, s.nkv, a.tiles_k);
+  const int64_t nq = a.map_q.blocks(), nk = a.map_k.blocks();
+  MMB_REQUIRE(grid_fits(nq + nk, 64 * NW), "mmb_cross_attention_bwd: %lld workgroups are more than a launch takes", (long long)(nq + nk));
   auto kern = bwd_kernel<T, DP, NW, VEC>;
   static PerDeviceOnce once;
   if (bytes > 64 * 1024 &&
@@ -328,13 +335,6 @@ static int run_bwd(BwdArgs& a, hipStream_t st) {
     set_error("mmb_cross_attention_bwd: the runtime refuses %d bytes of LDS", bytes);
     return MMB_ERR_LAUNCH;
   }
-  const Shape& s = a.sh;
-  a.tiles_q = (int)(((int64_t)s.g * s.Nq + 32 * NW - 1) / (32 * NW));
-  a.tiles_k = (int)(((int64_t)s.Nk + 32 * NW - 1) / (32 * NW));
-  a.map_q = grid_map(s.B, s.nkv, a.tiles_q);
-  a.map_k = grid_map(s.B, s.nkv, a.tiles_k);
-  const int64_t nq = a.map_q.blocks(), nk = a.map_k.blocks();
-  MMB_REQUIRE(nq + nk <= 0x7fffffffLL, "mmb_cross_attention_bwd: %lld workgroups", (long long)(nq + nk));
   a.few_keys = s.Nk <= 32;
   // (818 clouds of 2 x 1306 slots, 15 heads on 3: 903 -> 557 us a training step)
   a.pack_heads = s.g > 1 && s.Nq < dkv_tile<T, DP>();

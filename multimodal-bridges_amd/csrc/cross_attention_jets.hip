@@ -396,7 +396,7 @@ static int launch_jets(JetArgs& a, hipStream_t st) {
   if (!BWD)
     while ((int64_t)s.B * s.nkv * a.parts < 1024 && a.parts * NW < s.g * (a.nqp / 16)) a.parts *= 2;
   a.map = {s.B, s.nkv * a.parts, s.B % 8 == 0 || s.B >= 64 ? 1 : 0};
-  MMB_REQUIRE(a.map.blocks() <= 0x7fffffffLL, "mmb_cross_attention: %lld workgroups", (long long)a.map.blocks());
+  MMB_REQUIRE(grid_fits(a.map.blocks(), 64 * NW), "mmb_cross_attention: %lld workgroups are more than a launch takes", (long long)a.map.blocks());
   void (*kern)(JetArgs);
   if constexpr (BWD) kern = jet_bwd_kernel<FT, NW, VEC>;
   else kern = jet_fwd_kernel<FT, NW, VEC>;

@@ -354,7 +354,7 @@ static int run_res(ResArgs& a, int dtype, bool vec, hipStream_t st) {
   if (!BWD)
     while ((int64_t)s.B * s.nkv * a.parts < 1024 && a.parts * kResWaves < s.g * (a.nqp / 32)) a.parts *= 2;
   a.map = {s.B, s.nkv * a.parts, s.B % 8 == 0 || s.B >= 64 ? 1 : 0};
-  MMB_REQUIRE(a.map.blocks() <= 0x7fffffffLL, "mmb_cross_attention: %lld workgroups", (long long)a.map.blocks());
+  MMB_REQUIRE(grid_fits(a.map.blocks(), 64 * kResWaves), "mmb_cross_attention: %lld workgroups are more than a launch takes", (long long)a.map.blocks());
   const int64_t bytes = res_bytes(s, dtype, BWD);
   if (dtype == MMB_DT_F32) return vec ? pick_res<BWD, float, true>(a, dtype, bytes, st) : pick_res<BWD, float, false>(a, dtype, bytes, st);
   if (dtype == MMB_DT_BF16) return vec ? pick_res<BWD, __bf16, true>(a, dtype, bytes, st) : pick_res<BWD, __bf16, false>(a, dtype, bytes, st);

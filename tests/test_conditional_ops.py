@@ -568,6 +568,23 @@ def test_grad_weight_rows_q8_extremes():
     assert dW[:, 64:96].isnan().all() and dW[:, :64].isfinite().all()
 
 
+def test_grad_weight_rows_q8_of_many_elements():
+    """dW of more elements than one launch has threads for at eight an element.  Three rows: every product is exact and a sum
+    of three 32-bit values is off by at most two roundings of the largest partial sum."""
+    from mmb_hip import ops
+    M, N, K = 3, 23201, 23200
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q8 = ops.checkpoint_rows(torch.randn(M, K, generator=g, device="cuda"))
+    dz = torch.randn(M, N, generator=g, device="cuda")
+    dW, db = ops.grad_weight_rows_q8(q8, dz)
+    x = ops.restore_rows(q8)
+    for lo in range(0, N, 4000):
+        z = dz[:, lo:lo + 4000].double()
+        tol = 3 * E * (z.abs().t() @ x.double().abs())
+        assert bool(((dW[lo:lo + 4000].double() - z.t() @ x.double()).abs() <= tol).all()), lo
+    assert bool(((db.double() - dz.double().sum(0)).abs() <= 3 * E * dz.double().abs().sum(0)).all())
+
+
 # ------------------------------------------------------------------------------------------------ together
 class Layer:
     """One conditional attention layer as a training step runs it: project, norm and rotate q and k, attend, project; the

@@ -223,3 +223,22 @@ def test_head_norm_refuses_overlaps():
 def test_checkpoints_refuse_overlaps(name, args):
     rc, msg = rc_of(name, *args)
     assert rc == -1 and b"overlap" in msg, msg
+
+
+@pytest.mark.parametrize("shape", [  # B, Nq, Nk, nh, nkv, D, dtype: the small-cloud forms, one wave, eight waves
+    (1 << 20, 8, 8, 16, 16, 16, 0), (1 << 20, 16, 16, 16, 16, 64, 2), (1 << 22, 1, 8, 64, 64, 1, 1), (1 << 20, 300, 400, 8, 8, 128, 1)])
+def test_cross_attention_refuses_more_workgroups_than_a_launch_takes(shape):
+    B, Nq, Nk, nh, nkv, D, dt = shape
+    far = [(i + 1) << 46 for i in range(9)]
+    rc, msg = fwd(B=B, Nq=Nq, Nk=Nk, nh=nh, nkv=nkv, D=D, dt=dt, q=far[0], q_ld=nh * D, k=far[1], k_ld=nkv * D, v=far[2], v_ld=nkv * D, out=far[3],
+                  out_ld=nh * D)
+    assert rc == -1 and b"workgroups" in msg, msg
+    rc, msg = rc_of("mmb_cross_attention_bwd", B, Nq, Nk, nh, nkv, D, dt, far[0], nh * D, far[1], nkv * D, far[2], nkv * D, None, None, 0.25,
+                    far[3], nh * D, far[4], nh * D, far[5], far[6], nh * D, far[7], nkv * D, far[8], nkv * D, 3 << 45, 1 << 40, None)
+    assert rc == -1 and b"workgroups" in msg, msg
+
+
+def test_cross_attention_refuses_tiles_beyond_32_bits():
+    rc, msg = rc_of("mmb_cross_attention_bwd", 1, 1, 2 ** 31 - 5000, 1024, 1024, 1, 2, 1 << 46, 1024, 1 << 47, 1024, 1 << 48, 1024, None, None,
+                    0.25, 1 << 49, 1024, 1 << 50, 1024, 1 << 51, 1 << 52, 1024, 1 << 53, 1024, 1 << 54, 1024, 1 << 55, 1 << 40, None)
+    assert rc == -1 and b"workgroups" in msg, msg
