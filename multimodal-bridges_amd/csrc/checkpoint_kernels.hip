@@ -528,7 +528,8 @@ extern "C" int mmb_restore_rows(int64_t M, int K, int dtype, const void* codes, 
 }
 
 extern "C" int mmb_grad_weight_rows_q8_workspace(int64_t M, int N, int K, int64_t* bytes_host) {
-  MMB_REQUIRE(M > 0 && N > 0 && K > 0 && bytes_host, "mmb_grad_weight_rows_q8_workspace: sizes must be positive, bytes_host not NULL");
+  MMB_REQUIRE(M > 0 && N > 0 && K > 0 && N <= (1 << 20) && K <= (1 << 20) && bytes_host,
+              "mmb_grad_weight_rows_q8_workspace: sizes must be positive, N and K at most 2^20, bytes_host not NULL");
   *bytes_host = (int64_t)gw_plan(M, N, K).splits * ((int64_t)N * K + N) * 4;
   return MMB_OK;
 }

@@ -242,3 +242,12 @@ def test_cross_attention_refuses_tiles_beyond_32_bits():
     rc, msg = rc_of("mmb_cross_attention_bwd", 1, 1, 2 ** 31 - 5000, 1024, 1024, 1, 2, 1 << 46, 1024, 1 << 47, 1024, 1 << 48, 1024, None, None,
                     0.25, 1 << 49, 1024, 1 << 50, 1024, 1 << 51, 1 << 52, 1024, 1 << 53, 1024, 1 << 54, 1024, 1 << 55, 1 << 40, None)
     assert rc == -1 and b"workgroups" in msg, msg
+
+
+def test_workspace_query_refuses_what_the_call_refuses():
+    """N and K up to 2^20: beyond, the query's own divisions would run past 32 bits."""
+    n = C.c_int64(-1)
+    assert rc_of("mmb_grad_weight_rows_q8_workspace", 8, 1 << 20, 1 << 20, C.byref(n))[0] == 0 and n.value == 4 * ((1 << 40) + (1 << 20))
+    for N, K in (((1 << 20) + 1, 8), (8, (1 << 20) + 1), (2 ** 31 - 1, 2 ** 31 - 1)):
+        rc, msg = rc_of("mmb_grad_weight_rows_q8_workspace", 8, N, K, C.byref(n))
+        assert rc == -1 and b"at most 2^20" in msg, msg
