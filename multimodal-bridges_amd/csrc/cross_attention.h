@@ -346,6 +346,17 @@ __device__ __forceinline__ void store_col(T* __restrict__ p, const f32x16* acc, 
     }
 }
 
+// Half precision: p in [0, 1] takes 2^12 into the product.  p = 1 / Nk of a long list would be subnormal, and below 2^-25 zero
+// while the sum still counts it: a long tail of like scores would lose that share of the output.
+constexpr float kHalfLog = 12.0f, kHalfP = 4096.0f;
+template <typename T> constexpr float p_log() { return __is_same(T, _Float16) ? kHalfLog : 0.0f; }
+
+// log-sum of a row from its maximum and sum; the forward's sums carry p's 2^12 in half precision
+template <typename T>
+__device__ __forceinline__ float row_lse(float m, float l, float scale) {
+  return l == 0.0f ? -INFINITY : m * scale + logf(__is_same(T, _Float16) ? l * (1.0f / kHalfP) : l);
+}
+
 // Running softmax over one tile of n keys: raw scores in s become p; m, l and what acc has summed follow the maximum.
 template <typename T, int DP, int TK>
 __device__ __forceinline__ void softmax_step(f32x16* s, int n, float c, float& m, float& l, f32x16* acc) {
@@ -374,13 +385,14 @@ __device__ __forceinline__ void softmax_step(f32x16* s, int n, float c, float& m
       for (int r = 0; r < 16; ++r) acc[t][r] *= alpha;
     m = mn;
   }
+  // 16-bit inputs: one fused step (the rounding of off moves all p of a row alike and cancels); float: the difference first,
+  // which is exact next to the maximum
+  const float off = fmaf(-ms, c, p_log<T>());
 #pragma unroll
   for (int st = 0; st < TK / 32; ++st)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      // 16-bit inputs: one fused step (the rounding of ms * c moves all p of a row alike and cancels); float: the
-      // difference first, which is exact next to the maximum
-      s[st][r] = __builtin_amdgcn_exp2f(sizeof(T) == 2 ? fmaf(s[st][r], c, -ms * c) : (s[st][r] - ms) * c);
+      s[st][r] = __builtin_amdgcn_exp2f(sizeof(T) == 2 ? fmaf(s[st][r], c, off) : (s[st][r] - ms) * c);
       l += s[st][r];
     }
 }
@@ -392,8 +404,9 @@ __device__ __forceinline__ void attend(const T* Ks, const T* Vs, int n, const u3
 #pragma unroll
   for (int st = 0; st < TK / 32; ++st) s[st] = dot_rows<T, DP>(Ks, 32 * st, qf, zero16());
   softmax_step<T, DP, TK>(s, n, c, m, l, acc);
-  // p is rounded to the inputs' type for the product (16-bit types: half a step of a value in [0, 1], the size of the
-  // output's own rounding; l sums the unrounded values), the sums over keys stay in 32 bits
+  // p is rounded to the inputs' type for the product (16-bit types: half a step relative to p, down to 2^-26 of the row's
+  // largest in half precision and 2^-37 absolutely below; the size of the output's own rounding; l sums the unrounded
+  // values), the sums over keys stay in 32 bits
 #pragma unroll
   for (int st = 0; st < TK / 32; ++st) dot_cols<T, DP>(Vs, 32 * st, s[st], acc);
 }
@@ -412,9 +425,6 @@ template <typename T>
 __device__ __forceinline__ float row_stat(float lse) {
   return lse == -INFINITY ? INFINITY : sizeof(T) == 2 ? lse * kLog2e : lse;
 }
-
-// half precision: p in [0, 1] takes 2^12 into the product (p = 1 / Nk of a long list would be subnormal)
-constexpr float kHalfLog = 12.0f, kHalfP = 4096.0f;
 
 // log2 of a power of two
 __device__ __forceinline__ float log2_pow2(float x) { return (float)((int)(__float_as_uint(x) >> 23) - 127); }

@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(64 * NW, 2) fwd_kernel(FwdArgs a) {
       o[d] = round_to<T>(s * inv);
     }
     if (a.lse && threadIdx.x < 32)
-      a.lse[((int64_t)b * sh.nh + head2) * sh.Nq + n2] = L == 0.0f ? -INFINITY : M * a.scale + logf(L);
+      a.lse[((int64_t)b * sh.nh + head2) * sh.Nq + n2] = row_lse<T>(M, L, a.scale);
   } else {
     if (a.nsplit > 1) {                           // this range's sums of the wave's 32 rows
       if (!wave_live) return;
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(64 * NW, 2) fwd_kernel(FwdArgs a) {
     }
     if (!live) return;
     store_col<T, DP, VEC>((T*)a.out + ((int64_t)b * sh.Nq + n) * a.out_ld + (int64_t)head * sh.D, acc, l == 0.0f ? 0.0f : 1.0f / l, sh.D);
-    if (a.lse && h == 0) a.lse[((int64_t)b * sh.nh + head) * sh.Nq + n] = l == 0.0f ? -INFINITY : m * a.scale + logf(l);
+    if (a.lse && h == 0) a.lse[((int64_t)b * sh.nh + head) * sh.Nq + n] = row_lse<T>(m, l, a.scale);
   }
 }
 
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(256) fwd_join_kernel(FwdArgs a) {
       if (d0 + i < sh.D) op[d0 + i] = v[i];
   }
   if (a.lse && threadIdx.x < 32)
-    a.lse[((int64_t)b * sh.nh + head) * sh.Nq + n] = L == 0.0f ? -INFINITY : M * a.scale + logf(L);
+    a.lse[((int64_t)b * sh.nh + head) * sh.Nq + n] = row_lse<T>(M, L, a.scale);
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------

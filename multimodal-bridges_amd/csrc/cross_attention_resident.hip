@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 2 : 3) res_fwd_kernel(Res
     if (r < nq) {
       const int n = qlist[r];
       store_col<T, DP, VEC>((T*)a.o + ((int64_t)b * sh.Nq + n) * a.out_ld + (int64_t)(h0 + hd) * sh.D, acc, l == 0.0f ? 0.0f : 1.0f / l, sh.D);
-      if (a.lse && h == 0) a.lse[((int64_t)b * sh.nh + h0 + hd) * sh.Nq + n] = l == 0.0f ? -INFINITY : m * a.scale + logf(l);
+      if (a.lse && h == 0) a.lse[((int64_t)b * sh.nh + h0 + hd) * sh.Nq + n] = row_lse<T>(m, l, a.scale);
     }
   }
 }

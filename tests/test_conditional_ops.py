@@ -207,6 +207,29 @@ def test_cross_attention_single_key(Nk, at):
         assert not dk[0, :at[0]].any() and not dk[1, :at[1]].any()
 
 
+@pytest.mark.parametrize("B,Nq,Nk,nh,D", [(1, 300, 16384, 1, 16), (1, 1, 16384, 2, 64), (2, 130, 3000, 4, 128), (260, 20, 128, 1, 32), (64, 300, 700, 4, 33)])
+def test_cross_attention_long_tail_of_small_probabilities(B, Nq, Nk, nh, D):
+    """One key takes nearly all of a row, the others e^-18 = 2^-26 of it each: less than half of half precision's smallest step,
+    but together Nk times that.  Values are 0 at the strong key and 1024 or 2048 at the others, so the output is the tail alone.
+    Bound: p of the tail is off by one rounding to half (u), its exponent by the rounding of 18 log2(e) and of the row's offset
+    (4 x 64 E), sums of Nk terms by Nk E each in numerator and denominator; the output's own rounding."""
+    dt = torch.float16
+    at = Nk // 3
+    q, k, v = torch.zeros(B * Nq, nh * D), torch.zeros(B * Nk, nh * D), torch.full((B * Nk, nh * D), 1024.0)
+    v[1::2] = 2048.0
+    q.view(-1, nh, D)[:, :, 0] = 1.0
+    k.view(B, Nk, nh, D)[:, at, :, 0] = 18.0
+    v.view(B, Nk, nh * D)[:, at] = 0.0
+    got = run_attention(*(t.to(dt) for t in (q, k, v, torch.zeros_like(q))), None, None, B, nh, nh, 1.0)
+    tail = math.exp(-18.0)
+    tot = v.view(B, Nk, nh * D)[0, :, 0].double().sum() * tail
+    den = 1.0 + (Nk - 1) * tail
+    want = torch.full((B * Nq, nh * D), float(tot) / den, dtype=torch.float64)
+    within(got["out"], want, (u(dt) + 256 * E + 2 * (Nk + 2) * E + FN) * want + out_step(dt, want), "out")
+    lse = torch.full((B, nh, Nq), 18.0 + math.log(den), dtype=torch.float64)
+    within(got["lse"], lse, torch.full_like(lse, 4 * 18 * E + FN + (Nk + 2) * E), "lse")
+
+
 def test_cross_attention_values_that_are_not_finite():
     """A NaN in a kept key spoils the clouds and heads that see it and no others; scores of -inf take no weight."""
     B, Nq, Nk, nh, D = 2, 5, 40, 2, 16
