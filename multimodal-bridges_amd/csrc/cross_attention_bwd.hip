@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) bwd_kernel(BwdArgs
   else dq_body<T, DP, NW, VEC>(a, blockIdx.x - a.n_dkv, lds);
 }
 
-// delta of every (row, head): LP lanes a head, its chunks dealt to them
+// delta of every (row, head) of a kept slot: LP lanes a head, its chunks dealt to them
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) delta_kernel(BwdArgs a, int lp) {
   constexpr int E = Traits<T>::EPC;
@@ -296,6 +296,7 @@ __global__ void __launch_bounds__(256) delta_kernel(BwdArgs a, int lp) {
   const int sub = threadIdx.x % lp;
   for (int64_t it = (int64_t)blockIdx.x * per + threadIdx.x / lp; it < items; it += (int64_t)gridDim.x * per) {
     const int64_t row = it / sh.nh;
+    if (a.mq && a.mq[row] == 0.0f) continue;      // (a masked slot's rows are not read; all lanes of the head leave)
     const int head = (int)(it - row * sh.nh);
     const T* o = (const T*)a.out + row * a.out_ld + (int64_t)head * sh.D;
     const T* g = (const T*)a.dout + row * a.dout_ld + (int64_t)head * sh.D;

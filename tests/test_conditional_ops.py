@@ -161,6 +161,24 @@ def test_cross_attention_peaked_scores(dtype):
     check_attention(run_attention(*args, 2, 2, 1, 1.0), ref_attention(*args[:4], 2, 2, 1, *args[4:], 1.0, dt))
 
 
+def test_cross_attention_reverse_leaves_masked_queries_unread():
+    """The workspace of the reverse holds dout . out of every (cloud, head, query): nothing is found out for masked ones."""
+    import mmb_hip
+    from mmb_hip import ops
+    B, Nq, Nk, nh, D = 3, 37, 90, 2, 16
+    q, k, v, do, mq, mk = (t.cuda() for t in make(B, Nq, Nk, nh, nh, D, torch.float32, 13, True))
+    out, lse = ops.cross_attention_fwd(q, k, v, B, nh, mq=ops.mask_prepare(mq), mk=ops.mask_prepare(mk), want_lse=True)
+    grads, ws = [torch.empty_like(t) for t in (q, k, v)], torch.full((B, nh, Nq), 123.0, device="cuda")
+    ld = nh * D
+    mmb_hip.call("mmb_cross_attention_bwd", B, Nq, Nk, nh, nh, D, 0, q.data_ptr(), ld, k.data_ptr(), ld, v.data_ptr(), ld,
+                 ops.f32(mq.reshape(-1)), ops.f32(mk.reshape(-1)), D ** -0.5, out.data_ptr(), ld, do.data_ptr(), ld, ops.f32(lse),
+                 grads[0].data_ptr(), ld, grads[1].data_ptr(), ld, grads[2].data_ptr(), ld, ws.data_ptr(), ws.numel() * 4, ops.stream())
+    gone = (mq == 0)[:, None].expand(B, nh, Nq)
+    assert gone.any() and bool((ws[gone] == 123.0).all())
+    kept = (do * out).view(B, Nq, nh, D).sum(-1).transpose(1, 2)[~gone]
+    torch.testing.assert_close(ws[~gone], kept, rtol=1e-4, atol=1e-4)
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("Nq,Nk", [(40, 50), (2, 900)])
 def test_cross_attention_masked_slots_hold_anything(dtype, Nq, Nk):
