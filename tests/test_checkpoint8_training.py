@@ -113,6 +113,44 @@ def test_with_a_coder_that_loses_nothing(golden, name, dropout, monkeypatch):
         assert float((got[n] - want[n]).norm()) <= 2e-5 * float(want[n].norm()) + 1e-9, n
 
 
+class PlainCode(Lossless):
+    """The code by its definition, in 64 bits: 32 features share the smallest step 2^e with 127 steps >= the largest."""
+
+    def __init__(self, x, keep_nonzero=False):
+        M, K = x.shape
+        xb = torch.nn.functional.pad(x.double(), (0, -K % 32)).view(M, -1, 32)
+        top = xb.abs().amax(-1, keepdim=True)
+        e = torch.frexp(top / 127)[1].double()                  # 2^e > top / 127 >= 2^(e - 1)
+        step = torch.exp2(torch.where(127 * torch.exp2(e - 1) >= top, e - 1, e).clamp(min=-127))
+        c = torch.round(xb / step)
+        if keep_nonzero:
+            c = torch.where((c == 0) & (xb != 0), xb.sign(), c)
+        self.x, self.shape = (c * step).view(M, -1)[:, :K].float().contiguous(), x.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,dropout", [("tr_tiny", 0.0), ("tr_tiny", 0.2), ("tr_odd", 0.2), ("S4", 0.0), ("S4", 0.2)])
+def test_gradients_are_those_of_the_decoded_activations(golden, name, dropout, monkeypatch):
+    """The kernels' codes against the code by its definition in their place, weight gradients in 64 bits from the values it
+    stands for: what is left is the order of 32-bit sums, as with the lossless coder above."""
+    from mmb_hip import ops
+    g, model = build(golden, name, 8, dropout)
+    model = model.cuda().train()
+    step(g, model)
+    got = grads(model)
+    used = []
+    monkeypatch.setattr(ops, "checkpoint_rows", lambda x, keep_nonzero=False: used.append(keep_nonzero) or PlainCode(x, keep_nonzero))
+    monkeypatch.setattr(ops, "restore_rows", lambda q, dtype=None, out=None: out.copy_(q.x))
+    monkeypatch.setattr(ops, "grad_weight_rows_q8", PlainCode.grad_weight)
+    g, model = build(golden, name, 8, dropout)
+    model = model.cuda().train()
+    step(g, model)
+    want = grads(model)
+    assert any(used) and not all(used) and got.keys() == want.keys()
+    for n in want:
+        assert float((got[n] - want[n]).norm()) <= 2e-5 * float(want[n].norm()) + 1e-9, n
+
+
 @pytest.mark.gpu
 def test_memory_held_between_the_passes(golden):
     """What the tape holds when the forward is done: the layers' matrices at 33/128 of their size; the other tensors (both
