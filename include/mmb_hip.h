@@ -437,7 +437,8 @@ int mmb_attention_dropout_mask(int B, int N, int nheads, const float* maskf, int
  * nheads_kv divides nheads: query heads h*g .. h*g+g-1 share key head h (g = nheads / nheads_kv).  1 <= D <= 128,
  * Nk <= 2^31 - 4097, nheads * Nq and B * nheads <= 2^30, fewer than 2^32 threads in a launch (some 2^24 clouds x key heads);
  * dtype MMB_DT_*: q, k, v, out (sums, softmax and lse in 32 bits; with 16-bit types the probabilities are rounded to the type
- * for the product with v).  maskf_q (B,Nq), maskf_k (B,Nk) | NULL: slots with 0 take no part -- their rows are
+ * for the product with v).  A score is a 32-bit sum: p is within |s_ij| 2^-22 or so of itself, and scores past 2^24 mean
+ * nothing (16-bit types: may give NaN).  maskf_q (B,Nq), maskf_k (B,Nk) | NULL: slots with 0 take no part -- their rows are
  * not read (whatever they hold), a masked query gets a zero row and lse -inf, as does a query without a kept key.
  * lse (B,nheads,Nq) | NULL.  scale > 0.  workspace: device memory of the size mmb_cross_attention_workspace gives for the
  * same arguments (0: none), owned by this call until it has run: two calls that may overlap (streams, captured graphs)
@@ -505,15 +506,16 @@ int mmb_head_norm_rotate_bwd(int64_t M, int nheads, int nheads2, int D, int dtyp
 /* Activations kept for the reverse pass in 8 bits.  32 consecutive features of a row share a step 2^e, e the smallest
  * exponent >= -127 with 127 * 2^e >= max |x|; codes (M, 32*ceil(K/32)) int8 = round(x / 2^e), ties to even, features past K
  * zero; steps (M, ceil(K/32)) uint8 = e + 127, 255 for a block that holds an infinity or NaN (it is restored as NaN).
- * |restored - x| <= 2^(e-1).  keep_nonzero != 0: values other than 0 get code +-1 at least (ReLU outputs: the gate is the same
- * from the checkpoint; |restored - x| < 2^e).  x: M rows of K, dtype MMB_DT_*.  codes 16-byte aligned.  Outputs of
- * these calls overlap no input and not each other. */
+ * |restored - x| <= 2^(e-1); where max |x| > 127 * 2^121 (e = 122) codes end at +-63, 64 steps being no float: < 2^e there.
+ * keep_nonzero != 0: values other than 0 get code +-1 at least (ReLU outputs: the gate is the same from the checkpoint;
+ * |restored - x| < 2^e).  x: M rows of K, dtype MMB_DT_*.  codes 16-byte aligned.  Outputs of these calls overlap no input and
+ * not each other. */
 int mmb_checkpoint_rows(int64_t M, int K, int dtype, int keep_nonzero, const void* x, int64_t x_ld, void* codes, void* steps, void* stream);
-/* y (M, K) = code * 2^e, rounded to dtype (exact in float and bf16) */
+/* y (M, K) = code * 2^e, rounded to dtype (exact in float and bf16; what lies past the largest half becomes it) */
 int mmb_restore_rows(int64_t M, int K, int dtype, const void* codes, const void* steps, void* y, int64_t y_ld, void* stream);
 /* Weight gradient of a Linear straight from its input's checkpoint: dW (N, K) = dZ^T Xhat, db (N) | NULL = column sums of
  * dZ (M, N) (dtype MMB_DT_*); accumulate != 0: added to what dW, db hold.  Products are exact (a code times a power of two
- * is one bf16 value, dZ is split into bf16 planes without loss), sums in 32 bits in a fixed order.  Infinite or NaN
+ * is one bf16 value, dZ is split into bf16 planes without loss down to 2^-133), sums in 32 bits in a fixed order.  Infinite or NaN
  * gradients give non-finite sums.  workspace: the size that mmb_grad_weight_rows_q8_workspace gives (bytes_host: HOST). */
 int mmb_grad_weight_rows_q8(int64_t M, int K, int N, int dtype, const void* codes, const void* steps, const void* dZ,
                             int64_t dz_ld, float* dW, int64_t dw_ld, float* db, int accumulate, void* workspace,

@@ -2,7 +2,9 @@
 //
 // 32 consecutive features of a row share a step 2^e: e is the smallest exponent (>= -127) with 127 * 2^e >= max |x|, the
 // codes are round(x / 2^e) in [-127, 127], ties to even.  Both divisions are by powers of two, so a code depends on no
-// rounding but its own, and a value stands for at most half a step off: |xhat - x| <= 2^(e-1) <= max|x| / 127.  An integer
+// rounding but its own, and a value stands for at most half a step off: |xhat - x| <= 2^(e-1), which is below max|x| / 127
+// but for blocks of subnormals (e = -127 is the smallest).  At the other end, e = 122, 64 steps would be 2^128: codes end at
+// 63 there and the values next to the largest float are up to a step off.  An integer
 // grid over a shared step holds a block of like-sized activations about four times closer than an 8-bit float would (whose
 // three mantissa bits spend the range on small values).
 // With keep_nonzero a value that would round to code 0 takes code +-1 (a step off at most, not half): what is told from the

@@ -389,6 +389,9 @@ def _ln_bwd(e, store, produced, arena):
         gx, fresh = store.target(x)
     else:
         gx, fresh = torch.empty(x.shape, dtype=torch.float32, device=x.device), True
+    # an x kept in 8 bits meets the mean and deviation of the exact rows: those of the decoded rows would be further from what
+    # the forward computed (relative error of dx at D = 64: 1.5e-3 against 1.8e-3; rows with one feature 30 times the others,
+    # D = 384: 0.9e-3 against 1.7e-3).  The attention needs its own log-sum again because its probabilities must sum to one.
     with store.kept.restored(x):
         ops.layernorm_bwd(x, norm.weight.detach(), stats, g, gx, not fresh, dgamma, dbeta)
     if not direct:
