@@ -387,31 +387,28 @@ __global__ void __launch_bounds__(2 * BN, 2) gw_kernel(GwArgs a) {
 
 // dW, db from the partial sums of the row ranges: eight threads share the ranges of one element, joined in LDS
 __global__ void __launch_bounds__(256)
-gw_fold_kernel(int splits, int64_t nw, int N, int K, const float* __restrict__ pw, const float* __restrict__ pb, float* __restrict__ dW,
-               int64_t dw_ld, float* __restrict__ db, int accumulate) {
+gw_fold_kernel(int64_t first, int splits, int64_t nw, int N, int K, const float* __restrict__ pw, const float* __restrict__ pb,
+               float* __restrict__ dW, int64_t dw_ld, float* __restrict__ db, int accumulate) {
   __shared__ float red[8][33];
   const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
-  for (int64_t i0 = (int64_t)blockIdx.x * 32; i0 < nw + N; i0 += (int64_t)gridDim.x * 32) {
-    const int64_t i = i0 + c;
-    float s = 0.0f;
-    if (i < nw) {
+  const int64_t i = first + (int64_t)blockIdx.x * 32 + c;
+  float s = 0.0f;
+  if (i < nw) {
 #pragma unroll 4
-      for (int p = g; p < splits; p += 8) s += pw[(int64_t)p * nw + i];
-    } else if (i < nw + N) {
-      for (int p = g; p < splits; p += 8) s += pb[(int64_t)p * N + (i - nw)];
-    }
-    __syncthreads();                               // (the sums of the turn before have been read)
-    red[g][c] = s;
-    __syncthreads();
-    if (g != 0 || i >= nw + N) continue;
+    for (int p = g; p < splits; p += 8) s += pw[(int64_t)p * nw + i];
+  } else if (i < nw + N) {
+    for (int p = g; p < splits; p += 8) s += pb[(int64_t)p * N + (i - nw)];
+  }
+  red[g][c] = s;
+  __syncthreads();
+  if (g != 0 || i >= nw + N) return;
 #pragma unroll
-    for (int q = 1; q < 8; ++q) s += red[q][c];
-    if (i < nw) {
-      float* d = dW + i / K * dw_ld + i % K;
-      *d = accumulate ? *d + s : s;
-    } else if (db) {
-      db[i - nw] = accumulate ? db[i - nw] + s : s;
-    }
+  for (int q = 1; q < 8; ++q) s += red[q][c];
+  if (i < nw) {
+    float* d = dW + i / K * dw_ld + i % K;
+    *d = accumulate ? *d + s : s;
+  } else if (db) {
+    db[i - nw] = accumulate ? db[i - nw] + s : s;
   }
 }
 
@@ -489,11 +486,15 @@ static int pick_tile(const GwArgs& a, const GwPlan& p, hipStream_t st) {
 template <typename T>
 static int grad_weight(GwArgs& a, const GwPlan& p, float* dW, int64_t dw_ld, float* db, int accumulate, hipStream_t st) {
   const bool vec = a.N % 8 == 0 && ((uintptr_t)a.dz & 15) == 0 && a.dz_ld * (int64_t)sizeof(T) % 16 == 0 && a.dz_ld < (1 << 24);
-  const int64_t nw = (int64_t)a.N * a.K, fold = (nw + a.N + 31) / 32, most = 1 << 23;
+  const int64_t nw = (int64_t)a.N * a.K, fold = (nw + a.N + 31) / 32, most = 1 << 23;      // (blocks of one launch)
   int rc = vec ? pick_tile<T, true>(a, p, st) : pick_tile<T, false>(a, p, st);
   if (rc != MMB_OK) return rc;
-  gw_fold_kernel<<<(unsigned)(fold < most ? fold : most), 256, 0, st>>>(a.splits, nw, a.N, a.K, a.pw, a.pb, dW, dw_ld, db, accumulate);
-  return check_launch("mmb_grad_weight_rows_q8 (fold)");
+  for (int64_t at = 0; at < fold && rc == MMB_OK; at += most) {
+    gw_fold_kernel<<<(unsigned)(fold - at < most ? fold - at : most), 256, 0, st>>>(at * 32, a.splits, nw, a.N, a.K, a.pw, a.pb, dW, dw_ld, db,
+                                                                                    accumulate);
+    rc = check_launch("mmb_grad_weight_rows_q8 (fold)");
+  }
+  return rc;
 }
 
 }  // namespace ckpt
