@@ -252,10 +252,11 @@ struct Plan {
     return nsplit > 1 ? (int64_t)s.B * s.nkv * tiles * (split ? 1 : nw) * nsplit * 32 * (pad_width(s.D) + 2) * 4 : 0;
   }
 };
-// Team form: 32 rows a wave, as many waves (1, 2, 4) as a cloud's rows fill, eight where those still give every CU two
-// workgroups: the more waves share a tile, the less of it each has to load (4096 x 5000 slots, bf16: 373 us with eight, 424
-// with four; 2047 x 4099, where eight would leave CUs idle: 325 against 298).  Split form when the team form would put
-// fewer than one workgroup on each of the 256 CUs, or one 32-row tile holds all rows, and there are keys to split.
+// Team form: 32 rows a wave, as many waves (1, 2, 4) as a cloud's rows fill, eight where that still leaves every CU two
+// workgroups (they run one after the other, two waves a SIMD): the more waves share a tile, the less of it each has to load
+// (4096 x 5000 slots, bf16: 364..388 us with eight, 424 with four; 2047 x 4099, where eight would leave CUs idle: 325 against
+// 298).  Split form when the team form would put fewer than one workgroup on each of the 256 CUs, or one 32-row tile holds all
+// rows, and there are keys to split.
 static Plan fwd_plan(const Shape& s) {
   const int64_t R = (int64_t)s.g * s.Nq, pairs = (int64_t)s.B * s.nkv;
   Plan p;
@@ -275,8 +276,12 @@ static Plan fwd_plan(const Shape& s) {
     p.chunk = (p.chunk + 31) / 32 * 32;
   } else if (p.nw == 4 && s.Nk >= 2560 && pairs * p.tiles < 512) {
     // the team form alone leaves CUs with one workgroup, whose four waves do not hide each other's latencies: the keys in two
-    // ranges and a second launch that joins them (2047 x 4099 slots, 16 heads on 8, fp16, D = 64: 79 us with two ranges, 93
-    // with one; masked 57, 72; bf16, D = 128: 115, 157; 2048 keys: 50, 47; two such clouds, masked: the same within 3 %)
+    // ranges and a second launch that joins them.  us with two ranges, with one, for 2047 slots, 16 heads on 8:
+    //   fp16, D = 64     2560 keys 49, 55    4099 keys 69, 85    (masked 63, 73 and 54, 70)
+    //   bf16, D = 128    2560 keys 71, 92    4099 keys 103, 144
+    //   float, D = 32    2560 keys 114, 129  4099 keys 180, 206
+    // Shorter lists gain less (fp16: 2048 keys 44, 46; 1800 keys 44, 45) and keep one range and one launch; two such clouds,
+    // masked: the same within 3 %.
     p.nsplit = 2;
     p.chunk = ((s.Nk + 1) / 2 + 63) / 64 * 64;
   }
