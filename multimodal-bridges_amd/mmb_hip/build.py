@@ -11,7 +11,7 @@ LIB = os.path.join(HERE, os.environ.get("MMB_LIB_NAME", "libmmb_hip.so"))      #
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # max-memory-clause: the fused kernels live on the 256-VGPR limit; this pre-RA strategy spills less there (S3 generation
 # kernel 168 -> 144 B/lane of scratch, S2 112 -> 68, training forward 392 -> 316) and measured +2..5 % on every bench
-# line (DESIGN section 2)
+# line
 # no packed float arithmetic: some of its forms have given wrong results on this machine without an error
 FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-Wall", "-Wno-unused-function",
