@@ -172,8 +172,10 @@ __device__ __forceinline__ u32x4 read_cols(const uint16_t* p, int pitch) {
 template <typename T, int BN, int BK>
 constexpr int gw_lds() { return 2 * MS * (Planes<T>::n * pitch_of(BN) + pitch_of(BK)) * 2; }
 
+// (No instance may spill registers: the compiler has stored one under a narrowed exec mask and read it back for all lanes.  One
+// wave a SIMD for 128 x 256 tiles of float -- their LDS admits no more -- and of half precision element by element.)
 template <typename T, int BN, int BK, bool VEC>
-__global__ void __launch_bounds__(2 * BN, 2) gw_kernel(GwArgs a) {
+__global__ void __launch_bounds__(2 * BN, BN < BK && (Planes<T>::n == 3 || (Planes<T>::n == 2 && !VEC)) ? 1 : 2) gw_kernel(GwArgs a) {
   constexpr int NT = 2 * BN, NWN = BN / 64;
   constexpr int PL = Planes<T>::n, PA = pitch_of(BN), PB = pitch_of(BK), NJ = BK / 64, XC = MS * BK / 16 / NT;
   extern __shared__ __attribute__((aligned(16))) uint16_t gw_sm[];

@@ -92,6 +92,12 @@ __device__ __forceinline__ void wave_sync() {
 // selecting afterwards (it does so for the tail of the keys and for rescaling, at three instructions an element).
 __device__ __forceinline__ void rarely() { asm volatile(""); }
 
+// a value that the compiler takes for another one: what is computed from it is computed again, not kept
+__device__ __forceinline__ int again(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 constexpr int kChunk = 512;                       // raw slots one compaction step looks at
 
 // Appends the slots n in [lo, min(lo + kChunk, hi)) with maskf[n] != 0 to list[], in order; returns how many.
@@ -326,8 +332,8 @@ struct ColScale {
 
 // column `lane & 31` of acc (features x columns) times mul -> one row of D features
 template <typename T, int DP, bool VEC>
-__device__ __forceinline__ void store_col(T* __restrict__ p, const f32x16* acc, float mul, int D) {
-  const int h = (threadIdx.x & 63) >> 5;
+__device__ __forceinline__ void store_col(T* __restrict__ p, const f32x16* acc, float mul, int D, int tid = threadIdx.x) {
+  const int h = (tid & 63) >> 5;
 #pragma unroll
   for (int t = 0; t < feature_tiles<DP>(); ++t)
 #pragma unroll

@@ -37,8 +37,9 @@ struct FwdArgs {
 template <typename T, int DP, int TK, bool SPLIT>
 constexpr int kv_lds() { return 2 * (SPLIT ? 1 : 2) * tile_bytes<T, DP, TK>(); }
 
+// No instance may spill registers (the reverse says why): one wave a SIMD where the tiles in LDS admit no more anyway.
 template <typename T, int DP, int NW, int TK, bool SPLIT, bool VEC>
-__global__ void __launch_bounds__(64 * NW, 2) fwd_kernel(FwdArgs a) {
+__global__ void __launch_bounds__(64 * NW, DP == 128 && sizeof(T) == 4 && (NW < 4 || SPLIT) ? 1 : 2) fwd_kernel(FwdArgs a) {
   constexpr int NT = 64 * NW, TEAM = SPLIT ? 1 : NW, TT = 64 * TEAM, ROWS = SPLIT ? 32 : 32 * NW;
   constexpr int TILE = kv_lds<T, DP, TK, SPLIT>(), NTILE = SPLIT ? NW : 1;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -111,8 +112,9 @@ __global__ void __launch_bounds__(64 * NW, 2) fwd_kernel(FwdArgs a) {
     SlotTiles<TEAM>::sync();                      // (team: whoever passes here has read the other buffer)
     // the next tile's rows come in while this one is worked on; issued behind the barrier, where finding their addresses
     // overlaps with this tile's products
-    kr.template load<VEC>(tid, nn, sh.D, [&](int i) { return kb + (int64_t)keys.slot(i) * a.k_ld; });
-    vr.template load<VEC>(tid, nn, sh.D, [&](int i) { return vb + (int64_t)keys.slot(i) * a.v_ld; });
+    const int lt = SPLIT ? again(threadIdx.x) & 63 : VEC ? tid : again(threadIdx.x);
+    kr.template load<VEC>(lt, nn, sh.D, [&](int i) { return kb + (int64_t)keys.slot(i) * a.k_ld; });
+    vr.template load<VEC>(lt, nn, sh.D, [&](int i) { return vb + (int64_t)keys.slot(i) * a.v_ld; });
     if (wave_live) attend<T, DP, TK>(Ks, Vs, nk, qf, c, m, l, acc);         // (a wave without rows only helps to load)
     nk = nn;
   }
@@ -187,8 +189,12 @@ __global__ void __launch_bounds__(64 * NW, 2) fwd_kernel(FwdArgs a) {
       return;
     }
     if (!live) return;
-    store_col<T, DP, VEC>((T*)a.out + ((int64_t)b * sh.Nq + n) * a.out_ld + (int64_t)head * sh.D, acc, l == 0.0f ? 0.0f : 1.0f / l, sh.D);
-    if (a.lse && h == 0) a.lse[((int64_t)b * sh.nh + head) * sh.Nq + n] = row_lse<T>(m, l, a.scale);
+    const int t = again(threadIdx.x);             // (places found again, not kept in registers through the walk)
+    int n_out = -1, gi_out = 0;
+    rt.locate(again(r0) + (t >> 6) * 32 + (t & 31), sh.Nq, mq != nullptr, n_out, gi_out);
+    const int head_out = hk * sh.g + gi_out;
+    store_col<T, DP, VEC>((T*)a.out + ((int64_t)b * sh.Nq + n_out) * a.out_ld + (int64_t)head_out * sh.D, acc, l == 0.0f ? 0.0f : 1.0f / l, sh.D, t);
+    if (a.lse && (t & 32) == 0) a.lse[((int64_t)b * sh.nh + head_out) * sh.Nq + n_out] = row_lse<T>(m, l, a.scale);
   }
 }
 
@@ -320,7 +326,7 @@ static int pick_nw(const Plan& p, const FwdArgs& a, hipStream_t st) {
   if (p.split) return launch_fwd<T, DP, 4, 32, true, VEC>(a, st);
   if (p.nw == 8) return launch_fwd<T, DP, 8, TK, false, VEC>(a, st);
   if (p.nw == 4) return launch_fwd<T, DP, 4, TK, false, VEC>(a, st);
-  if (p.nw == 2) return launch_fwd<T, DP, 2, TK, false, VEC>(a, st);
+  if (p.nw == 2) return launch_fwd<T, DP, 2, DP == 128 ? 32 : TK, false, VEC>(a, st);
   return launch_fwd<T, DP, 1, 32, false, VEC>(a, st);
 }
 template <typename T, bool VEC>

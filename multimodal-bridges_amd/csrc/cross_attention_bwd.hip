@@ -102,8 +102,9 @@ __device__ __forceinline__ void dq_body(const BwdArgs& a, int64_t id, char* lds)
     vr.store(threadIdx.x, Vs);
     const int nn = keys.next(TK);
     SlotTiles<NW>::sync();
-    kr.template load<VEC>(threadIdx.x, nn, sh.D, [&](int i) { return kb + (int64_t)keys.slot(i) * a.k_ld; });
-    vr.template load<VEC>(threadIdx.x, nn, sh.D, [&](int i) { return vb + (int64_t)keys.slot(i) * a.v_ld; });
+    const int lt = again(threadIdx.x);
+    kr.template load<VEC>(lt, nn, sh.D, [&](int i) { return kb + (int64_t)keys.slot(i) * a.k_ld; });
+    vr.template load<VEC>(lt, nn, sh.D, [&](int i) { return vb + (int64_t)keys.slot(i) * a.v_ld; });
     if (!wave_live) {                             // a wave without rows only helps to load
       nk = nn;
       continue;
@@ -149,9 +150,13 @@ __device__ __forceinline__ void dq_body(const BwdArgs& a, int64_t id, char* lds)
     nk = nn;
   }
   if (!live) return;
-  if (a.few_keys && h == 0) a.delta[stat] = delta;
-  store_col<T, DP, VEC>((T*)a.dq + flat * a.dq_ld + (int64_t)head * sh.D, acc,
-                        __is_same(T, _Float16) ? a.scale / cs.sc : a.scale, sh.D);
+  const int tid = again(threadIdx.x);              // (places found again, not kept in registers through the walk)
+  int n_out = -1, gi_out = 0;
+  rt.locate(again(r0) + (tid >> 6) * 32 + (tid & 31), sh.Nq, mq != nullptr, n_out, gi_out);
+  const int head_out = hk * sh.g + gi_out;
+  if (a.few_keys && (tid & 32) == 0) a.delta[((int64_t)b * sh.nh + head_out) * sh.Nq + n_out] = delta;
+  store_col<T, DP, VEC>((T*)a.dq + ((int64_t)b * sh.Nq + n_out) * a.dq_ld + (int64_t)head_out * sh.D, acc,
+                        __is_same(T, _Float16) ? a.scale / cs.sc : a.scale, sh.D, tid);
 }
 
 template <typename T, int DP, int NW, bool VEC>
@@ -214,8 +219,9 @@ __device__ __forceinline__ void dkv_body(const BwdArgs& a, int64_t id, char* lds
         const int s = i / nh;
         return base + (int64_t)rows.slot(s) * ld + (i - s * nh) * sh.D;
       };
-      qr.template load<VEC>(threadIdx.x, n, sh.D, [&](int i) { return at(i, qb, a.q_ld); });
-      gr.template load<VEC>(threadIdx.x, n, sh.D, [&](int i) { return at(i, gb, a.dout_ld); });
+      const int lt = again(threadIdx.x);
+      qr.template load<VEC>(lt, n, sh.D, [&](int i) { return at(i, qb, a.q_ld); });
+      gr.template load<VEC>(lt, n, sh.D, [&](int i) { return at(i, gb, a.dout_ld); });
       st_l = -INFINITY;
       if (threadIdx.x < TQ && threadIdx.x < n) {  // (both loads at once; looked at when the tile is stored)
         const int s = (int)threadIdx.x / nh;
@@ -229,8 +235,9 @@ __device__ __forceinline__ void dkv_body(const BwdArgs& a, int64_t id, char* lds
       T* Qs = tiles + buf * 2 * TILE_E;
       T* Gs = Qs + TILE_E;
       float* sl = stats + buf * 2 * TQ;
-      qr.store(threadIdx.x, Qs);
-      gr.store(threadIdx.x, Gs);
+      const int ts = again(threadIdx.x);
+      qr.store(ts, Qs);
+      gr.store(ts, Gs);
       if (threadIdx.x < TQ) {
         const float x = row_stat<T>(st_l);        // rows past the end, and rows without a key: p = 0
         sl[threadIdx.x] = __is_same(T, _Float16) ? x - kHalfLog : x;
@@ -271,17 +278,31 @@ __device__ __forceinline__ void dkv_body(const BwdArgs& a, int64_t id, char* lds
       nq = nn;
     }
   }
-  if (key < 0) return;
+  const int tid = again(threadIdx.x), place = (tid >> 6) * 32 + (tid & 31), kc_out = again(k0) + place;
+  const int key_out = mk ? klist[place] : (kc_out < sh.Nk ? kc_out : -1);
+  if (key_out < 0) return;
+  const int64_t out = (int64_t)b * sh.Nk + key_out;
   // (dp carried p's 2^12 too)
-  store_col<T, DP, VEC>((T*)a.dk + flat * a.dk_ld + (int64_t)hk * sh.D, dk,
-                        __is_same(T, _Float16) ? a.scale / kHalfP / cs.sc : a.scale, sh.D);
-  store_col<T, DP, VEC>((T*)a.dv + flat * a.dv_ld + (int64_t)hk * sh.D, dv,
-                        __is_same(T, _Float16) ? 1.0f / kHalfP : 1.0f, sh.D);
+  store_col<T, DP, VEC>((T*)a.dk + out * a.dk_ld + (int64_t)hk * sh.D, dk,
+                        __is_same(T, _Float16) ? a.scale / kHalfP / cs.sc : a.scale, sh.D, tid);
+  store_col<T, DP, VEC>((T*)a.dv + out * a.dv_ld + (int64_t)hk * sh.D, dv,
+                        __is_same(T, _Float16) ? 1.0f / kHalfP : 1.0f, sh.D, tid);
+}
+
+// Waves a SIMD that an instance leaves registers for.  None may spill: the compiler stored a spilled register under a narrowed
+// exec mask and read it back for all lanes (bfloat16 heads of 33 .. 63 off the chunk of eight on two waves: delta went to
+// whatever address scratch memory held).  So two only where 256 registers are enough; again() keeps what is cheap to find out of
+// them.
+template <typename T, int DP, int NW, bool VEC>
+constexpr int bwd_waves() {
+  if (DP == 128) return 1;
+  if (DP == 64 && (NW == 1 || (NW == 2 && sizeof(T) == 2 && !VEC))) return 1;
+  return 2;
 }
 
 // workgroups [0, n_dkv) own keys, the others query rows
 template <typename T, int DP, int NW, bool VEC>
-__global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) bwd_kernel(BwdArgs a) {
+__global__ void __launch_bounds__(64 * NW, (bwd_waves<T, DP, NW, VEC>())) bwd_kernel(BwdArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   if (blockIdx.x < a.n_dkv) dkv_body<T, DP, NW, VEC>(a, blockIdx.x, lds);
   else dq_body<T, DP, NW, VEC>(a, blockIdx.x - a.n_dkv, lds);
@@ -361,7 +382,11 @@ static int run_bwd(BwdArgs& a, hipStream_t st) {
 template <typename T, int DP, bool VEC>
 static int pick_nw(BwdArgs& a, hipStream_t st) {
   const int64_t R = (int64_t)a.sh.g * a.sh.Nq, m = R > a.sh.Nk ? R : a.sh.Nk;
-  return m > 64 ? run_bwd<T, DP, 4, VEC>(a, st) : m > 32 ? run_bwd<T, DP, 2, VEC>(a, st) : run_bwd<T, DP, 1, VEC>(a, st);
+  if (m > 64) return run_bwd<T, DP, 4, VEC>(a, st);
+  // (one wave alone would need more than 512 registers for tiles of 128-wide heads)
+  if constexpr (DP < 128)
+    if (m <= 32) return run_bwd<T, DP, 1, VEC>(a, st);
+  return run_bwd<T, DP, 2, VEC>(a, st);
 }
 template <typename T, bool VEC>
 static int pick_dp(BwdArgs& a, hipStream_t st) {

@@ -57,8 +57,9 @@ __device__ __forceinline__ void fill2(T* __restrict__ d0, T* __restrict__ d1, co
   }
 }
 
+// (no instance here may spill registers: cross_attention_bwd.hip says why)
 template <typename T, int DP, int NW, bool VEC>
-__global__ void __launch_bounds__(64 * NW, DP == 128 ? 2 : 3) res_fwd_kernel(ResArgs a) {
+__global__ void __launch_bounds__(64 * NW, DP < 128 ? 3 : sizeof(T) == 4 && !VEC ? 1 : 2) res_fwd_kernel(ResArgs a) {
   using R = ResTile<T, DP>;
   constexpr int S = DP / (2 * R::E);
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -122,14 +123,14 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 2 : 3) res_fwd_kernel(Res
     l += __shfl_xor(l, 32);
     if (r < nq) {
       const int n = qlist[r];
-      store_col<T, DP, VEC>((T*)a.o + ((int64_t)b * sh.Nq + n) * a.out_ld + (int64_t)(h0 + hd) * sh.D, acc, l == 0.0f ? 0.0f : 1.0f / l, sh.D);
+      store_col<T, DP, VEC>((T*)a.o + ((int64_t)b * sh.Nq + n) * a.out_ld + (int64_t)(h0 + hd) * sh.D, acc, l == 0.0f ? 0.0f : 1.0f / l, sh.D, again(threadIdx.x));
       if (a.lse && h == 0) a.lse[((int64_t)b * sh.nh + h0 + hd) * sh.Nq + n] = row_lse<T>(m, l, a.scale);
     }
   }
 }
 
 template <typename T, int DP, int NW, bool VEC>
-__global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(ResArgs a) {
+__global__ void __launch_bounds__(64 * NW, DP == 128 || (DP == 64 && sizeof(T) == 4 && !VEC) ? 1 : 2) res_bwd_kernel(ResArgs a) {
   using R = ResTile<T, DP>;
   constexpr int S = DP / (2 * R::E), E = R::E;
   constexpr bool HALF = __is_same(T, _Float16);
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(Res
       dot_cols<T, DP>(kh, kt0, s, acc);
     }
     if (r0 + col < nq)
-      store_col<T, DP, VEC>((T*)a.dq + (qrow + qlist[r0 + col]) * a.dq_ld + (int64_t)(h0 + hd) * sh.D, acc, HALF ? a.scale / cs.sc : a.scale, sh.D);
+      store_col<T, DP, VEC>((T*)a.dq + (qrow + qlist[r0 + col]) * a.dq_ld + (int64_t)(h0 + hd) * sh.D, acc, HALF ? a.scale / cs.sc : a.scale, sh.D, again(threadIdx.x));
   }
   // ---- dk, dv: queries resident
   u32x4 kf[S], vf[S];
@@ -263,6 +264,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(Res
   for (int gi = 0; gi < heads; ++gi)
     fill2<T, DP, 64 * NW, VEC>(A0 + gi * qs, A1 + gi * qs, qb + (int64_t)gi * sh.D, a.q_ld, gb + (int64_t)gi * sh.D, a.dout_ld, qlist, nq, sh.D);
   __syncthreads();
+  const int h2 = (again(threadIdx.x) & 63) >> 5;
   for (int it = wave; it < kt; it += NW) {
     const int r = it * 32 + col;
     if (it != wave) fetch_k(it);
@@ -283,8 +285,8 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(Res
         f32x16 dp = dot_rows<T, DP>(gh, q0, vf, zero16());
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4) {
-          const f32x4 ls = *reinterpret_cast<const f32x4*>(lh + q0 + 8 * g4 + 4 * h);
-          const f32x4 dl = *reinterpret_cast<const f32x4*>(dh + q0 + 8 * g4 + 4 * h);
+          const f32x4 ls = *reinterpret_cast<const f32x4*>(lh + q0 + 8 * g4 + 4 * h2);
+          const f32x4 dl = *reinterpret_cast<const f32x4*>(dh + q0 + 8 * g4 + 4 * h2);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int r2 = 4 * g4 + i;
@@ -303,8 +305,9 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) res_bwd_kernel(Res
     }
     if (r < nk) {
       const int64_t n = krow + klist[r];
-      store_col<T, DP, VEC>((T*)a.dk + n * a.dk_ld + (int64_t)hk * sh.D, dk, HALF ? a.scale / kHalfP / cs.sc : a.scale, sh.D);
-      store_col<T, DP, VEC>((T*)a.dv + n * a.dv_ld + (int64_t)hk * sh.D, dv, HALF ? 1.0f / kHalfP : 1.0f, sh.D);
+      const int t = again(threadIdx.x);           // (feature places found again: no register to spare for them)
+      store_col<T, DP, VEC>((T*)a.dk + n * a.dk_ld + (int64_t)hk * sh.D, dk, HALF ? a.scale / kHalfP / cs.sc : a.scale, sh.D, t);
+      store_col<T, DP, VEC>((T*)a.dv + n * a.dv_ld + (int64_t)hk * sh.D, dv, HALF ? 1.0f / kHalfP : 1.0f, sh.D, t);
     }
   }
 }

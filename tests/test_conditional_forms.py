@@ -167,6 +167,25 @@ def test_eight_waves_with_several_row_tiles(D, masked, dtype):
     check_attention(run_attention(*args, B, nh, nh, scale), ref_attention(*args[:4], B, nh, nh, *args[4:], scale, TYPES[dtype]))
 
 
+# rows of a head's group, keys: the streaming form on one, two and four waves a workgroup, delta from the row's own p (at most
+# 32 keys) and from a launch of its own
+SMALL = [(4, 21, 8, 8, 4), (3, 9, 20, 2, 2), (3, 9, 60, 2, 1), (2, 30, 32, 3, 3), (5, 2, 33, 4, 2), (2, 1, 1, 2, 1), (2, 70, 30, 2, 1), (2, 7, 130, 3, 1)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("D", [1, 20, 24, 32, 33, 40, 63, 64, 65, 72, 100, 127, 128])
+def test_every_instance_of_the_streaming_form(D, dtype):
+    """All head widths (padded to 32, 64, 128; in chunks and element by element) at every number of waves, masked and not.  The
+    bounds' sum of first-order errors is widened by 2^-9: two roundings at their worst are 2u + u^2 off, not 2u."""
+    dt = TYPES[dtype]
+    for i, (B, Nq, Nk, nh, nkv) in enumerate(SMALL):
+        print(D, dtype, (B, Nq, Nk, nh, nkv), flush=True)
+        args = make(B, Nq, Nk, nh, nkv, D, dt, 100 * i + D, bool(i % 2))
+        scale = 1.0 / math.sqrt(D)
+        ref = ref_attention(*args[:4], B, nh, nkv, *args[4:], scale, dt)
+        check_attention(run_attention(*args, B, nh, nkv, scale), {n: (v, t * (1 + 2.0 ** -9)) for n, (v, t) in ref.items()})
+
+
 # M, K, N: tiles of 256 x 256 and of 128 x 256, rows of dZ loaded in chunks (N a multiple of 8); ranges of several steps
 GRADS = [(700, 264, 248), (2000, 1024, 1000), (515, 320, 64), (900, 320, 320), (65, 256, 256), (31, 136, 136), (3000, 130, 520)]
 

@@ -251,3 +251,32 @@ def test_workspace_query_refuses_what_the_call_refuses():
     for N, K in (((1 << 20) + 1, 8), (8, (1 << 20) + 1), (2 ** 31 - 1, 2 ** 31 - 1)):
         rc, msg = rc_of("mmb_grad_weight_rows_q8_workspace", 8, N, K, C.byref(n))
         assert rc == -1 and b"at most 2^20" in msg, msg
+
+
+def kernels_of(path):
+    """Names and resources of the GPU kernels in a library: the metadata notes of the code objects that it carries."""
+    import struct
+    msgpack = pytest.importorskip("msgpack")
+    data = open(path, "rb").read()
+    at = data.find(b"\x7fELF\x02\x01\x01\x40")
+    while at >= 0:
+        if struct.unpack_from("<H", data, at + 18)[0] == 224:       # a GPU's machine number
+            table, count = struct.unpack_from("<Q", data, at + 40)[0], struct.unpack_from("<H", data, at + 60)[0]
+            for i in range(count):
+                section = at + table + 64 * i
+                if struct.unpack_from("<I", data, section + 4)[0] == 7:                     # notes
+                    note = at + struct.unpack_from("<Q", data, section + 24)[0]
+                    name, size, _ = struct.unpack_from("<III", data, note)
+                    start = note + 12 + (name + 3) // 4 * 4
+                    yield from msgpack.unpackb(data[start:start + size], strict_map_key=False)["amdhsa.kernels"]
+        at = data.find(b"\x7fELF\x02\x01\x01\x40", at + 4)
+
+
+def test_no_kernel_of_the_conditional_operators_spills_registers():
+    """The compiler has stored a spilled register under a narrowed exec mask and read it back for all lanes: the reverse of cross
+    attention (bfloat16, head widths off the chunk of eight between 33 and 63, two waves, at most 32 keys) then wrote to
+    addresses that scratch memory happened to hold.  Without spills there is nothing to misplace."""
+    import mmb_hip
+    ours = [k for k in kernels_of(mmb_hip.LIB_PATH) if any(n in k[".name"] for n in ("3mmb5xattn", "3mmb8headnorm", "3mmb4ckpt"))]
+    assert len(ours) > 100
+    assert not [(k[".name"], k[".vgpr_spill_count"]) for k in ours if k[".vgpr_spill_count"]]
